@@ -1,5 +1,5 @@
 """ctypes binding of libhf_moe.so (the C ABI declared in include/hf_moe.h,
-include/hf_synth.h and include/hf_ingest.h).
+include/hf_synth.h, include/hf_ingest.h and include/hf_fp8.h).
 
 The library is built in-tree by hummingflight_b200/build.py. Loading fails
 loudly when it is missing: there is no CPU fallback.
@@ -20,6 +20,7 @@ HF_OK, HF_ERR_ARG, HF_ERR_CUDA, HF_ERR_NCCL, HF_ERR_TIMEOUT, HF_ERR_OOM, HF_ERR_
 HF_MEM_HOST, HF_MEM_DEVICE = 0, 1
 HF_BF16, HF_F32 = 0, 1
 HF_PATH_AUTO, HF_PATH_GEMV, HF_PATH_GEMM = 0, 1, 2
+HF_SCORE_SIGMOID, HF_SCORE_SOFTMAX = 0, 1
 
 
 class HfMoeConfig(ctypes.Structure):
@@ -34,6 +35,11 @@ class HfMoeConfig(ctypes.Structure):
 class HfMoeRouting(ctypes.Structure):
     _fields_ = [("topk_ids", c_vp), ("topk_weights", c_vp), ("margins", c_vp), ("counts", c_vp),
                 ("offsets", c_vp), ("perm", c_vp), ("slot_out", c_vp)]
+
+
+class HfRouteSpec(ctypes.Structure):
+    _fields_ = [("num_experts", c_int), ("top_k", c_int), ("score", c_int), ("n_group", c_int),
+                ("topk_group", c_int), ("group_top", c_int), ("scale", c_float), ("norm", c_int)]
 
 
 class HfStOptions(ctypes.Structure):
@@ -118,6 +124,18 @@ SIGNATURES = {
     "hf_st_upload": (c_int, [c_vp, c_int, c_vp, c_u64, c_int]),
     "hf_moe_load_safetensors": (c_int, [c_vp, c_int, c_int, ctypes.POINTER(ctypes.c_char_p), c_int,
                                         ctypes.POINTER(HfIngestStats)]),
+    "hf_route_workspace_size": (c_size, [c_int, ctypes.POINTER(HfRouteSpec)]),
+    "hf_route_logits": (c_int, [c_vp, c_int, c_vp, c_int, ctypes.POINTER(HfRouteSpec),
+                                ctypes.POINTER(HfMoeRouting), c_vp, c_size, c_vp]),
+    "hf_fp8_quantize": (c_int, [c_vp, c_int, ctypes.c_longlong, c_int, c_int, c_vp, c_vp, c_vp]),
+    "hf_fp8_gemm_workspace_size": (c_size, [c_int, c_int, c_int]),
+    "hf_fp8_gemm": (c_int, [c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_int, c_vp, c_size,
+                            c_vp]),
+    "hf_fp8_moe_experts_workspace_size": (c_size, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "hf_fp8_moe_experts": (c_int, [c_vp, c_vp, c_int, c_int, c_int, c_vp, c_int, ctypes.c_longlong,
+                                   c_int, c_int, ctypes.POINTER(HfMoeRouting), c_vp, c_vp, c_int,
+                                   c_vp, c_size, c_vp]),
+    "hf_fp8_status": (c_int, [c_vp, c_vp]),
     "hf_ingest_release_staging": (c_int, []),
     "hf_st_layer_shards": (c_int, [ctypes.c_char_p, c_int, c_vp, c_size, ctypes.POINTER(c_int)]),
 }

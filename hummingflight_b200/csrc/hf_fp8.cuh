@@ -1,0 +1,83 @@
+// hf_fp8.cuh -- e4m3 helpers and the interface between the FP8 host code and
+// its kernels.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "hf_fp8.h"
+#include "hf_internal.cuh"
+
+namespace hf {
+
+constexpr int kFp8Block = HF_FP8_BLOCK;
+
+// Four floats (|v| <= 448, or NaN) as e4m3, rounded to nearest even; a in the
+// lowest byte.
+__device__ __forceinline__ uint32_t pack4_e4m3(float a, float b, float c, float d) {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+    return uint32_t(lo) | (uint32_t(hi) << 16);
+}
+
+// Two e4m3 values as halves (exact: every e4m3 value is an FP16 one).
+__device__ __forceinline__ uint32_t unpack2_e4m3(uint16_t v) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(v));
+    return h;
+}
+
+// Scale of a block whose largest magnitude is m: the smallest power of two with
+// m <= 448 s (448 = 1.75 * 2^8), at least 2^-126; 1 for a block of zeros; NaN
+// for one that holds Inf or NaN. inv: 1 / s, a power of two as well.
+__device__ __forceinline__ float block_scale(float m, float& inv) {
+    const uint32_t b = __float_as_uint(m);
+    if (b >= 0x7f800000u) {
+        inv = __uint_as_float(0x7fc00000u);
+        return inv;
+    }
+    if (b == 0u) {
+        inv = 1.0f;
+        return 1.0f;
+    }
+    // biased exponent of s: that of m less 8, one more above 1.75
+    const int e = int(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+    const int se = e < 1 ? 1 : e;
+    inv = __uint_as_float(uint32_t(254 - se) << 23);
+    return __uint_as_float(uint32_t(se) << 23);
+}
+
+// 8 consecutive activations as fp32.
+template <bool XF32>
+__device__ __forceinline__ void load8(const void* x, long long i, float (&v)[8]) {
+    if constexpr (XF32) {
+        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + i);
+        const float4 a = __ldg(p), b = __ldg(p + 1);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+        unpack8(ld_nc_u4(static_cast<const uint16_t*>(x) + i), v);
+    }
+}
+
+// ------------------------------------------------------------------ products
+// Rows of e4m3 activations (positions) against weight rows. One group (offsets
+// null: all rows) or E groups: expert g multiplies positions [offsets[g],
+// offsets[g+1]).
+struct Fp8Args {
+    const uint8_t* xq;      // [rows x K]
+    const float* sx;        // [rows x ceil(K/128)]
+    const uint8_t* w;       // group g's matrix at w + g * w_stride, [N x K]
+    const float* sw;        // its scales at sw + g * sw_stride
+    long long w_stride, sw_stride;
+    const int32_t* offsets; // [G + 1] or null
+    int G, rows, N, K;
+    void* out;              // [rows x ld_out] bf16 or f32
+    int out_f32;
+    long long ld_out;
+    int* err;
+};
+hf_status launch_fp8_product(const Fp8Args& a, cudaStream_t st);
+
+}  // namespace hf

@@ -8,7 +8,8 @@ Names and argument meaning follow the reference:
   :93-96). ``moe_layer(layer, input, output)`` is the per-token, fp32-host
   entry with the reference's signature; ``forward`` runs T tokens on device.
 * :func:`gemv_bf16_f32` ~ ``gemv_bf16_f32`` (compute/cpu_kernels.h:16-17).
-* :func:`top_k_scores` ~ ``topKScores`` (compute/moe_router.h:29-57).
+* :func:`top_k_scores` ~ ``topKScores`` (compute/moe_router.h:29-57);
+  :func:`route_logits` is its general form (softmax, groups, permutation).
 
 Errors raise :class:`HfError` carrying the C status; nothing falls back to the
 CPU. Torch supplies device memory and the current CUDA stream only.
@@ -16,13 +17,14 @@ CPU. Torch supplies device memory and the current CUDA stream only.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import numpy as np
 
 from . import _lib
 from ._lib import (HF_BF16, HF_F32, HF_MEM_DEVICE, HF_MEM_HOST, HF_PATH_AUTO, HF_PATH_GEMM,
-                   HF_PATH_GEMV, HfError, HfMoeConfig, HfMoeRouting, call)
+                   HF_PATH_GEMV, HfError, HfMoeConfig, HfMoeRouting, HfRouteSpec, call)
 from .configs import GLM, LayerShape
 
 _PATHS = {"auto": HF_PATH_AUTO, "gemv": HF_PATH_GEMV, "gemm": HF_PATH_GEMM}
@@ -70,6 +72,51 @@ def _host_u16(a):
     if isinstance(a, np.ndarray):
         return np.ascontiguousarray(a).view(np.uint16)
     return a
+
+
+def check_tensor(name, t, dtypes, shape, device=None, rows=False):
+    """Raises ValueError unless `t` is a contiguous tensor of one of the dtypes
+    and the shape (rows: its rows may lie apart), on `device`."""
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name}: dtype {t.dtype} is not one of {', '.join(map(str, dtypes))}")
+    if t.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)} is not {tuple(shape)}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name}: on {t.device}, not on {device}")
+    if not t.is_contiguous() and not (rows and t.dim() == 2 and t.stride(1) == 1):
+        raise ValueError(f"{name}: must be contiguous")
+
+
+class on_device:
+    """The context a call on `device` runs in: makes the device current when it
+    is not, and gives the stream (the device's current one unless given)."""
+
+    def __init__(self, device, stream=None):
+        if device.type != "cuda":
+            raise ValueError(f"tensors must be on a CUDA device, not on {device}")
+        self._index, self._stream, self._back = device.index, stream, None
+
+    def __enter__(self):
+        torch = _torch()
+        if self._index is not None and torch.cuda.current_device() != self._index:
+            self._back = torch.cuda.current_device()
+            torch.cuda.set_device(self._index)
+        return (self._stream or torch.cuda.current_stream()).cuda_stream
+
+    def __exit__(self, *exc):
+        if self._back is not None:
+            _torch().cuda.set_device(self._back)
+
+
+def scratch(workspace, need: int, device):
+    """`workspace` if it has `need` bytes on the device, a new one if none is given."""
+    torch = _torch()
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    check_tensor("workspace", workspace, (torch.uint8,), workspace.shape, device)
+    if workspace.numel() < need:
+        raise ValueError(f"workspace: {workspace.numel()} bytes, {need} are needed")
+    return workspace
 
 
 class MoELayer:
@@ -325,6 +372,66 @@ def top_k_scores(scores, bias, top_k: int, routed_scaling_factor: float, norm_to
     return idx, w
 
 
+_SCORES = {"sigmoid": _lib.HF_SCORE_SIGMOID, "softmax": _lib.HF_SCORE_SOFTMAX}
+
+
+@functools.lru_cache(maxsize=64)
+def _route_spec(E, top_k, score, n_group, topk_group, group_top, scale, norm):
+    if score not in _SCORES:
+        raise ValueError(f"score must be one of {sorted(_SCORES)}")
+    return HfRouteSpec(E, top_k, _SCORES[score], n_group, topk_group, group_top, scale, int(norm))
+
+
+def route_workspace_size(T: int, num_experts: int, top_k: int) -> int:
+    """Bytes of scratch of route_logits over T tokens (0 up to 128 tokens)."""
+    spec = _route_spec(num_experts, top_k, "sigmoid", 1, 1, 1, 1.0, True)
+    return int(_lib.lib().hf_route_workspace_size(T, ctypes.byref(spec)))
+
+
+def route_logits(logits, bias=None, top_k: int = 8, score: str = "sigmoid", n_group: int = 1,
+                 topk_group: int = 1, group_top: int = 2, routed_scaling_factor: float = 1.0,
+                 norm_topk_prob: bool = True, out: Optional[dict] = None, workspace=None,
+                 stream=None):
+    """Routing from router logits [T x E] (device, bf16 or fp32): sigmoid or
+    softmax scores, + bias [E] fp32 for the choice, the best topk_group of
+    n_group expert groups (a group's score: the sum of its best group_top keys),
+    top_k, weights renormalised and scaled (hf_route_logits in include/hf_moe.h).
+
+    Returns device tensors topk_ids [T x k], topk_weights [T x k], counts [E+1],
+    offsets [E+2] and perm [T*k] (the shared group E is empty): what
+    hummingflight_b200.fp8.moe_experts takes. `out`: such a dict to write into."""
+    torch = _torch()
+    T, E = logits.shape
+    check_tensor("logits", logits, (torch.float32, torch.bfloat16), (T, E))
+    dev = logits.device
+    if bias is not None:
+        check_tensor("bias", bias, (torch.float32,), (E,), dev)
+    spec = _route_spec(E, top_k, score, n_group, topk_group, group_top, routed_scaling_factor,
+                       bool(norm_topk_prob))
+    i32 = torch.int32
+    if out is None:
+        out = dict(topk_ids=torch.empty((T, top_k), dtype=i32, device=dev),
+                   topk_weights=torch.empty((T, top_k), dtype=torch.float32, device=dev),
+                   counts=torch.empty(E + 1, dtype=i32, device=dev),
+                   offsets=torch.empty(E + 2, dtype=i32, device=dev),
+                   perm=torch.empty(T * top_k, dtype=i32, device=dev))
+    else:
+        check_tensor("topk_ids", out["topk_ids"], (i32,), (T, top_k), dev)
+        check_tensor("topk_weights", out["topk_weights"], (torch.float32,), (T, top_k), dev)
+        check_tensor("counts", out["counts"], (i32,), (E + 1,), dev)
+        check_tensor("offsets", out["offsets"], (i32,), (E + 2,), dev)
+        check_tensor("perm", out["perm"], (i32,), (T * top_k,), dev)
+    r = HfMoeRouting(out["topk_ids"].data_ptr(), out["topk_weights"].data_ptr(), None,
+                     out["counts"].data_ptr(), out["offsets"].data_ptr(), out["perm"].data_ptr(),
+                     None)
+    with on_device(dev, stream) as s:
+        need = int(_lib.lib().hf_route_workspace_size(T, spec))
+        workspace = scratch(workspace, need, dev)
+        call("hf_route_logits", logits.data_ptr(), _dtype_code(logits), _ptr(bias), T, spec, r,
+             _ptr(workspace), need, s)
+    return out
+
+
 def dense_mlp_workspace_size(T: int, H: int, I: int) -> int:
     return int(_lib.lib().hf_dense_mlp_workspace_size(T, H, I))
 
@@ -402,7 +509,8 @@ def synth_f32_uniform(dst, seed: int, layer: int, kind: int, expert: int, lo: fl
     return dst
 
 
-__all__ = ["MoELayer", "balanced_placement", "gemv_bf16_f32", "top_k_scores", "dense_mlp_forward",
+__all__ = ["MoELayer", "balanced_placement", "gemv_bf16_f32", "top_k_scores", "route_logits",
+           "route_workspace_size", "dense_mlp_forward",
            "dense_mlp_workspace_size", "dense_mlp_status", "dense_block_forward", "rmsnorm",
            "synth_bf16_normal",
            "synth_f32_uniform", "HfError", "HF_BF16", "HF_F32"]

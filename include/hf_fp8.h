@@ -1,0 +1,87 @@
+/*
+ * hf_fp8.h -- FP8 (e4m3) operators of the B200 MoE library: quantised rows, the
+ * block-scaled product, and the routed SwiGLU experts over FP8 weights.
+ *
+ * The reference keeps every weight in BF16; an FP8 checkpoint of the same model
+ * stores each weight matrix as e4m3 values with one fp32 scale per block of
+ * 128 x 128 (the value is q * scale), which halves the bytes a decode step
+ * streams and doubles the tensor cores' rate.
+ *
+ * Status, streams and errors as in hf_moe.h: argument errors return HF_ERR_ARG
+ * before anything is enqueued, calls are asynchronous on `stream`, pointers
+ * belong to the current device. e4m3 values are passed as uint8_t bits.
+ */
+#ifndef HF_FP8_H
+#define HF_FP8_H
+
+#include "hf_moe.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define HF_FP8_BLOCK 128 /* columns of a row, and rows and columns of a weight, per scale */
+
+/* Rows to e4m3 with one scale per 128 columns:
+ *   s[t, b] = the smallest power of two with max|x[t, 128b ..]| <= 448 s
+ *             (1 for a block of zeros, at least 2^-126)
+ *   q[t, j] = x[t, j] / s, rounded to nearest even
+ * Dividing by a power of two is exact, so each value is rounded once; e4m3 has
+ * the same relative precision at either end of a binade, so nothing is lost
+ * against a scale of max / 448. A block that holds Inf or NaN becomes NaN
+ * (scale and values): it is never saturated.
+ * x: device [T x K] BF16 or fp32, rows ldx elements apart, 16-byte aligned
+ * (pointer and pitch); q: device [T x K]; scales: device fp32 [T x ceil(K/128)].
+ * K a multiple of 16. */
+HF_API hf_status hf_fp8_quantize(const void* x, hf_dtype x_dtype, long long ldx, int T, int K,
+                                 uint8_t* q, float* scales, hf_stream stream);
+
+/* out = (xq * sx) (wq * sw)^T over T rows:
+ *   out[t, n] = sum_b sx[t, b] sw[n / 128, b] sum_{j in block b} xq[t, j] wq[n, j]
+ * with products and sums in fp32. xq: device e4m3 [T x K]; sx: fp32
+ * [T x ceil(K/128)] (any values, not only powers of two); wq: e4m3 [N x K];
+ * sw: fp32 [ceil(N/128) x ceil(K/128)]; out: [T x N] of out_dtype. K a multiple
+ * of 16, any T and N; xq, wq and the workspace 16-byte (workspace: 256-byte)
+ * aligned. The single-token form reads the weight once on the CUDA cores. */
+HF_API size_t hf_fp8_gemm_workspace_size(int T, int N, int K);
+HF_API hf_status hf_fp8_gemm(const uint8_t* xq, const float* sx, const uint8_t* wq, const float* sw,
+                             int T, int N, int K, void* out, hf_dtype out_dtype, void* workspace,
+                             size_t workspace_bytes, hf_stream stream);
+
+/* The routed SwiGLU experts over FP8 weights (expertFFNRaw and the combine,
+ * glm_forward.cpp:434-449, 555-556, 639-640, with quantised operands):
+ *   xq, sx  = quantise(x)
+ *   g, u    = xq Wg^T, xq Wu^T                    (of the token's experts)
+ *   mq, ms  = quantise(silu(g) * u)               (per 128 intermediate columns)
+ *   y_i     = mq Wd^T
+ *   out     = resid + sum_i w_i y_i               (rank order, fp32)
+ * experts: device e4m3, E blocks [gate I*H | up I*H | down H*I] (the layout of
+ * Scheduler::getExpertPtr, engine/scheduler.h:80-84); scales: device fp32, E
+ * blocks [gate ceil(I/128) x ceil(H/128) | up, the same | down ceil(H/128) x
+ * ceil(I/128)]. x: device [T x H] BF16 or fp32, rows ldx elements apart.
+ * routing: topk_weights [T x k], counts, offsets and perm as written by
+ * hf_route_logits or hf_moe_route for the same T and k (a shared segment behind
+ * the routed ones is left out; topk_ids is not read); offsets, perm entries out
+ * of range are skipped. resid: device [T x H] of out_dtype or NULL, may be out
+ * itself. out: device [T x H] of out_dtype; the expert outputs are kept in the
+ * same type until the combine. The shared expert, or a dense MLP, is the call
+ * with E = 1, k = 1 and the routed output as resid. H and I multiples of 16,
+ * k in 1..32, E in 1..1024, T * k below 2^31; pointers 16-byte aligned, the
+ * workspace 256-byte. A workspace serves any number of layers in stream order. */
+HF_API size_t hf_fp8_moe_experts_workspace_size(int T, int top_k, int E, int H, int I,
+                                                hf_dtype out_dtype);
+HF_API hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E, int H,
+                                    int I, const void* x, hf_dtype x_dtype, long long ldx, int T,
+                                    int top_k, const hf_moe_routing* routing, const void* resid,
+                                    void* out, hf_dtype out_dtype, void* workspace,
+                                    size_t workspace_bytes, hf_stream stream);
+
+/* Waits for `stream` and reports whether a bounded device wait of the last
+ * hf_fp8_gemm or hf_fp8_moe_experts on this workspace gave up (HF_ERR_TIMEOUT:
+ * that call's outputs are invalid). */
+HF_API hf_status hf_fp8_status(const void* workspace, hf_stream stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* HF_FP8_H */

@@ -303,6 +303,47 @@ HF_API hf_status hf_gemv_bf16_f32(const uint16_t* A, const float* x, float* y, i
 HF_API hf_status hf_topk_scores(const float* scores, int T, int E, const float* bias, int k, float scale,
                          int norm, int32_t* idx, float* weights, hf_stream stream);
 
+/* Routing from router logits: scores, a balance bias, expert groups, top-k,
+ * renormalised weights and the permutation into expert segments. The general
+ * form of hf_topk_scores, for routers that hf_moe_route does not cover; its
+ * outputs feed hf_fp8_moe_experts. No counterpart in the reference beyond
+ * topKScores (compute/moe_router.h:29-57), which is the case of a sigmoid with
+ * a bias, one group and k <= 8.
+ *
+ *   p_e   = 1 / (1 + exp(-l_e))  or  exp(l_e) / sum_f exp(l_f)
+ *   key_e = p_e + bias_e
+ * The experts form n_group groups of E / n_group consecutive ids. A group's
+ * score is the sum of its best min(group_top, E / n_group) keys; the topk_group
+ * best groups are kept and the experts of the others are out of the choice. The
+ * top_k experts of the highest keys follow in rank order, with the weights p_e,
+ * divided by their sum (rank order) when norm is set and that sum is positive,
+ * times scale. Ties (of keys and of groups) go to the lower id. Which expert
+ * ranks before which is decided as if in 64-bit arithmetic; without a bias the
+ * keys rank as the logits do. A NaN key ranks below every number. A softmax
+ * row of which every logit is -inf has p = 0; one with a NaN or +inf logit has
+ * NaN weights. */
+typedef enum hf_score { HF_SCORE_SIGMOID = 0, HF_SCORE_SOFTMAX = 1 } hf_score;
+typedef struct hf_route_spec {
+    int num_experts; /* E, 1..1024                                             */
+    int top_k;       /* 1..32, at most the experts of topk_group groups        */
+    int score;       /* hf_score                                               */
+    int n_group;     /* 1..32, divides E; 1 = no groups                        */
+    int topk_group;  /* 1..n_group                                             */
+    int group_top;   /* 1 (a group's best key) or 2 (the sum of its best two)  */
+    float scale;     /* routed_scaling_factor                                  */
+    int norm;        /* norm_topk_prob                                         */
+} hf_route_spec;
+HF_API size_t hf_route_workspace_size(int T, const hf_route_spec* spec);
+/* logits: device [T x E] fp32 or BF16; bias: device fp32 [E] or NULL. Writes
+ * routing->topk_ids [T x k], topk_weights [T x k], counts [E+1], offsets [E+2]
+ * and perm [T*k] (the shared group E is empty); all five are required, margins
+ * and slot_out must be NULL. T = 0 writes zero counts and offsets. workspace:
+ * device scratch of hf_route_workspace_size bytes (0 and NULL up to 128 tokens),
+ * 256-byte aligned, used in stream order only. Asynchronous on `stream`. */
+HF_API hf_status hf_route_logits(const void* logits, hf_dtype dtype, const float* bias, int T,
+                                 const hf_route_spec* spec, const hf_moe_routing* routing,
+                                 void* workspace, size_t workspace_bytes, hf_stream stream);
+
 /* Dense SwiGLU MLP (GLMForward::denseMlp, glm_forward.cpp:411-432; the
  * reference's per-token gemv_bf16_f32 x3 + fp32 SwiGLU) over T tokens.
  * gate, up: device BF16 [I x H]; down: device BF16 [H x I], three separate
