@@ -75,36 +75,6 @@ hf_status launch_quantize(const QuantArgs& a, bool f32, int dev, cudaStream_t st
     return HF_OK;
 }
 
-// mid = silu(g) * u of fp32 rows [g | u], quantised.
-__global__ void __launch_bounds__(256) k_swiglu_quantize(const float* gu, int rows, int I, int nb,
-                                                         uint8_t* q, float* s) {
-    const int sub = threadIdx.x & 15;
-    const unsigned half = 0xffffu << (threadIdx.x & 16);
-    const long long blocks = (long long)rows * nb;
-    for (long long i = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); i < blocks;
-         i += (long long)gridDim.x * 16) {
-        const int p = int(i / nb), b = int(i % nb);
-        const int c = b * kFp8Block + sub * 8;
-        float v[8] = {};
-        uint32_t m = 0;
-        if (c < I) {
-            const float* g = gu + size_t(p) * 2 * I + c;
-            for (int j = 0; j < 8; ++j) v[j] = swiglu(g[j], g[j + I]);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(half, m, o));
-        float inv;
-        const float sc = block_scale(__uint_as_float(m), inv);
-        if (c < I)
-            *reinterpret_cast<uint2*>(q + size_t(p) * I + c) =
-                make_uint2(pack4_e4m3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
-                           pack4_e4m3(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
-        if (sub == 0) s[size_t(p) * nb + b] = sc;
-    }
-}
-
 // ------------------------------------------------------------------ combine
 // out[t] = resid[t] + sum_i w[t, i] y[pos(t, i)], rank order, fp32: the
 // reference's separate multiply and add per pick.
@@ -156,7 +126,7 @@ __global__ void __launch_bounds__(256) k_fp8_combine(const void* y, const int32_
 
 // ------------------------------------------------------------------ workspaces
 struct ExpertsWs {
-    size_t err, pos, xq, sx, gu, mq, ms, y, total;
+    size_t pos, xq, sx, mq, ms, y, total;
 };
 
 ExpertsWs experts_ws(int T, int k, int H, int I, bool f32) {
@@ -171,7 +141,6 @@ ExpertsWs experts_ws(int T, int k, int H, int I, bool f32) {
     w.pos = take(n * 4);
     w.xq = take(n * H);
     w.sx = take(n * blocks128(H) * 4);
-    w.gu = take(n * 2 * I * 4);
     w.mq = take(n * I);
     w.ms = take(n * blocks128(I) * 4);
     w.y = take(n * H * (f32 ? 4 : 2));
@@ -240,6 +209,7 @@ hf_status hf_fp8_gemm(const uint8_t* xq, const float* sx, const uint8_t* wq, con
     a.xq = xq;
     a.sx = sx;
     a.w = wq;
+    a.a_rows = N;
     a.sw = sw;
     a.G = 1;
     a.rows = T;
@@ -247,9 +217,9 @@ hf_status hf_fp8_gemm(const uint8_t* xq, const float* sx, const uint8_t* wq, con
     a.K = K;
     a.out = out;
     a.out_f32 = out_dtype == HF_F32;
-    a.ld_out = N;
     a.err = static_cast<int*>(workspace);
-    return launch_fp8_product(a, as_cuda(stream));
+    a.clear_err = 1;
+    return launch_fp8_product(a, false, as_cuda(stream));
 }
 
 size_t hf_fp8_moe_experts_workspace_size(int T, int top_k, int E, int H, int I,
@@ -314,42 +284,36 @@ hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E,
     qa.err = reinterpret_cast<int*>(ws);
     HF_TRY(launch_quantize(qa, x_dtype == HF_F32, dev, st));
 
+    // gate/up: an expert's block is 3 I rows of H; down: 3 H rows of I
     Fp8Args a{};
     a.xq = qa.q;
     a.sx = qa.s;
     a.w = experts;
+    a.a_rows = 3ll * E * I;
+    a.a_stride = 3 * I;
     a.sw = scales;
-    a.w_stride = 3ll * I * H;
     a.sw_stride = 3ll * ib * hb;
+    a.sw_up = (long long)ib * hb;
     a.offsets = r->offsets;
     a.G = E;
     a.rows = n;
     a.N = I;
     a.K = H;
-    a.out_f32 = 1;
-    a.ld_out = 2 * I;
+    a.mid_q = ws + L.mq;
+    a.mid_s = reinterpret_cast<float*>(ws + L.ms);
     a.err = qa.err;
-    float* gu = reinterpret_cast<float*>(ws + L.gu);
-    a.out = gu;
-    HF_TRY(launch_fp8_product(a, st));
-    a.w += (long long)I * H;
-    a.sw += ib * hb;
-    a.out = gu + I;
-    HF_TRY(launch_fp8_product(a, st));
-    uint8_t* mq = ws + L.mq;
-    float* ms = reinterpret_cast<float*>(ws + L.ms);
-    k_swiglu_quantize<<<num_sms(dev) * 8, 256, 0, st>>>(gu, n, I, ib, mq, ms);
-    HF_CUDA(cudaGetLastError());
-    a.xq = mq;
-    a.sx = ms;
-    a.w = experts + 2ll * I * H;
+    HF_TRY(launch_fp8_product(a, true, st));
+    a.xq = a.mid_q;
+    a.sx = a.mid_s;
+    a.a_rows = 3ll * E * H;
+    a.a_stride = 3 * H;
+    a.a_base = 2 * H;
     a.sw = scales + 2ll * ib * hb;
     a.N = H;
     a.K = I;
     a.out = ws + L.y;
     a.out_f32 = f32;
-    a.ld_out = H;
-    HF_TRY(launch_fp8_product(a, st));
+    HF_TRY(launch_fp8_product(a, false, st));
     const int grid = num_sms(dev) * 8;
     if (f32)
         k_fp8_combine<true><<<grid, 256, 0, st>>>(ws + L.y, qa.pos, r->topk_weights, T, top_k, H,

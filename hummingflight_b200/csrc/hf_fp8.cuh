@@ -63,21 +63,29 @@ __device__ __forceinline__ void load8(const void* x, long long i, float (&v)[8])
 
 // ------------------------------------------------------------------ products
 // Rows of e4m3 activations (positions) against weight rows. One group (offsets
-// null: all rows) or E groups: expert g multiplies positions [offsets[g],
-// offsets[g+1]).
+// null: all rows) or G groups: group g multiplies positions [offsets[g],
+// offsets[g+1]) by its own matrix.
 struct Fp8Args {
     const uint8_t* xq;      // [rows x K]
     const float* sx;        // [rows x ceil(K/128)]
-    const uint8_t* w;       // group g's matrix at w + g * w_stride, [N x K]
-    const float* sw;        // its scales at sw + g * sw_stride
-    long long w_stride, sw_stride;
+    const uint8_t* w;       // view of K-wide rows: row n of group g at g * a_stride + a_base + n
+    long long a_rows;       // rows of the view
+    int a_stride, a_base;
+    const float* sw;        // scales [ceil(N/128) x ceil(K/128)] of group g at sw + g * sw_stride
+    long long sw_stride;
     const int32_t* offsets; // [G + 1] or null
     int G, rows, N, K;
-    void* out;              // [rows x ld_out] bf16 or f32
+    // product: out [rows x N], bf16 or f32
+    void* out;
     int out_f32;
-    long long ld_out;
-    int* err;
+    // gate/up: the up rows follow the N gate rows, their scales sw_up floats
+    // further; silu(g) * u quantised into mid_q [rows x N], mid_s [rows x ceil(N/128)]
+    long long sw_up;
+    uint8_t* mid_q;
+    float* mid_s;
+    int* err;               // error word: set when a bounded wait gives up
+    int clear_err;          // the first kernel of a call clears it
 };
-hf_status launch_fp8_product(const Fp8Args& a, cudaStream_t st);
+hf_status launch_fp8_product(const Fp8Args& a, bool glu, cudaStream_t st);
 
 }  // namespace hf

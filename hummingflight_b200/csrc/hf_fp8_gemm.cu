@@ -1,87 +1,497 @@
-// hf_fp8_gemm.cu -- the block-scaled product of e4m3 rows and e4m3 weight rows:
+// hf_fp8_gemm.cu -- the block-scaled product of e4m3 rows and e4m3 weight rows
+// on the tensor cores, for one weight matrix or one per expert segment:
 //   out[p, n] = sum_b sx[p, b] sw[n / 128, b] sum_{j in block b} xq[p, j] w[n, j]
 //
-// 64 positions x 64 weight rows per block, the operands widened to fp32 in
-// shared memory in steps of 32 columns, each block of 128 columns summed in
-// fp32 and then scaled.
+// Orientation: the MMA's M = 128 weight rows, N = positions (tokens), both
+// K-major, so the row-major weights feed the tensor cores as they lie and a
+// segment of any length costs MMA columns in steps of 16 only. A tile is two
+// blocks of 128 weight rows (gate and up rows of the same intermediate columns,
+// or 256 output columns) x up to BN positions.
+//
+// The scales change every 128 columns of K, so the tensor memory accumulator
+// holds one block of 128 (four kind::f8f6f4 steps of 32) and is then read back,
+// multiplied by the position's and the weight block's scale and added to fp32
+// registers, two values an instruction. Two or four accumulator buffers let
+// the MMAs of the next blocks run meanwhile.
+//
+// Warps: 0 TMA producer, 1 MMA issuer and TMEM owner, 2 scales (it writes the
+// products of both scales per position into a ring in shared memory), 4-11
+// accumulation and epilogue (two per TMEM lane quadrant, alternate 16-column
+// chunks). One CTA per SM, tiles dealt round-robin; the tiles that share weight
+// rows have adjacent ids, so their CTAs read those rows from L2 together.
+// Every wait is bounded (hf_sm100.cuh).
+//
+// The gate/up epilogue evaluates silu(g) * u, takes the maximum over the tile's
+// 128 intermediate columns (one block) per position and writes e4m3 values and
+// the scale, so the intermediate never leaves the SM in more than 8 bits.
+#include <algorithm>
+
 #include "hf_fp8.cuh"
+#include "hf_sm100.cuh"
 
 namespace hf {
 namespace {
 
-__global__ void __launch_bounds__(256) k_fp8_tile(Fp8Args a) {
-    if (a.err && !a.offsets && blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) *a.err = 0;
-    __shared__ float xs[32][65], ws[32][65];
-    const int g = blockIdx.y, kb = (a.K + kFp8Block - 1) / kFp8Block;
-    const int n0 = blockIdx.x * 64, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    int p0 = 0, p1 = a.rows;
-    if (a.offsets) {
-        p0 = max(0, a.offsets[g]);
-        p1 = min(a.rows, a.offsets[g + 1]);
+using namespace sm100;
+
+constexpr int kThreads = 384;
+constexpr int kAccWarps = 8;
+constexpr int kScaleSlots = 4;
+constexpr uint32_t kABytes = 128 * 128;  // 128 weight rows x 128 bytes
+constexpr uint64_t kWaitNs = 2000ull * 1000 * 1000;
+constexpr uint64_t kDrainNs = 500ull * 1000 * 1000;
+
+template <int BN>
+struct Cfg {
+    static constexpr int kStageBytes = 2 * kABytes + BN * 128;
+    static constexpr int kCols = 2 * BN;                     // TMEM columns of one buffer
+    static constexpr int kBufs = 512 / kCols >= 4 ? 4 : 2;
+    static constexpr uint32_t kTmemCols = kBufs * kCols;     // a power of two, 128..512
+    static constexpr int kBoxB = BN < 32 ? BN : 32;          // position rows of one TMA box
+    static constexpr int kScaleBytes = kScaleSlots * 2 * BN * 4;
+    static constexpr int kRedBytes = 5 * BN * 4;             // maxima of 4 quadrants, 1 / scale
+    static constexpr int kBarBytes = 512;
+    static constexpr int kFixed = kScaleBytes + kRedBytes + kBarBytes;
+    // the plan: offsets and tile prefix of up to 1024 segments
+    static constexpr int kStages0 = (227 * 1024 - 1024 - kFixed - 2 * 1025 * 4) / kStageBytes;
+    static constexpr int kStages = kStages0 > 8 ? 8 : kStages0;
+    static_assert((2 * kStages + 2 * kBufs + 2 * kScaleSlots + 1) * 8 + 8 <= kBarBytes, "barriers");
+    static_assert(kStageBytes % 1024 == 0 && kStages >= 3, "stages");
+    static int smem(int G) { return 1024 + kStages * kStageBytes + kFixed + 2 * (G + 1) * 4; }
+};
+
+struct Tile {
+    int row0, n;      // first position, positions
+    int m0;           // first weight row of block 0 in its matrix
+    int a0, a1;       // TMA rows of the two blocks
+    const float* s0;  // weight scales of the two blocks, [kb]
+    const float* s1;
+};
+
+__device__ __forceinline__ int find_segment(const int* pref, int G, int u) {
+    int lo = 0, hi = G - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (pref[mid] <= u) lo = mid;
+        else hi = mid - 1;
     }
-    const uint8_t* w = a.w + g * a.w_stride;
-    const float* sw = a.sw + g * a.sw_stride + size_t(n0 / kFp8Block) * kb;
-    for (int m0 = p0 + blockIdx.z * 64; m0 < p1; m0 += gridDim.z * 64) {
-        float acc[4][4] = {};
-        for (int b = 0; b < kb; ++b) {
-            float part[4][4] = {};
-            for (int c0 = b * kFp8Block; c0 < min(a.K, (b + 1) * kFp8Block); c0 += 32) {
-                __syncthreads();
-                for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-                    const int r = i / 16, c = (i % 16) * 2;
-                    uint32_t hx = 0, hw = 0;
-                    if (m0 + r < p1 && c0 + c < a.K)
-                        hx = unpack2_e4m3(*reinterpret_cast<const uint16_t*>(
-                            a.xq + size_t(m0 + r) * a.K + c0 + c));
-                    if (n0 + r < a.N && c0 + c < a.K)
-                        hw = unpack2_e4m3(*reinterpret_cast<const uint16_t*>(
-                            w + size_t(n0 + r) * a.K + c0 + c));
-                    const float2 fx = __half22float2(*reinterpret_cast<const __half2*>(&hx));
-                    const float2 fw = __half22float2(*reinterpret_cast<const __half2*>(&hw));
-                    xs[c][r] = fx.x;
-                    xs[c + 1][r] = fx.y;
-                    ws[c][r] = fw.x;
-                    ws[c + 1][r] = fw.y;
-                }
-                __syncthreads();
-#pragma unroll 8
-                for (int c = 0; c < 32; ++c)
+    return lo;
+}
+
+template <bool GLU, int BN>
+__device__ __forceinline__ void decode(const Fp8Args& a, const int* off, const int* pref, int KB,
+                                       int u, Tile& t) {
+    const int g = find_segment(pref, a.G, u);
+    const int c = off[g + 1] - off[g];
+    const int nt = (c + BN - 1) / BN, nw = (c + nt - 1) / nt;  // equal widths
+    const int local = u - pref[g], mi = local / nt, ni = local % nt;
+    t.row0 = off[g] + ni * nw;
+    t.n = min(nw, c - ni * nw);
+    t.m0 = mi * (GLU ? 128 : 256);
+    t.a0 = g * a.a_stride + a.a_base + t.m0;
+    t.a1 = t.a0 + (GLU ? a.N : 128);
+    const int rb = t.m0 / kFp8Block;
+    t.s0 = a.sw + g * a.sw_stride + size_t(rb) * KB;
+    // past the last row block of the matrix nothing is stored: any scale does
+    if (GLU) t.s1 = t.s0 + a.sw_up;
+    else t.s1 = t.m0 + 128 < a.N ? t.s0 + KB : t.s0;
+}
+
+__device__ __forceinline__ bool drain_wait(uint64_t* bar, uint32_t parity) {
+    const uint64_t dl = globaltimer() + kDrainNs;
+    while (!mbar_try_wait(bar, parity))
+        if (globaltimer() > dl) return false;
+    return true;
+}
+
+// acc (two floats) += d * s
+__device__ __forceinline__ void fma2(unsigned long long& acc, uint32_t d0, uint32_t d1,
+                                     unsigned long long s) {
+    asm("{\n\t.reg .b64 d;\n\tmov.b64 d, {%1, %2};\n\tfma.rn.f32x2 %0, d, %3, %0;\n\t}"
+        : "+l"(acc)
+        : "r"(d0), "r"(d1), "l"(s));
+}
+__device__ __forceinline__ float lo_f(unsigned long long v) {
+    return __uint_as_float(uint32_t(v));
+}
+__device__ __forceinline__ float hi_f(unsigned long long v) {
+    return __uint_as_float(uint32_t(v >> 32));
+}
+
+template <bool GLU, int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_fp8_mma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+              const Fp8Args a) {
+    using C = Cfg<BN>;
+    constexpr int S = C::kStages, NB = C::kBufs;
+    constexpr int CH = BN >= 32 ? BN / 32 : 1;  // 16-column chunks of one accumulation warp
+    extern __shared__ __align__(1024) uint8_t raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
+                                               ~uintptr_t(1023));
+    float* sc = reinterpret_cast<float*>(smem + S * C::kStageBytes);  // [slot][2][BN]
+    uint32_t* red = reinterpret_cast<uint32_t*>(sc + kScaleSlots * 2 * BN);  // [4][BN]
+    float* invs = reinterpret_cast<float*>(red + 4 * BN);                    // [BN]
+    uint64_t* full = reinterpret_cast<uint64_t*>(invs + BN);
+    uint64_t* empty = full + S;
+    uint64_t* tfull = empty + S;
+    uint64_t* tempty = tfull + NB;
+    uint64_t* sfull = tempty + NB;
+    uint64_t* sempty = sfull + kScaleSlots;
+    uint64_t* final_bar = sempty + kScaleSlots;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* off = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(full) + C::kBarBytes);  // [G+1]
+    int* pref = off + a.G + 1;                                                           // [G+1]
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int KB = (a.K + kFp8Block - 1) / kFp8Block;
+    const int MB = GLU ? (a.N + 127) / 128 : (a.N + 255) / 256;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < NB; ++b) {
+            mbar_init(&tfull[b], 1);
+            mbar_init(&tempty[b], kAccWarps);
+        }
+        for (int b = 0; b < kScaleSlots; ++b) {
+            mbar_init(&sfull[b], 1);
+            mbar_init(&sempty[b], kAccWarps);
+        }
+        mbar_init(final_bar, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+        if (a.clear_err && blockIdx.x == 0) *a.err = 0;
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, C::kTmemCols);
+        tmem_relinquish();
+    }
+    if (a.offsets) {
+        for (int g = threadIdx.x; g <= a.G; g += kThreads)
+            off[g] = min(max(a.offsets[g], 0), a.rows);
+    } else if (threadIdx.x == 0) {
+        off[0] = 0;
+        off[1] = a.rows;
+    }
+    __syncthreads();
+    if (warp == 2) {  // tile prefix
+        int run = 0;
+        for (int g0 = 0; g0 < a.G; g0 += 32) {
+            const int g = g0 + lane;
+            const int c = g < a.G ? max(off[g + 1] - off[g], 0) : 0;
+            int inc = (c + BN - 1) / BN * MB;
+            const int v = inc;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            part[i][j] = fmaf(xs[c][ty * 4 + i], ws[c][tx * 4 + j], part[i][j]);
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(~0u, inc, o);
+                if (lane >= o) inc += y;
             }
-            const float s = sw[b];
+            if (g < a.G) pref[g] = run + inc - v;
+            run += __shfl_sync(~0u, inc, 31);
+        }
+        if (lane == 0) pref[a.G] = run;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int total = pref[a.G];
+    const auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return mbar_wait_for(bar, parity, abort_flag, kWaitNs);
+    };
+
+    if (warp < 4) {
+        if constexpr (BN == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 0 && lane == 0) {
+            // ------------------------------------------------------ TMA producer
+            tma_prefetch_desc(&tmA);
+            tma_prefetch_desc(&tmB);
+            uint32_t it = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+                Tile t;
+                decode<GLU, BN>(a, off, pref, KB, u, t);
+                const int nb = (t.n + C::kBoxB - 1) / C::kBoxB;
+                for (int kb = 0; kb < KB; ++kb, ++it) {
+                    const uint32_t s = it % S;
+                    if (!wait(&empty[s], ((it / S) & 1) ^ 1)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* st = smem + s * C::kStageBytes;
+                    mbar_arrive_expect_tx(&full[s], 2 * kABytes + nb * C::kBoxB * 128);
+                    tma_load_2d(st, &tmA, &full[s], kb * 128, t.a0);
+                    tma_load_2d(st + kABytes, &tmA, &full[s], kb * 128, t.a1);
+                    for (int j = 0; j < nb; ++j)
+                        tma_load_2d(st + 2 * kABytes + j * C::kBoxB * 128, &tmB, &full[s], kb * 128,
+                                    t.row0 + j * C::kBoxB);
+                }
+            }
+            if (!ok) {  // every issued load lands before the CTA leaves
+                const uint32_t first = it > uint32_t(S) ? it - S : 0;
+                for (uint32_t i = first; i < it; ++i) drain_wait(&full[i % S], (i / S) & 1);
+            }
+        } else if (warp == 1 && lane == 0) {
+            // ------------------------------------------------------ MMA issuer
+            uint32_t it = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+                Tile t;
+                decode<GLU, BN>(a, off, pref, KB, u, t);
+                const uint32_t idesc = idesc_e4m3_m128(uint32_t(t.n + 15) & ~15u);
+                for (int kb = 0; kb < KB; ++kb, ++it) {
+                    const uint32_t s = it % S, b = it % NB;
+                    if (!wait(&tempty[b], ((it / NB) & 1) ^ 1) || !wait(&full[s], (it / S) & 1)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t st = smem_u32(smem + s * C::kStageBytes);
+                    const uint32_t d = tmem_base + b * C::kCols;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int p = m0 + ty * 4 + i;
-                const float si = p < p1 ? a.sx[size_t(p) * kb + b] * s : 0.0f;
+                    for (int ai = 0; ai < 2; ++ai)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(part[i][j], si, acc[i][j]);
+                        for (int kk = 0; kk < 4; ++kk)
+                            mma_f8(d + ai * BN, desc_k_sw128(st + ai * kABytes) + 2 * kk,
+                                   desc_k_sw128(st + 2 * kABytes) + 2 * kk, idesc, kk != 0);
+                    mma_commit(&empty[s]);
+                    mma_commit(&tfull[b]);
+                }
+            }
+            mma_commit(final_bar);  // completes once every MMA issued above is done
+            drain_wait(final_bar, 0);
+        } else if (warp == 2) {
+            // ------------------------------------------------------ scales
+            constexpr int PL = (BN + 31) / 32;
+            uint32_t it = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+                Tile t;
+                decode<GLU, BN>(a, off, pref, KB, u, t);
+                float x[PL], w0 = t.s0[0], w1 = t.s1[0];
+                const float* xp[PL];
+#pragma unroll
+                for (int j = 0; j < PL; ++j) {
+                    const int c = j * 32 + lane;
+                    xp[j] = c < t.n ? a.sx + size_t(t.row0 + c) * KB : nullptr;
+                    x[j] = xp[j] ? xp[j][0] : 0.0f;
+                }
+                for (int kb = 0; kb < KB; ++kb, ++it) {
+                    float xn[PL], v0 = 0.0f, v1 = 0.0f;  // the next block's, in flight
+                    const bool more = kb + 1 < KB;
+#pragma unroll
+                    for (int j = 0; j < PL; ++j) xn[j] = more && xp[j] ? xp[j][kb + 1] : 0.0f;
+                    if (more) {
+                        v0 = t.s0[kb + 1];
+                        v1 = t.s1[kb + 1];
+                    }
+                    const uint32_t q = it % kScaleSlots;
+                    if (!wait(&sempty[q], ((it / kScaleSlots) & 1) ^ 1)) {
+                        ok = false;
+                        break;
+                    }
+                    float* p = sc + q * 2 * BN;
+#pragma unroll
+                    for (int j = 0; j < PL; ++j) {
+                        const int c = j * 32 + lane;
+                        if (c < BN) {
+                            p[c] = x[j] * w0;
+                            p[BN + c] = x[j] * w1;
+                        }
+                        x[j] = xn[j];
+                    }
+                    w0 = v0;
+                    w1 = v1;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sfull[q]);
+                }
             }
         }
+    } else {
+        // ---------------------------------------------------------- accumulation
+        if constexpr (BN == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int q = warp & 3, h = (warp - 4) >> 2;
+        const int r = q * 32 + lane;
+        const uint32_t lanes = tmem_base + (uint32_t(q * 32) << 16);
+        uint32_t it = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+            Tile t;
+            decode<GLU, BN>(a, off, pref, KB, u, t);
+            // chunks of 16 columns at (2 i + h) * 16
+            const int nc = t.n > h * 16 ? (t.n - h * 16 + 31) / 32 : 0;
+            unsigned long long g[CH][8], v[CH][8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < CH; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int p = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-                if (p >= p1 || n >= a.N) continue;
-                const size_t o = size_t(p) * a.ld_out + n;
-                if (a.out_f32) static_cast<float*>(a.out)[o] = acc[i][j];
-                else static_cast<__nv_bfloat16*>(a.out)[o] = __float2bfloat16_rn(acc[i][j]);
+                for (int j = 0; j < 8; ++j) g[i][j] = v[i][j] = 0ull;
+            for (int kb = 0; kb < KB; ++kb, ++it) {
+                const uint32_t b = it % NB, sl = it % kScaleSlots;
+                if (!wait(&tfull[b], (it / NB) & 1) || !wait(&sfull[sl], (it / kScaleSlots) & 1)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t ta = lanes + b * C::kCols + h * 16;
+                const float* p = sc + sl * 2 * BN + h * 16;
+                uint32_t d0[2][16], d1[2][16];
+                if (nc > 0) {
+                    tmem_ld16(ta, d0[0]);
+                    tmem_ld16(ta + BN, d1[0]);
+                    tmem_ld_wait_regs(d0[0], d1[0]);
+                }
+#pragma unroll
+                for (int i = 0; i < CH; ++i) {
+                    if (i < nc) {
+                        if (i + 1 < nc) {
+                            tmem_ld16(ta + (i + 1) * 32, d0[(i + 1) & 1]);
+                            tmem_ld16(ta + BN + (i + 1) * 32, d1[(i + 1) & 1]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const ulonglong2 s0 =
+                                *reinterpret_cast<const ulonglong2*>(p + i * 32 + j * 4);
+                            const ulonglong2 s1 =
+                                *reinterpret_cast<const ulonglong2*>(p + BN + i * 32 + j * 4);
+                            const uint32_t(&e0)[16] = d0[i & 1];
+                            const uint32_t(&e1)[16] = d1[i & 1];
+                            fma2(g[i][2 * j], e0[4 * j], e0[4 * j + 1], s0.x);
+                            fma2(g[i][2 * j + 1], e0[4 * j + 2], e0[4 * j + 3], s0.y);
+                            fma2(v[i][2 * j], e1[4 * j], e1[4 * j + 1], s1.x);
+                            fma2(v[i][2 * j + 1], e1[4 * j + 2], e1[4 * j + 3], s1.y);
+                        }
+                        if (i + 1 < nc) tmem_ld_wait_regs(d0[(i + 1) & 1], d1[(i + 1) & 1]);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&tempty[b]);
+                    mbar_arrive(&sempty[sl]);
+                }
             }
+            if (!ok) break;
+            if constexpr (GLU) {
+                // silu(g) * u, and its maximum over the 128 rows per position
+                const bool rv = t.m0 + r < a.N;
+#pragma unroll
+                for (int i = 0; i < CH; ++i) {
+                    if (i < nc) {
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float m0 = rv ? swiglu_fast(lo_f(g[i][j]), lo_f(v[i][j])) : 0.0f;
+                            const float m1 = rv ? swiglu_fast(hi_f(g[i][j]), hi_f(v[i][j])) : 0.0f;
+                            const uint32_t b0 = __float_as_uint(m0), b1 = __float_as_uint(m1);
+                            g[i][j] = (unsigned long long)b0 | ((unsigned long long)b1 << 32);
+                            const uint32_t x0 = __reduce_max_sync(~0u, b0 & 0x7fffffffu);
+                            const uint32_t x1 = __reduce_max_sync(~0u, b1 & 0x7fffffffu);
+                            if (lane == 2 * j) top = x0;
+                            if (lane == 2 * j + 1) top = x1;
+                        }
+                        if (lane < 16) red[q * BN + (2 * i + h) * 16 + lane] = top;
+                    }
+                }
+                named_bar_sync(1 + h, 128);
+                for (int c = r; c < nc * 16; c += 128) {
+                    const int col = ((c >> 4) * 2 + h) * 16 + (c & 15);
+                    const uint32_t top = max(max(red[col], red[BN + col]),
+                                             max(red[2 * BN + col], red[3 * BN + col]));
+                    float inv;
+                    const float s = block_scale(__uint_as_float(top), inv);
+                    invs[col] = inv;
+                    if (col < t.n)
+                        a.mid_s[size_t(t.row0 + col) * ((a.N + 127) / 128) + t.m0 / 128] = s;
+                }
+                named_bar_sync(1 + h, 128);
+                if (rv) {
+#pragma unroll
+                    for (int i = 0; i < CH; ++i) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const int c = (2 * i + h) * 16 + 2 * j;
+                            if (i < nc && c < t.n) {
+                                uint16_t e;
+                                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
+                                    : "=h"(e)
+                                    : "f"(hi_f(g[i][j]) * invs[c + 1]), "f"(lo_f(g[i][j]) * invs[c]));
+                                uint8_t* o = a.mid_q + size_t(t.row0 + c) * a.N + t.m0 + r;
+                                o[0] = uint8_t(e);
+                                if (c + 1 < t.n) o[a.N] = uint8_t(e >> 8);
+                            }
+                        }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < CH; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int c = (2 * i + h) * 16 + 2 * j + e;
+                            if (i < nc && c < t.n) {
+                                const float y0 = e ? hi_f(g[i][j]) : lo_f(g[i][j]);
+                                const float y1 = e ? hi_f(v[i][j]) : lo_f(v[i][j]);
+                                const size_t o = size_t(t.row0 + c) * a.N + t.m0 + r;
+                                const bool r0 = t.m0 + r < a.N, r1 = t.m0 + 128 + r < a.N;
+                                if (a.out_f32) {
+                                    float* y = static_cast<float*>(a.out) + o;
+                                    if (r0) y[0] = y0;
+                                    if (r1) y[128] = y1;
+                                } else {
+                                    __nv_bfloat16* y = static_cast<__nv_bfloat16*>(a.out) + o;
+                                    if (r0) y[0] = __float2bfloat16_rn(y0);
+                                    if (r1) y[128] = __float2bfloat16_rn(y1);
+                                }
+                            }
+                        }
+            }
+        }
     }
+    __syncwarp();  // warps 0 and 1 ran their loops on one lane
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, C::kTmemCols);
+    }
+    if (threadIdx.x == 0 && *abort_flag) atomicOr(a.err, 1);
+}
+
+template <bool GLU, int BN>
+hf_status launch_one(const Fp8Args& a, cudaStream_t st) {
+    using C = Cfg<BN>;
+    int dev = 0;
+    HF_CUDA(cudaGetDevice(&dev));
+    const auto kern = k_fp8_mma<GLU, BN>;
+    const int smem = C::smem(a.G);
+    HF_CUDA(ensure_smem(reinterpret_cast<const void*>(kern), smem));
+    CUtensorMap A, B;
+    HF_TRY(make_map_u8(&A, a.w, a.K, a.a_rows, a.K, 128));
+    HF_TRY(make_map_u8(&B, a.xq, a.K, a.rows, a.K, C::kBoxB));
+    kern<<<num_sms(dev), kThreads, smem, st>>>(A, B, a);
+    HF_CUDA(cudaGetLastError());
+    return HF_OK;
 }
 
 }  // namespace
 
-hf_status launch_fp8_product(const Fp8Args& a, cudaStream_t st) {
-    const int mt = (a.rows + 63) / 64;
-    const dim3 grid(unsigned((a.N + 63) / 64), unsigned(a.G), unsigned(mt < 8 ? mt : 8));
-    k_fp8_tile<<<grid, 256, 0, st>>>(a);
-    HF_CUDA(cudaGetLastError());
-    return HF_OK;
+hf_status launch_fp8_product(const Fp8Args& a, bool glu, cudaStream_t st) {
+    const int avg = (a.rows + a.G - 1) / a.G;
+    if (glu) {
+        if (avg <= 16) return launch_one<true, 16>(a, st);
+        if (avg <= 32) return launch_one<true, 32>(a, st);
+        if (avg <= 64) return launch_one<true, 64>(a, st);
+        return launch_one<true, 128>(a, st);
+    }
+    if (avg <= 16) return launch_one<false, 16>(a, st);
+    if (avg <= 32) return launch_one<false, 32>(a, st);
+    if (avg <= 64) return launch_one<false, 64>(a, st);
+    return launch_one<false, 128>(a, st);
 }
 
 }  // namespace hf

@@ -898,5 +898,22 @@ hf_status make_map_bf16(CUtensorMap* m, const void* base, uint64_t cols, uint64_
     return HF_OK;
 }
 
+// 2-D byte view: `rows` rows of `cols` bytes, `pitch` bytes apart; box of 128
+// bytes x box_rows rows, 128-byte swizzle, OOB reads as zero.
+hf_status make_map_u8(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows,
+                      uint64_t pitch, uint32_t box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail(HF_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t dims[2] = {cols, rows};
+    const cuuint64_t strides[1] = {pitch};
+    const cuuint32_t box[2] = {128, box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides,
+                    box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(HF_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
+    return HF_OK;
+}
 
 }  // namespace hf

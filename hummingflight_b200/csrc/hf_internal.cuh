@@ -401,6 +401,8 @@ hf_status launch_gemm(const GemmMaps& m, const GemmArgs& a, int num_b, int grid,
 hf_status launch_gather(const GatherArgs& a, int x_f32, cudaStream_t st);
 hf_status make_map_bf16(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows,
                         uint64_t pitch, uint32_t box_rows);
+hf_status make_map_u8(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows,
+                      uint64_t pitch, uint32_t box_rows);
 
 // Device generator (hf_synth.cu).
 hf_status synth_bf16(uint16_t* dst, uint64_t n, uint64_t key, float scale, cudaStream_t st);
