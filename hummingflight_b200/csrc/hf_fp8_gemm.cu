@@ -78,6 +78,38 @@ __device__ __forceinline__ int find_segment(const int* pref, int G, int u) {
     return lo;
 }
 
+// Segment offsets (clipped to the rows) and the prefix of their tiles, into
+// shared memory; the whole block calls it.
+template <int BN>
+__device__ __forceinline__ void load_plan(const Fp8Args& a, int MB, int* off, int* pref) {
+    const int lane = threadIdx.x & 31;
+    if (a.offsets) {
+        for (int g = threadIdx.x; g <= a.G; g += blockDim.x)
+            off[g] = min(max(a.offsets[g], 0), a.rows);
+    } else if (threadIdx.x == 0) {
+        off[0] = 0;
+        off[1] = a.rows;
+    }
+    __syncthreads();
+    if (threadIdx.x >= 64 && threadIdx.x < 96) {  // warp 2
+        int run = 0;
+        for (int g0 = 0; g0 < a.G; g0 += 32) {
+            const int g = g0 + lane;
+            const int c = g < a.G ? max(off[g + 1] - off[g], 0) : 0;
+            int inc = (c + BN - 1) / BN * MB;
+            const int v = inc;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(~0u, inc, o);
+                if (lane >= o) inc += y;
+            }
+            if (g < a.G) pref[g] = run + inc - v;
+            run += __shfl_sync(~0u, inc, 31);
+        }
+        if (lane == 0) pref[a.G] = run;
+    }
+}
+
 template <bool GLU, int BN>
 __device__ __forceinline__ void decode(const Fp8Args& a, const int* off, const int* pref, int KB,
                                        int u, Tile& t) {
@@ -110,6 +142,11 @@ __device__ __forceinline__ void fma2(unsigned long long& acc, uint32_t d0, uint3
     asm("{\n\t.reg .b64 d;\n\tmov.b64 d, {%1, %2};\n\tfma.rn.f32x2 %0, d, %3, %0;\n\t}"
         : "+l"(acc)
         : "r"(d0), "r"(d1), "l"(s));
+}
+__device__ __forceinline__ unsigned long long pair_of(float v) {
+    unsigned long long p;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(p) : "f"(v));
+    return p;
 }
 __device__ __forceinline__ float lo_f(unsigned long long v) {
     return __uint_as_float(uint32_t(v));
@@ -169,31 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_alloc(tmem_slot, C::kTmemCols);
         tmem_relinquish();
     }
-    if (a.offsets) {
-        for (int g = threadIdx.x; g <= a.G; g += kThreads)
-            off[g] = min(max(a.offsets[g], 0), a.rows);
-    } else if (threadIdx.x == 0) {
-        off[0] = 0;
-        off[1] = a.rows;
-    }
-    __syncthreads();
-    if (warp == 2) {  // tile prefix
-        int run = 0;
-        for (int g0 = 0; g0 < a.G; g0 += 32) {
-            const int g = g0 + lane;
-            const int c = g < a.G ? max(off[g + 1] - off[g], 0) : 0;
-            int inc = (c + BN - 1) / BN * MB;
-            const int v = inc;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(~0u, inc, o);
-                if (lane >= o) inc += y;
-            }
-            if (g < a.G) pref[g] = run + inc - v;
-            run += __shfl_sync(~0u, inc, 31);
-        }
-        if (lane == 0) pref[a.G] = run;
-    }
+    load_plan<BN>(a, MB, off, pref);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -204,7 +217,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     if (warp < 4) {
-        if constexpr (BN == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 0 && lane == 0) {
             // ------------------------------------------------------ TMA producer
             tma_prefetch_desc(&tmA);
@@ -312,7 +324,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         // ---------------------------------------------------------- accumulation
-        if constexpr (BN == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int q = warp & 3, h = (warp - 4) >> 2;
         const int r = q * 32 + lane;
         const uint32_t lanes = tmem_base + (uint32_t(q * 32) << 16);
@@ -462,6 +473,296 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0 && *abort_flag) atomicOr(a.err, 1);
 }
 
+// 32 consecutive outputs of a position: 16-byte stores where the row starts on
+// a 16-byte boundary and all 32 exist.
+__device__ __forceinline__ void store32(const Fp8Args& a, size_t row, int col,
+                                        const unsigned long long (&v)[16]) {
+    const size_t o = row * a.N + col;
+    if (a.out_f32) {
+        float* y = static_cast<float*>(a.out) + o;
+        if (col + 32 <= a.N && (reinterpret_cast<uintptr_t>(y) & 15) == 0) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 2)
+                *reinterpret_cast<float4*>(y + 2 * j) =
+                    make_float4(lo_f(v[j]), hi_f(v[j]), lo_f(v[j + 1]), hi_f(v[j + 1]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (col + j < a.N) y[j] = j & 1 ? hi_f(v[j >> 1]) : lo_f(v[j >> 1]);
+        }
+    } else {
+        uint16_t* y = static_cast<uint16_t*>(a.out) + o;
+        uint32_t p[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(lo_f(v[j]), hi_f(v[j]));
+            p[j] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        if (col + 32 <= a.N && (reinterpret_cast<uintptr_t>(y) & 15) == 0) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+                *reinterpret_cast<uint4*>(y + 2 * j) = make_uint4(p[j], p[j + 1], p[j + 2], p[j + 3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (col + j < a.N) y[j] = uint16_t(j & 1 ? p[j >> 1] >> 16 : p[j >> 1]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ long segments
+// M = 128 positions, N = 256 weight rows (128 gate and 128 up rows, or 256
+// output columns): an accumulator lane is one position, so a thread needs two
+// scales per block, its position's times that of either weight block, and no
+// table. 64 columns of both blocks per thread.
+// warps 0 and 1 as above, 2 and 3 idle, 4-11 accumulation with the registers that the
+// first four give up: 4 * 32 * 80 + 8 * 32 * 208 of the launch's 384 * 168
+constexpr int kWideThreads = 384;
+constexpr int kWideStages = 4;
+constexpr int kWideStage = 3 * kABytes;  // 128 positions, 2 x 128 weight rows
+constexpr int kWideBar = 256;
+constexpr int kWideBox = 64;             // position rows of one TMA box
+inline int wide_smem(int G) {
+    return 1024 + kWideStages * kWideStage + kWideBar + 2 * 128 * 4 + 2 * (G + 1) * 4;
+}
+
+template <bool GLU>
+__global__ void __launch_bounds__(kWideThreads, 1)
+    k_fp8_wide(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+               const Fp8Args a) {
+    constexpr int S = kWideStages;
+    extern __shared__ __align__(1024) uint8_t raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
+                                               ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * kWideStage);
+    uint64_t* empty = full + S;
+    uint64_t* tfull = empty + S;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* final_bar = tempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    uint32_t* red = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(full) + kWideBar);
+    int* off = reinterpret_cast<int*>(red + 2 * 128);
+    int* pref = off + a.G + 1;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int KB = (a.K + kFp8Block - 1) / kFp8Block;
+    const int MB = GLU ? (a.N + 127) / 128 : (a.N + 255) / 256;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&tfull[b], 1);
+            mbar_init(&tempty[b], kAccWarps);
+        }
+        mbar_init(final_bar, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+        if (a.clear_err && blockIdx.x == 0) *a.err = 0;
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    load_plan<128>(a, MB, off, pref);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int total = pref[a.G];
+    const auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return mbar_wait_for(bar, parity, abort_flag, kWaitNs);
+    };
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (warp == 0 && lane == 0) {
+            // ---------------------------------------------------------- TMA producer
+            tma_prefetch_desc(&tmA);
+            tma_prefetch_desc(&tmB);
+            uint32_t it = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+                Tile t;
+                decode<GLU, 128>(a, off, pref, KB, u, t);
+                const int nb = (t.n + kWideBox - 1) / kWideBox;
+                for (int kb = 0; kb < KB; ++kb, ++it) {
+                    const uint32_t s = it % S;
+                    if (!wait(&empty[s], ((it / S) & 1) ^ 1)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* st = smem + s * kWideStage;
+                    mbar_arrive_expect_tx(&full[s], 2 * kABytes + nb * kWideBox * 128);
+                    for (int j = 0; j < nb; ++j)
+                        tma_load_2d(st + j * kWideBox * 128, &tmB, &full[s], kb * 128,
+                                    t.row0 + j * kWideBox);
+                    tma_load_2d(st + kABytes, &tmA, &full[s], kb * 128, t.a0);
+                    tma_load_2d(st + 2 * kABytes, &tmA, &full[s], kb * 128, t.a1);
+                }
+            }
+            if (!ok) {  // every issued load lands before the CTA leaves
+                const uint32_t first = it > uint32_t(S) ? it - S : 0;
+                for (uint32_t i = first; i < it; ++i) drain_wait(&full[i % S], (i / S) & 1);
+            }
+        } else if (warp == 1 && lane == 0) {
+            // ---------------------------------------------------------- MMA issuer
+            const uint32_t idesc = idesc_e4m3_m128(256);
+            uint32_t it = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+                for (int kb = 0; kb < KB; ++kb, ++it) {
+                    const uint32_t s = it % S, b = it & 1;
+                    if (!wait(&tempty[b], ((it >> 1) & 1) ^ 1) || !wait(&full[s], (it / S) & 1)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t st = smem_u32(smem + s * kWideStage);
+    #pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        mma_f8(tmem_base + b * 256, desc_k_sw128(st) + 2 * kk,
+                               desc_k_sw128(st + kABytes) + 2 * kk, idesc, kk != 0);
+                    mma_commit(&empty[s]);
+                    mma_commit(&tfull[b]);
+                }
+            }
+            mma_commit(final_bar);  // completes once every MMA issued above is done
+            drain_wait(final_bar, 0);
+        }
+    } else {
+        // ---------------------------------------------------------- accumulation
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int q = warp & 3, h = (warp - 4) >> 2;
+        const int r = q * 32 + lane;
+        const uint32_t lanes = tmem_base + (uint32_t(q * 32) << 16) + h * 64;
+        uint32_t it = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+            Tile t;
+            decode<GLU, 128>(a, off, pref, KB, u, t);
+            const bool work = q * 32 < t.n, rv = r < t.n;
+            const float* xp = a.sx + size_t(t.row0 + (rv ? r : 0)) * KB;
+            unsigned long long acc[4][16];  // columns h*64 + 32 c of block 0 (c < 2) and 1
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) acc[c][j] = 0ull;
+            float x = xp[0], w0 = t.s0[0], w1 = t.s1[0];
+            for (int kb = 0; kb < KB; ++kb, ++it) {
+                const uint32_t b = it & 1;
+                const float y0 = x * w0, y1 = x * w1;
+                if (kb + 1 < KB) {  // the next block's scales, in flight
+                    x = xp[kb + 1];
+                    w0 = t.s0[kb + 1];
+                    w1 = t.s1[kb + 1];
+                }
+                if (!wait(&tfull[b], (it >> 1) & 1)) {
+                    ok = false;
+                    break;
+                }
+                if (work) {
+                    tc_fence_after();
+                    const uint32_t ta = lanes + b * 256;
+                    const unsigned long long s0 = pair_of(y0), s1 = pair_of(y1);
+                    uint32_t d[2][16];
+                    tmem_ld16(ta, d[0]);
+                    tmem_ld_wait_reg16(d[0]);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        if (c < 7) tmem_ld16(ta + ((c + 1) >> 2) * 128 + ((c + 1) & 3) * 16, d[(c + 1) & 1]);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            fma2(acc[c >> 1][(c & 1) * 8 + j], d[c & 1][2 * j], d[c & 1][2 * j + 1],
+                                 c < 4 ? s0 : s1);
+                        if (c < 7) tmem_ld_wait_reg16(d[(c + 1) & 1]);
+                    }
+                    tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&tempty[b]);
+            }
+            if (!ok) break;
+            const size_t row = size_t(t.row0 + r);
+            if constexpr (GLU) {
+                // silu(g) * u of this thread's 64 columns; the other 64 of the block
+                // are the other half's warp's
+                const int left = a.N - t.m0 - h * 64;  // columns before the end
+                uint32_t top = 0;
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const int col = c * 32 + 2 * j;
+                        float m0 = 0.0f, m1 = 0.0f;
+                        if (col < left) {  // N is a multiple of 16
+                            m0 = swiglu_fast(lo_f(acc[c][j]), lo_f(acc[c + 2][j]));
+                            m1 = swiglu_fast(hi_f(acc[c][j]), hi_f(acc[c + 2][j]));
+                        }
+                        const uint32_t b0 = __float_as_uint(m0), b1 = __float_as_uint(m1);
+                        top = max(top, max(b0 & 0x7fffffffu, b1 & 0x7fffffffu));
+                        acc[c][j] = (unsigned long long)b0 | ((unsigned long long)b1 << 32);
+                    }
+                red[h * 128 + r] = top;
+                named_bar_sync(1 + q, 64);
+                top = max(top, red[(h ^ 1) * 128 + r]);
+                named_bar_sync(1 + q, 64);  // both have read before the next tile writes
+                float inv;
+                const float s = block_scale(__uint_as_float(top), inv);
+                if (rv) {
+                    if (h == 0) a.mid_s[row * ((a.N + 127) / 128) + t.m0 / 128] = s;
+                    uint8_t* o = a.mid_q + row * a.N + t.m0 + h * 64;
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int j = (v & 1) * 8 + e * 2;
+                            const unsigned long long p0 = acc[v >> 1][j], p1 = acc[v >> 1][j + 1];
+                            w[e] = pack4_e4m3(lo_f(p0) * inv, hi_f(p0) * inv, lo_f(p1) * inv,
+                                              hi_f(p1) * inv);
+                        }
+                        if (v * 16 < left)
+                            *reinterpret_cast<uint4*>(o + v * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            } else if (rv) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int col = t.m0 + (c >> 1) * 128 + h * 64 + (c & 1) * 32;
+                    store32(a, row, col, acc[c]);
+                }
+            }
+        }
+    }
+    __syncwarp();  // warps 0 and 1 ran their loops on one lane
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+    if (threadIdx.x == 0 && *abort_flag) atomicOr(a.err, 1);
+}
+
+template <bool GLU>
+hf_status launch_wide(const Fp8Args& a, cudaStream_t st) {
+    int dev = 0;
+    HF_CUDA(cudaGetDevice(&dev));
+    const auto kern = k_fp8_wide<GLU>;
+    const int smem = wide_smem(a.G);
+    HF_CUDA(ensure_smem(reinterpret_cast<const void*>(kern), smem));
+    CUtensorMap A, B;
+    HF_TRY(make_map_u8(&A, a.w, a.K, a.a_rows, a.K, 128));
+    HF_TRY(make_map_u8(&B, a.xq, a.K, a.rows, a.K, kWideBox));
+    kern<<<num_sms(dev), kWideThreads, smem, st>>>(A, B, a);
+    HF_CUDA(cudaGetLastError());
+    return HF_OK;
+}
+
 template <bool GLU, int BN>
 hf_status launch_one(const Fp8Args& a, cudaStream_t st) {
     using C = Cfg<BN>;
@@ -482,16 +783,10 @@ hf_status launch_one(const Fp8Args& a, cudaStream_t st) {
 
 hf_status launch_fp8_product(const Fp8Args& a, bool glu, cudaStream_t st) {
     const int avg = (a.rows + a.G - 1) / a.G;
-    if (glu) {
-        if (avg <= 16) return launch_one<true, 16>(a, st);
-        if (avg <= 32) return launch_one<true, 32>(a, st);
-        if (avg <= 64) return launch_one<true, 64>(a, st);
-        return launch_one<true, 128>(a, st);
-    }
-    if (avg <= 16) return launch_one<false, 16>(a, st);
-    if (avg <= 32) return launch_one<false, 32>(a, st);
-    if (avg <= 64) return launch_one<false, 64>(a, st);
-    return launch_one<false, 128>(a, st);
+    if (avg > 64) return glu ? launch_wide<true>(a, st) : launch_wide<false>(a, st);
+    if (avg > 32) return glu ? launch_one<true, 64>(a, st) : launch_one<false, 64>(a, st);
+    if (avg > 16) return glu ? launch_one<true, 32>(a, st) : launch_one<false, 32>(a, st);
+    return glu ? launch_one<true, 16>(a, st) : launch_one<false, 16>(a, st);
 }
 
 }  // namespace hf

@@ -201,6 +201,14 @@ __device__ __forceinline__ void tmem_ld_wait_regs(uint32_t (&a)[16], uint32_t (&
                  :
                  : "memory");
 }
+__device__ __forceinline__ void tmem_ld_wait_reg16(uint32_t (&a)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]),
+                   "+r"(a[6]), "+r"(a[7]), "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]),
+                   "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15])
+                 :
+                 : "memory");
+}
 
 // Shared-memory matrix descriptor of a K-major tile stored as 128-byte rows
 // with the 128-byte swizzle (what a TMA box of 64 bf16 x rows with
