@@ -25,6 +25,8 @@
 // 128 intermediate columns (one block) per position and writes e4m3 values and
 // the scale, so the intermediate never leaves the SM in more than 8 bits.
 #include <algorithm>
+#include <map>
+#include <mutex>
 
 #include "hf_fp8.cuh"
 #include "hf_sm100.cuh"
@@ -55,7 +57,7 @@ struct Cfg {
     // the plan: offsets and tile prefix of up to 1024 segments
     static constexpr int kStages0 = (227 * 1024 - 1024 - kFixed - 2 * 1025 * 4) / kStageBytes;
     static constexpr int kStages = kStages0 > 8 ? 8 : kStages0;
-    static_assert((2 * kStages + 2 * kBufs + 2 * kScaleSlots + 1) * 8 + 8 <= kBarBytes, "barriers");
+    static_assert((2 * kStages + kBufs + 2 * kScaleSlots + 1) * 8 + 8 <= kBarBytes, "barriers");
     static_assert(kStageBytes % 1024 == 0 && kStages >= 3, "stages");
     static int smem(int G) { return 1024 + kStages * kStageBytes + kFixed + 2 * (G + 1) * 4; }
 };
@@ -169,9 +171,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t* red = reinterpret_cast<uint32_t*>(sc + kScaleSlots * 2 * BN);  // [4][BN]
     float* invs = reinterpret_cast<float*>(red + 4 * BN);                    // [BN]
     uint64_t* full = reinterpret_cast<uint64_t*>(invs + BN);
-    uint64_t* empty = full + S;
-    uint64_t* tfull = empty + S;
-    uint64_t* tempty = tfull + NB;
+    uint64_t* done = full + S;      // a block's MMAs: its stage is free, its sums are ready
+    uint64_t* tempty = done + S;
     uint64_t* sfull = tempty + NB;
     uint64_t* sempty = sfull + kScaleSlots;
     uint64_t* final_bar = sempty + kScaleSlots;
@@ -187,12 +188,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
             mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
+            mbar_init(&done[s], 1);
         }
-        for (int b = 0; b < NB; ++b) {
-            mbar_init(&tfull[b], 1);
-            mbar_init(&tempty[b], kAccWarps);
-        }
+        for (int b = 0; b < NB; ++b) mbar_init(&tempty[b], kAccWarps);
         for (int b = 0; b < kScaleSlots; ++b) {
             mbar_init(&sfull[b], 1);
             mbar_init(&sempty[b], kAccWarps);
@@ -217,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     if (warp < 4) {
-        if (warp == 0 && lane == 0) {
+        if (warp == 0) {
             // ------------------------------------------------------ TMA producer
             tma_prefetch_desc(&tmA);
             tma_prefetch_desc(&tmB);
@@ -229,24 +227,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int nb = (t.n + C::kBoxB - 1) / C::kBoxB;
                 for (int kb = 0; kb < KB; ++kb, ++it) {
                     const uint32_t s = it % S;
-                    if (!wait(&empty[s], ((it / S) & 1) ^ 1)) {
+                    if (!wait(&done[s], ((it / S) & 1) ^ 1)) {
                         ok = false;
                         break;
                     }
-                    uint8_t* st = smem + s * C::kStageBytes;
-                    mbar_arrive_expect_tx(&full[s], 2 * kABytes + nb * C::kBoxB * 128);
-                    tma_load_2d(st, &tmA, &full[s], kb * 128, t.a0);
-                    tma_load_2d(st + kABytes, &tmA, &full[s], kb * 128, t.a1);
-                    for (int j = 0; j < nb; ++j)
-                        tma_load_2d(st + 2 * kABytes + j * C::kBoxB * 128, &tmB, &full[s], kb * 128,
-                                    t.row0 + j * C::kBoxB);
+                    if (elect_one()) {
+                        uint8_t* st = smem + s * C::kStageBytes;
+                        mbar_arrive_expect_tx(&full[s], 2 * kABytes + nb * C::kBoxB * 128);
+                        tma_load_2d(st, &tmA, &full[s], kb * 128, t.a0);
+                        tma_load_2d(st + kABytes, &tmA, &full[s], kb * 128, t.a1);
+                        for (int j = 0; j < nb; ++j)
+                            tma_load_2d(st + 2 * kABytes + j * C::kBoxB * 128, &tmB, &full[s],
+                                        kb * 128, t.row0 + j * C::kBoxB);
+                    }
+                    __syncwarp();
                 }
             }
             if (!ok) {  // every issued load lands before the CTA leaves
                 const uint32_t first = it > uint32_t(S) ? it - S : 0;
                 for (uint32_t i = first; i < it; ++i) drain_wait(&full[i % S], (i / S) & 1);
             }
-        } else if (warp == 1 && lane == 0) {
+        } else if (warp == 1) {
             // ------------------------------------------------------ MMA issuer
             uint32_t it = 0;
             bool ok = true;
@@ -261,19 +262,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t st = smem_u32(smem + s * C::kStageBytes);
-                    const uint32_t d = tmem_base + b * C::kCols;
+                    if (elect_one()) {
+                        const uint32_t st = smem_u32(smem + s * C::kStageBytes);
+                        const uint32_t d = tmem_base + b * C::kCols;
 #pragma unroll
-                    for (int ai = 0; ai < 2; ++ai)
+                        for (int ai = 0; ai < 2; ++ai)
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            mma_f8(d + ai * BN, desc_k_sw128(st + ai * kABytes) + 2 * kk,
-                                   desc_k_sw128(st + 2 * kABytes) + 2 * kk, idesc, kk != 0);
-                    mma_commit(&empty[s]);
-                    mma_commit(&tfull[b]);
+                            for (int kk = 0; kk < 4; ++kk)
+                                mma_f8(d + ai * BN, desc_k_sw128(st + ai * kABytes) + 2 * kk,
+                                       desc_k_sw128(st + 2 * kABytes) + 2 * kk, idesc, kk != 0);
+                        mma_commit(&done[s]);
+                    }
+                    __syncwarp();
                 }
             }
-            mma_commit(final_bar);  // completes once every MMA issued above is done
+            if (elect_one()) mma_commit(final_bar);  // once every MMA issued above is done
+            __syncwarp();
             drain_wait(final_bar, 0);
         } else if (warp == 2) {
             // ------------------------------------------------------ scales
@@ -341,7 +345,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int j = 0; j < 8; ++j) g[i][j] = v[i][j] = 0ull;
             for (int kb = 0; kb < KB; ++kb, ++it) {
                 const uint32_t b = it % NB, sl = it % kScaleSlots;
-                if (!wait(&tfull[b], (it / NB) & 1) || !wait(&sfull[sl], (it / kScaleSlots) & 1)) {
+                if (!wait(&done[it % S], (it / S) & 1) ||
+                    !wait(&sfull[sl], (it / kScaleSlots) & 1)) {
                     ok = false;
                     break;
                 }
@@ -463,7 +468,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     }
-    __syncwarp();  // warps 0 and 1 ran their loops on one lane
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
@@ -473,90 +477,146 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0 && *abort_flag) atomicOr(a.err, 1);
 }
 
-// 32 consecutive outputs of a position: 16-byte stores where the row starts on
-// a 16-byte boundary and all 32 exist.
-__device__ __forceinline__ void store32(const Fp8Args& a, size_t row, int col,
-                                        const unsigned long long (&v)[16]) {
-    const size_t o = row * a.N + col;
-    if (a.out_f32) {
-        float* y = static_cast<float*>(a.out) + o;
-        if (col + 32 <= a.N && (reinterpret_cast<uintptr_t>(y) & 15) == 0) {
+// Four lanes' rows of four 16-byte chunks, transposed: lane l (of four) gets
+// chunk l of each of the four rows, c[j] from row j.
+__device__ __forceinline__ void transpose4(uint4 (&c)[4]) {
+    const int l = threadIdx.x & 3;
+    uint32_t(&w)[16] = *reinterpret_cast<uint32_t(*)[16]>(&c[0]);
+    // two butterfly steps: exchange chunk bit b with lane bit b
 #pragma unroll
-            for (int j = 0; j < 16; j += 2)
-                *reinterpret_cast<float4*>(y + 2 * j) =
-                    make_float4(lo_f(v[j]), hi_f(v[j]), lo_f(v[j + 1]), hi_f(v[j + 1]));
-        } else {
+    for (int b = 1; b <= 2; b <<= 1) {
+        const bool hi = l & b;
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (col + j < a.N) y[j] = j & 1 ? hi_f(v[j >> 1]) : lo_f(v[j >> 1]);
-        }
-    } else {
-        uint16_t* y = static_cast<uint16_t*>(a.out) + o;
-        uint32_t p[16];
+        for (int j = 0; j < 4; ++j) {
+            if (j & b) continue;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(lo_f(v[j]), hi_f(v[j]));
-            p[j] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-        if (col + 32 <= a.N && (reinterpret_cast<uintptr_t>(y) & 15) == 0) {
-#pragma unroll
-            for (int j = 0; j < 16; j += 4)
-                *reinterpret_cast<uint4*>(y + 2 * j) = make_uint4(p[j], p[j + 1], p[j + 2], p[j + 3]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (col + j < a.N) y[j] = uint16_t(j & 1 ? p[j >> 1] >> 16 : p[j >> 1]);
+            for (int k = 0; k < 4; ++k) {
+                uint32_t& lo_w = w[4 * j + k];
+                uint32_t& hi_w = w[4 * (j + b) + k];
+                const uint32_t got = __shfl_xor_sync(~0u, hi ? lo_w : hi_w, b);
+                if (hi) lo_w = got;
+                else hi_w = got;
+            }
         }
     }
 }
 
+// A warp's 32 x 32 block of outputs: lane l holds position row + l (of which n
+// exist), columns [col, col + 32). Rows that start on a 16-byte boundary leave
+// as 64-byte runs of four lanes, so that a store instruction touches 8 rows and
+// not 32 (which bounded the epilogue); others value by value.
+__device__ __forceinline__ void store32(const Fp8Args& a, long long row, int n, int col,
+                                        const unsigned long long (&v)[16]) {
+    const int lane = threadIdx.x & 31, size = a.out_f32 ? 4 : 2;
+    uint8_t* base = static_cast<uint8_t*>(a.out) + (row * a.N + col) * size;
+    const bool whole = col + 32 <= a.N && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 &&
+                       (a.N * size) % 16 == 0;
+    if (whole) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            if (half && !a.out_f32) break;
+            uint4 c[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (a.out_f32) {
+                    const unsigned long long p = v[half * 8 + 2 * j], q = v[half * 8 + 2 * j + 1];
+                    c[j] = make_uint4(uint32_t(p), uint32_t(p >> 32), uint32_t(q), uint32_t(q >> 32));
+                } else {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const __nv_bfloat162 b =
+                            __floats2bfloat162_rn(lo_f(v[4 * j + k]), hi_f(v[4 * j + k]));
+                        w[k] = *reinterpret_cast<const uint32_t*>(&b);
+                    }
+                    c[j] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            transpose4(c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int r = (lane & ~3) + j;
+                if (r < n)
+                    *reinterpret_cast<uint4*>(base + (long long)r * a.N * size + half * 64 +
+                                              (lane & 3) * 16) = c[j];
+            }
+        }
+    } else if (lane < n) {
+        base += (long long)lane * a.N * size;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (col + j < a.N) {
+                const float y = j & 1 ? hi_f(v[j >> 1]) : lo_f(v[j >> 1]);
+                if (a.out_f32) reinterpret_cast<float*>(base)[j] = y;
+                else reinterpret_cast<__nv_bfloat16*>(base)[j] = __float2bfloat16_rn(y);
+            }
+    }
+}
+
 // ------------------------------------------------------------------ long segments
-// M = 128 positions, N = 256 weight rows (128 gate and 128 up rows, or 256
-// output columns): an accumulator lane is one position, so a thread needs two
-// scales per block, its position's times that of either weight block, and no
-// table. 64 columns of both blocks per thread.
-// warps 0 and 1 as above, 2 and 3 idle, 4-11 accumulation with the registers that the
-// first four give up: 4 * 32 * 80 + 8 * 32 * 208 of the launch's 384 * 168
-constexpr int kWideThreads = 384;
-constexpr int kWideStages = 4;
-constexpr int kWideStage = 3 * kABytes;  // 128 positions, 2 x 128 weight rows
-constexpr int kWideBar = 256;
-constexpr int kWideBox = 64;             // position rows of one TMA box
-inline int wide_smem(int G) {
-    return 1024 + kWideStages * kWideStage + kWideBar + 2 * 128 * 4 + 2 * (G + 1) * 4;
+// A pair of CTAs (cta_group::2): M = 256 positions, 128 per CTA, N = 256 weight
+// rows (128 gate and 128 up rows, or 256 output columns), of which each CTA
+// loads 128. One CTA that loads 256 weight rows for its 128 positions needs 94
+// bytes per clock and SM from L2 at the MMA's rate, more than L2 gives; the
+// pair needs 63.
+//
+// An accumulator lane is one position, so a thread needs two scales per block:
+// its position's times that of either weight block. Warp 2 writes these products
+// to a ring in shared memory, four blocks of K at a time. 16 accumulation warps,
+// 32 columns of both weight blocks per thread.
+constexpr int kPairThreads = 640;
+constexpr int kPairWarps = 16;
+constexpr int kPairStages = 6;
+constexpr int kPairStage = 2 * kABytes;  // 128 positions, 128 weight rows
+constexpr int kPairBar = 256;
+constexpr int kPairBox = 64;             // position rows of one TMA box
+constexpr int kPairGroup = 4;            // blocks of K per scale slot
+constexpr int kPairSlots = 2;
+constexpr int kPairScale = kPairGroup * 2 * 128 * 4;  // bytes of a slot
+inline int pair_smem(int G) {
+    return 1024 + kPairStages * kPairStage + kPairBar + kPairSlots * kPairScale + 4 * 128 * 4 +
+           2 * (G + 1) * 4;
 }
 
 template <bool GLU>
-__global__ void __launch_bounds__(kWideThreads, 1)
-    k_fp8_wide(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    k_fp8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                const Fp8Args a) {
-    constexpr int S = kWideStages;
+    constexpr int S = kPairStages;
     extern __shared__ __align__(1024) uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
                                                ~uintptr_t(1023));
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * kWideStage);
-    uint64_t* empty = full + S;
-    uint64_t* tfull = empty + S;
-    uint64_t* tempty = tfull + 2;
-    uint64_t* final_bar = tempty + 2;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * kPairStage);
+    uint64_t* done = full + S;      // a block's MMAs: its stage is free, its sums are ready
+    uint64_t* tempty = done + S;
+    uint64_t* sfull = tempty + 2;
+    uint64_t* sempty = sfull + kPairSlots;
+    uint64_t* final_bar = sempty + kPairSlots;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    uint32_t* red = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(full) + kWideBar);
-    int* off = reinterpret_cast<int*>(red + 2 * 128);
+    static_assert((2 * S + 2 + 2 * kPairSlots + 1) * 8 + 8 <= kPairBar, "barriers");
+    float* sc = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(full) + kPairBar);
+    uint32_t* red = reinterpret_cast<uint32_t*>(sc + kPairSlots * kPairScale / 4);
+    int* off = reinterpret_cast<int*>(red + 4 * 128);
     int* pref = off + a.G + 1;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = int(cluster_rank());
     const int KB = (a.K + kFp8Block - 1) / kFp8Block;
     const int MB = GLU ? (a.N + 127) / 128 : (a.N + 255) / 256;
+    const int first = int(blockIdx.x >> 1), step = int(gridDim.x >> 1);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
             mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
+            mbar_init(&done[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
-            mbar_init(&tfull[b], 1);
-            mbar_init(&tempty[b], kAccWarps);
+            mbar_init(&tempty[b], 2 * kPairWarps);  // both CTAs' (the leader's is used)
+        }
+        for (int b = 0; b < kPairSlots; ++b) {
+            mbar_init(&sfull[b], 1);
+            mbar_init(&sempty[b], kPairWarps);
         }
         mbar_init(final_bar, 1);
         *abort_flag = 0;
@@ -564,164 +624,233 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         if (a.clear_err && blockIdx.x == 0) *a.err = 0;
     }
     if (warp == 1) {
-        tmem_alloc(tmem_slot, 512);
-        tmem_relinquish();
+        tmem_alloc_pair(tmem_slot, 512);
+        tmem_relinquish_pair();
     }
-    load_plan<128>(a, MB, off, pref);
+    load_plan<256>(a, MB, off, pref);
     tc_fence_before();
     __syncthreads();
+    cluster_sync();  // the peer's barriers exist before any remote arrive
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int total = pref[a.G];
+    // No barrier that the peer arrives on hands over data in ordinary memory (TMA
+    // and the MMAs write and read shared memory, tcgen05 fences order the tensor
+    // memory), so every wait orders this CTA's accesses only.
     const auto wait = [&](uint64_t* bar, uint32_t parity) {
         return mbar_wait_for(bar, parity, abort_flag, kWaitNs);
     };
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        if (warp == 0 && lane == 0) {
-            // ---------------------------------------------------------- TMA producer
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 0) {
+            // ------------------------------------------------------ TMA producer
             tma_prefetch_desc(&tmA);
             tma_prefetch_desc(&tmB);
             uint32_t it = 0;
             bool ok = true;
-            for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+            for (int u = first; u < total && ok; u += step) {
                 Tile t;
-                decode<GLU, 128>(a, off, pref, KB, u, t);
-                const int nb = (t.n + kWideBox - 1) / kWideBox;
+                decode<GLU, 256>(a, off, pref, KB, u, t);
+                const int n0 = min(t.n, 128), n1 = t.n - n0;
+                const int nb0 = (n0 + kPairBox - 1) / kPairBox, nb1 = (n1 + kPairBox - 1) / kPairBox;
+                const int nb = rank ? nb1 : nb0, row = t.row0 + rank * 128;
+                const int wrow = rank ? t.a1 : t.a0;
                 for (int kb = 0; kb < KB; ++kb, ++it) {
                     const uint32_t s = it % S;
-                    if (!wait(&empty[s], ((it / S) & 1) ^ 1)) {
+                    if (!wait(&done[s], ((it / S) & 1) ^ 1)) {
                         ok = false;
                         break;
                     }
-                    uint8_t* st = smem + s * kWideStage;
-                    mbar_arrive_expect_tx(&full[s], 2 * kABytes + nb * kWideBox * 128);
-                    for (int j = 0; j < nb; ++j)
-                        tma_load_2d(st + j * kWideBox * 128, &tmB, &full[s], kb * 128,
-                                    t.row0 + j * kWideBox);
-                    tma_load_2d(st + kABytes, &tmA, &full[s], kb * 128, t.a0);
-                    tma_load_2d(st + 2 * kABytes, &tmA, &full[s], kb * 128, t.a1);
+                    if (elect_one()) {
+                        uint8_t* st = smem + s * kPairStage;
+                        const uint32_t fb = cluster_addr(&full[s], 0);
+                        if (rank == 0)
+                            mbar_arrive_expect_tx(&full[s],
+                                                  2 * kABytes + (nb0 + nb1) * kPairBox * 128);
+                        for (int j = 0; j < nb; ++j)
+                            tma_load_2d_pair(st + j * kPairBox * 128, &tmB, fb, kb * 128,
+                                             row + j * kPairBox);
+                        tma_load_2d_pair(st + kABytes, &tmA, fb, kb * 128, wrow);
+                    }
+                    __syncwarp();
                 }
             }
-            if (!ok) {  // every issued load lands before the CTA leaves
-                const uint32_t first = it > uint32_t(S) ? it - S : 0;
-                for (uint32_t i = first; i < it; ++i) drain_wait(&full[i % S], (i / S) & 1);
+            if (!ok && rank == 0) {  // every issued load lands before the pair leaves
+                const uint32_t from = it > uint32_t(S) ? it - S : 0;
+                for (uint32_t i = from; i < it; ++i) drain_wait(&full[i % S], (i / S) & 1);
             }
-        } else if (warp == 1 && lane == 0) {
-            // ---------------------------------------------------------- MMA issuer
-            const uint32_t idesc = idesc_e4m3_m128(256);
+        } else if (warp == 1 && rank == 0) {
+            // ------------------------------------------------------ MMA issuer
+            const uint32_t idesc = idesc_e4m3_m256(256);
             uint32_t it = 0;
             bool ok = true;
-            for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+            for (int u = first; u < total && ok; u += step) {
                 for (int kb = 0; kb < KB; ++kb, ++it) {
                     const uint32_t s = it % S, b = it & 1;
-                    if (!wait(&tempty[b], ((it >> 1) & 1) ^ 1) || !wait(&full[s], (it / S) & 1)) {
+                    if (!wait(&tempty[b], ((it >> 1) & 1) ^ 1) ||
+                        !wait(&full[s], (it / S) & 1)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t st = smem_u32(smem + s * kWideStage);
-    #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        mma_f8(tmem_base + b * 256, desc_k_sw128(st) + 2 * kk,
-                               desc_k_sw128(st + kABytes) + 2 * kk, idesc, kk != 0);
-                    mma_commit(&empty[s]);
-                    mma_commit(&tfull[b]);
+                    if (elect_one()) {
+                        const uint32_t st = smem_u32(smem + s * kPairStage);
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            mma_f8_pair(tmem_base + b * 256, desc_k_sw128(st) + 2 * kk,
+                                        desc_k_sw128(st + kABytes) + 2 * kk, idesc, kk != 0);
+                        mma_commit_both(&done[s]);
+                    }
+                    __syncwarp();
                 }
             }
-            mma_commit(final_bar);  // completes once every MMA issued above is done
+            if (elect_one()) mma_commit_pair(smem_u32(final_bar));  // every MMA above is done
+            __syncwarp();
             drain_wait(final_bar, 0);
+        } else if (warp == 2) {
+            // ------------------------------------------------------ scales
+            const bool vec = KB % 4 == 0 && (reinterpret_cast<uintptr_t>(a.sx) & 15) == 0;
+            uint32_t is = 0;
+            bool ok = true;
+            for (int u = first; u < total && ok; u += step) {
+                Tile t;
+                decode<GLU, 256>(a, off, pref, KB, u, t);
+                const int n = min(128, t.n - rank * 128);
+                for (int kb = 0; kb < KB; kb += kPairGroup, ++is) {
+                    float x[4][kPairGroup], w0[kPairGroup], w1[kPairGroup];
+#pragma unroll
+                    for (int e = 0; e < kPairGroup; ++e) {
+                        const bool in = kb + e < KB;
+                        w0[e] = in ? t.s0[kb + e] : 0.0f;
+                        w1[e] = in ? t.s1[kb + e] : 0.0f;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = j * 32 + lane;
+                        const float* p = a.sx + size_t(t.row0 + rank * 128 + (r < n ? r : 0)) * KB + kb;
+                        if (r >= n) {
+#pragma unroll
+                            for (int e = 0; e < kPairGroup; ++e) x[j][e] = 0.0f;
+                        } else if (vec) {
+                            const float4 v = *reinterpret_cast<const float4*>(p);
+                            x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < kPairGroup; ++e) x[j][e] = kb + e < KB ? p[e] : 0.0f;
+                        }
+                    }
+                    const uint32_t q = is % kPairSlots;
+                    if (!wait(&sempty[q], ((is / kPairSlots) & 1) ^ 1)) {
+                        ok = false;
+                        break;
+                    }
+                    float* o = sc + q * (kPairScale / 4) + lane;
+#pragma unroll
+                    for (int e = 0; e < kPairGroup; ++e)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            o[(e * 2) * 128 + j * 32] = x[j][e] * w0[e];
+                            o[(e * 2 + 1) * 128 + j * 32] = x[j][e] * w1[e];
+                        }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sfull[q]);
+                }
+            }
         }
     } else {
         // ---------------------------------------------------------- accumulation
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
         const int q = warp & 3, h = (warp - 4) >> 2;
         const int r = q * 32 + lane;
-        const uint32_t lanes = tmem_base + (uint32_t(q * 32) << 16) + h * 64;
-        uint32_t it = 0;
+        const uint32_t lanes = tmem_base + (uint32_t(q * 32) << 16) + h * 32;
+        const uint32_t lead_tempty = cluster_addr(&tempty[0], 0);
+        uint32_t it = 0, is = 0;
         bool ok = true;
-        for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+        for (int u = first; u < total && ok; u += step) {
             Tile t;
-            decode<GLU, 128>(a, off, pref, KB, u, t);
-            const bool work = q * 32 < t.n, rv = r < t.n;
-            const float* xp = a.sx + size_t(t.row0 + (rv ? r : 0)) * KB;
-            unsigned long long acc[4][16];  // columns h*64 + 32 c of block 0 (c < 2) and 1
+            decode<GLU, 256>(a, off, pref, KB, u, t);
+            const int n = t.n - rank * 128;  // this CTA's positions
+            const bool work = q * 32 < n, rv = r < n;
+            unsigned long long acc[2][16];  // columns [32 h, 32 h + 32) of either block
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) acc[c][j] = 0ull;
-            float x = xp[0], w0 = t.s0[0], w1 = t.s1[0];
             for (int kb = 0; kb < KB; ++kb, ++it) {
                 const uint32_t b = it & 1;
-                const float y0 = x * w0, y1 = x * w1;
-                if (kb + 1 < KB) {  // the next block's scales, in flight
-                    x = xp[kb + 1];
-                    w0 = t.s0[kb + 1];
-                    w1 = t.s1[kb + 1];
+                const int e = kb % kPairGroup;
+                const uint32_t sl = is % kPairSlots;
+                if (e == 0 && !wait(&sfull[sl], (is / kPairSlots) & 1)) {
+                    ok = false;
+                    break;
                 }
-                if (!wait(&tfull[b], (it >> 1) & 1)) {
+                const float* ps = sc + sl * (kPairScale / 4) + e * 256 + r;
+                const unsigned long long s0 = pair_of(ps[0]), s1 = pair_of(ps[128]);
+                if (!wait(&done[it % S], (it / S) & 1)) {
                     ok = false;
                     break;
                 }
                 if (work) {
                     tc_fence_after();
                     const uint32_t ta = lanes + b * 256;
-                    const unsigned long long s0 = pair_of(y0), s1 = pair_of(y1);
                     uint32_t d[2][16];
                     tmem_ld16(ta, d[0]);
                     tmem_ld_wait_reg16(d[0]);
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        if (c < 7) tmem_ld16(ta + ((c + 1) >> 2) * 128 + ((c + 1) & 3) * 16, d[(c + 1) & 1]);
+                    for (int c = 0; c < 4; ++c) {
+                        if (c < 3)
+                            tmem_ld16(ta + ((c + 1) >> 1) * 128 + ((c + 1) & 1) * 16, d[(c + 1) & 1]);
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
                             fma2(acc[c >> 1][(c & 1) * 8 + j], d[c & 1][2 * j], d[c & 1][2 * j + 1],
-                                 c < 4 ? s0 : s1);
-                        if (c < 7) tmem_ld_wait_reg16(d[(c + 1) & 1]);
+                                 c < 2 ? s0 : s1);
+                        if (c < 3) tmem_ld_wait_reg16(d[(c + 1) & 1]);
                     }
                     tc_fence_before();
                 }
+                const bool last = e == kPairGroup - 1 || kb == KB - 1;  // of this scale slot
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&tempty[b]);
+                if (lane == 0) {
+                    mbar_arrive_remote_cta(lead_tempty + b * 8);
+                    if (last) mbar_arrive(&sempty[sl]);
+                }
+                if (last) ++is;
             }
             if (!ok) break;
-            const size_t row = size_t(t.row0 + r);
+            const size_t row = size_t(t.row0 + rank * 128 + r);
             if constexpr (GLU) {
-                // silu(g) * u of this thread's 64 columns; the other 64 of the block
-                // are the other half's warp's
-                const int left = a.N - t.m0 - h * 64;  // columns before the end
+                // silu(g) * u of this thread's 32 columns; the block's other columns
+                // are the three other warps' of this quadrant
+                const int left = a.N - t.m0 - h * 32;  // columns before the end
                 uint32_t top = 0;
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int col = c * 32 + 2 * j;
-                        float m0 = 0.0f, m1 = 0.0f;
-                        if (col < left) {  // N is a multiple of 16
-                            m0 = swiglu_fast(lo_f(acc[c][j]), lo_f(acc[c + 2][j]));
-                            m1 = swiglu_fast(hi_f(acc[c][j]), hi_f(acc[c + 2][j]));
-                        }
-                        const uint32_t b0 = __float_as_uint(m0), b1 = __float_as_uint(m1);
-                        top = max(top, max(b0 & 0x7fffffffu, b1 & 0x7fffffffu));
-                        acc[c][j] = (unsigned long long)b0 | ((unsigned long long)b1 << 32);
+                for (int j = 0; j < 16; ++j) {
+                    float m0 = 0.0f, m1 = 0.0f;
+                    if (2 * j < left) {  // N is a multiple of 16
+                        m0 = swiglu_fast(lo_f(acc[0][j]), lo_f(acc[1][j]));
+                        m1 = swiglu_fast(hi_f(acc[0][j]), hi_f(acc[1][j]));
                     }
+                    const uint32_t b0 = __float_as_uint(m0), b1 = __float_as_uint(m1);
+                    top = max(top, max(b0 & 0x7fffffffu, b1 & 0x7fffffffu));
+                    acc[0][j] = (unsigned long long)b0 | ((unsigned long long)b1 << 32);
+                }
                 red[h * 128 + r] = top;
-                named_bar_sync(1 + q, 64);
-                top = max(top, red[(h ^ 1) * 128 + r]);
-                named_bar_sync(1 + q, 64);  // both have read before the next tile writes
+                named_bar_sync(1 + q, 128);
+                top = max(max(red[r], red[128 + r]), max(red[256 + r], red[384 + r]));
+                named_bar_sync(1 + q, 128);  // all have read before the next tile writes
                 float inv;
                 const float s = block_scale(__uint_as_float(top), inv);
                 if (rv) {
                     if (h == 0) a.mid_s[row * ((a.N + 127) / 128) + t.m0 / 128] = s;
-                    uint8_t* o = a.mid_q + row * a.N + t.m0 + h * 64;
+                    uint8_t* o = a.mid_q + row * a.N + t.m0 + h * 32;
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) {
+                    for (int v = 0; v < 2; ++v) {
                         uint32_t w[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const int j = (v & 1) * 8 + e * 2;
-                            const unsigned long long p0 = acc[v >> 1][j], p1 = acc[v >> 1][j + 1];
+                            const unsigned long long p0 = acc[0][v * 8 + e * 2];
+                            const unsigned long long p1 = acc[0][v * 8 + e * 2 + 1];
                             w[e] = pack4_e4m3(lo_f(p0) * inv, hi_f(p0) * inv, lo_f(p1) * inv,
                                               hi_f(p1) * inv);
                         }
@@ -729,36 +858,57 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                             *reinterpret_cast<uint4*>(o + v * 16) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                 }
-            } else if (rv) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int col = t.m0 + (c >> 1) * 128 + h * 64 + (c & 1) * 32;
-                    store32(a, row, col, acc[c]);
-                }
+            } else if (work) {
+                const long long p = t.row0 + rank * 128 + q * 32;
+                store32(a, p, n - q * 32, t.m0 + h * 32, acc[0]);
+                store32(a, p, n - q * 32, t.m0 + 128 + h * 32, acc[1]);
             }
         }
     }
-    __syncwarp();  // warps 0 and 1 ran their loops on one lane
     tc_fence_before();
     __syncthreads();
+    cluster_sync();  // no remote arrive or TMEM write targets a finished CTA
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, 512);
+        tmem_dealloc_pair(tmem_base, 512);
     }
     if (threadIdx.x == 0 && *abort_flag) atomicOr(a.err, 1);
 }
 
+// CTAs of a pair kernel that can be resident at once (an SM without a partner
+// in its GPC cannot host a pair), per kernel and device.
+int pair_grid(const void* kern, int smem, int dev) {
+    static std::mutex mu;
+    static std::map<std::pair<const void*, int>, int> cache;
+    std::lock_guard<std::mutex> lk(mu);
+    int& grid = cache[{kern, dev}];
+    if (grid == 0) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(unsigned(num_sms(dev) & ~1));
+        cfg.blockDim = dim3(kPairThreads);
+        cfg.dynamicSmemBytes = size_t(smem);
+        int clusters = 0;
+        if (cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) != cudaSuccess || clusters <= 0) {
+            cudaGetLastError();
+            clusters = num_sms(dev) / 2;
+        }
+        grid = std::min(2 * clusters, num_sms(dev) & ~1);
+    }
+    return grid;
+}
+
 template <bool GLU>
-hf_status launch_wide(const Fp8Args& a, cudaStream_t st) {
+hf_status launch_pair(const Fp8Args& a, cudaStream_t st) {
     int dev = 0;
     HF_CUDA(cudaGetDevice(&dev));
-    const auto kern = k_fp8_wide<GLU>;
-    const int smem = wide_smem(a.G);
-    HF_CUDA(ensure_smem(reinterpret_cast<const void*>(kern), smem));
+    const auto kern = k_fp8_pair<GLU>;
+    const void* kp = reinterpret_cast<const void*>(kern);
+    const int smem = pair_smem(a.G);
+    HF_CUDA(ensure_smem(kp, pair_smem(kMaxExperts)));
     CUtensorMap A, B;
     HF_TRY(make_map_u8(&A, a.w, a.K, a.a_rows, a.K, 128));
-    HF_TRY(make_map_u8(&B, a.xq, a.K, a.rows, a.K, kWideBox));
-    kern<<<num_sms(dev), kWideThreads, smem, st>>>(A, B, a);
+    HF_TRY(make_map_u8(&B, a.xq, a.K, a.rows, a.K, kPairBox));
+    kern<<<pair_grid(kp, pair_smem(kMaxExperts), dev), kPairThreads, smem, st>>>(A, B, a);
     HF_CUDA(cudaGetLastError());
     return HF_OK;
 }
@@ -783,7 +933,7 @@ hf_status launch_one(const Fp8Args& a, cudaStream_t st) {
 
 hf_status launch_fp8_product(const Fp8Args& a, bool glu, cudaStream_t st) {
     const int avg = (a.rows + a.G - 1) / a.G;
-    if (avg > 64) return glu ? launch_wide<true>(a, st) : launch_wide<false>(a, st);
+    if (avg > 64) return glu ? launch_pair<true>(a, st) : launch_pair<false>(a, st);
     if (avg > 32) return glu ? launch_one<true, 64>(a, st) : launch_one<false, 64>(a, st);
     if (avg > 16) return glu ? launch_one<true, 32>(a, st) : launch_one<false, 32>(a, st);
     return glu ? launch_one<true, 16>(a, st) : launch_one<false, 16>(a, st);

@@ -23,6 +23,20 @@ __device__ __forceinline__ uint64_t globaltimer() {
     return t;
 }
 
+// One lane of a converged warp, always the same. TMA and tcgen05 instructions
+// take their operands from uniform registers; under a branch on the lane
+// number the compiler cannot see that one lane is left and issues them slowly
+// (600 clocks for three TMA loads), under this predicate it can.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+
 // ------------------------------------------------------------------ mbarrier
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
@@ -262,6 +276,14 @@ __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_bar) {
                  : "memory");
 }
 
+// The same ordering only this CTA's accesses: for barriers that hand over
+// tensor memory (ordered by the tcgen05 fences on both sides) and no data in
+// shared or global memory, where a release at cluster scope costs more than
+// the read-back it follows.
+__device__ __forceinline__ void mbar_arrive_remote_cta(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
 __device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
 }
@@ -328,12 +350,31 @@ __device__ __forceinline__ void mma_bf16_pair(uint32_t d_tmem, uint64_t adesc, u
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
 }
 
+__device__ __forceinline__ void mma_f8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                            uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+
 // Arrives once on the mbarrier at `cluster_bar` (this CTA's or the peer's)
 // when every pair MMA issued so far by this thread has completed.
 __device__ __forceinline__ void mma_commit_pair(uint32_t cluster_bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                      cluster_bar)
                  : "memory");
+}
+
+// The same on the mbarriers at this offset in both CTAs of the pair, with one
+// instruction.
+__device__ __forceinline__ void mma_commit_both(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(smem_u32(bar)),
+        "h"(uint16_t(3))
+        : "memory");
 }
 
 // Instruction descriptor of a pair MMA: M = 256 across the two CTAs.
@@ -343,6 +384,10 @@ __device__ __forceinline__ uint32_t idesc_bf16_m256(uint32_t n) {
 // The same with FP16 A and B (format fields 0): both operands of one
 // kind::f16 MMA are always of one type.
 __device__ __forceinline__ uint32_t idesc_f16_m256(uint32_t n) {
+    return (1u << 4) | ((n >> 3) << 17) | ((256u >> 4) << 24);
+}
+
+__device__ __forceinline__ uint32_t idesc_e4m3_m256(uint32_t n) {
     return (1u << 4) | ((n >> 3) << 17) | ((256u >> 4) << 24);
 }
 
