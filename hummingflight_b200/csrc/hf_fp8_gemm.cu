@@ -145,11 +145,6 @@ __device__ __forceinline__ void fma2(unsigned long long& acc, uint32_t d0, uint3
         : "+l"(acc)
         : "r"(d0), "r"(d1), "l"(s));
 }
-__device__ __forceinline__ unsigned long long pair_of(float v) {
-    unsigned long long p;
-    asm("mov.b64 %0, {%1, %1};" : "=l"(p) : "f"(v));
-    return p;
-}
 __device__ __forceinline__ float lo_f(unsigned long long v) {
     return __uint_as_float(uint32_t(v));
 }
@@ -506,7 +501,7 @@ __device__ __forceinline__ void transpose4(uint4 (&c)[4]) {
 // as 64-byte runs of four lanes, so that a store instruction touches 8 rows and
 // not 32 (which bounded the epilogue); others value by value.
 __device__ __forceinline__ void store32(const Fp8Args& a, long long row, int n, int col,
-                                        const unsigned long long (&v)[16]) {
+                                        const float* v) {
     const int lane = threadIdx.x & 31, size = a.out_f32 ? 4 : 2;
     uint8_t* base = static_cast<uint8_t*>(a.out) + (row * a.N + col) * size;
     const bool whole = col + 32 <= a.N && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 &&
@@ -519,14 +514,15 @@ __device__ __forceinline__ void store32(const Fp8Args& a, long long row, int n, 
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (a.out_f32) {
-                    const unsigned long long p = v[half * 8 + 2 * j], q = v[half * 8 + 2 * j + 1];
-                    c[j] = make_uint4(uint32_t(p), uint32_t(p >> 32), uint32_t(q), uint32_t(q >> 32));
+                    const float* f = v + half * 16 + 4 * j;
+                    c[j] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]),
+                                      __float_as_uint(f[2]), __float_as_uint(f[3]));
                 } else {
                     uint32_t w[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const __nv_bfloat162 b =
-                            __floats2bfloat162_rn(lo_f(v[4 * j + k]), hi_f(v[4 * j + k]));
+                            __floats2bfloat162_rn(v[8 * j + 2 * k], v[8 * j + 2 * k + 1]);
                         w[k] = *reinterpret_cast<const uint32_t*>(&b);
                     }
                     c[j] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -546,9 +542,8 @@ __device__ __forceinline__ void store32(const Fp8Args& a, long long row, int n, 
 #pragma unroll
         for (int j = 0; j < 32; ++j)
             if (col + j < a.N) {
-                const float y = j & 1 ? hi_f(v[j >> 1]) : lo_f(v[j >> 1]);
-                if (a.out_f32) reinterpret_cast<float*>(base)[j] = y;
-                else reinterpret_cast<__nv_bfloat16*>(base)[j] = __float2bfloat16_rn(y);
+                if (a.out_f32) reinterpret_cast<float*>(base)[j] = v[j];
+                else reinterpret_cast<__nv_bfloat16*>(base)[j] = __float2bfloat16_rn(v[j]);
             }
     }
 }
@@ -562,10 +557,16 @@ __device__ __forceinline__ void store32(const Fp8Args& a, long long row, int n, 
 //
 // An accumulator lane is one position, so a thread needs two scales per block:
 // its position's times that of either weight block. Warp 2 writes these products
-// to a ring in shared memory, four blocks of K at a time. 16 accumulation warps,
-// 32 columns of both weight blocks per thread.
-constexpr int kPairThreads = 640;
-constexpr int kPairWarps = 16;
+// to a ring in shared memory, four blocks of K at a time.
+//
+// The MMA's N is cut in two halves of 128 (64 rows of either weight block: that
+// is what N = 128 takes from each CTA's shared memory), each with two buffers
+// and four warps of its own, 64 columns of both weight blocks a thread: a half's read-back then has the time of three
+// half MMAs (768 clocks) to be done, where one buffer of 256 left it 512.
+// warps 0-2 as above, 3 idle, 4-11 accumulation with the registers that the first
+// four give up: 4 * 32 * 56 + 8 * 32 * 224 of the launch's 384 * 168
+constexpr int kPairThreads = 384;
+constexpr int kPairWarps = 8;
 constexpr int kPairStages = 6;
 constexpr int kPairStage = 2 * kABytes;  // 128 positions, 128 weight rows
 constexpr int kPairBar = 256;
@@ -574,7 +575,7 @@ constexpr int kPairGroup = 4;            // blocks of K per scale slot
 constexpr int kPairSlots = 2;
 constexpr int kPairScale = kPairGroup * 2 * 128 * 4;  // bytes of a slot
 inline int pair_smem(int G) {
-    return 1024 + kPairStages * kPairStage + kPairBar + kPairSlots * kPairScale + 4 * 128 * 4 +
+    return 1024 + kPairStages * kPairStage + kPairBar + kPairSlots * kPairScale + 2 * 128 * 4 +
            2 * (G + 1) * 4;
 }
 
@@ -587,17 +588,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
                                                ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * kPairStage);
-    uint64_t* done = full + S;      // a block's MMAs: its stage is free, its sums are ready
-    uint64_t* tempty = done + S;
-    uint64_t* sfull = tempty + 2;
+    uint64_t* done = full + S;      // [half][stage] MMAs: sums ready (half 1: the stage is free)
+    uint64_t* tempty = done + 2 * S;  // [half][buffer]
+    uint64_t* sfull = tempty + 4;
     uint64_t* sempty = sfull + kPairSlots;
     uint64_t* final_bar = sempty + kPairSlots;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    static_assert((2 * S + 2 + 2 * kPairSlots + 1) * 8 + 8 <= kPairBar, "barriers");
+    static_assert((3 * S + 4 + 2 * kPairSlots + 1) * 8 + 8 <= kPairBar, "barriers");
     float* sc = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(full) + kPairBar);
     uint32_t* red = reinterpret_cast<uint32_t*>(sc + kPairSlots * kPairScale / 4);
-    int* off = reinterpret_cast<int*>(red + 4 * 128);
+    int* off = reinterpret_cast<int*>(red + 2 * 128);
     int* pref = off + a.G + 1;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -610,10 +611,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         for (int s = 0; s < S; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&done[s], 1);
+            mbar_init(&done[S + s], 1);
         }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(&tempty[b], 2 * kPairWarps);  // both CTAs' (the leader's is used)
-        }
+        for (int b = 0; b < 4; ++b) mbar_init(&tempty[b], kPairWarps);  // both CTAs' of a half
         for (int b = 0; b < kPairSlots; ++b) {
             mbar_init(&sfull[b], 1);
             mbar_init(&sempty[b], kPairWarps);
@@ -658,7 +658,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 const int wrow = rank ? t.a1 : t.a0;
                 for (int kb = 0; kb < KB; ++kb, ++it) {
                     const uint32_t s = it % S;
-                    if (!wait(&done[s], ((it / S) & 1) ^ 1)) {
+                    if (!wait(&done[S + s], ((it / S) & 1) ^ 1)) {
                         ok = false;
                         break;
                     }
@@ -682,27 +682,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             }
         } else if (warp == 1 && rank == 0) {
             // ------------------------------------------------------ MMA issuer
-            const uint32_t idesc = idesc_e4m3_m256(256);
+            const uint32_t idesc = idesc_e4m3_m256(128);
             uint32_t it = 0;
             bool ok = true;
             for (int u = first; u < total && ok; u += step) {
                 for (int kb = 0; kb < KB; ++kb, ++it) {
                     const uint32_t s = it % S, b = it & 1;
-                    if (!wait(&tempty[b], ((it >> 1) & 1) ^ 1) ||
-                        !wait(&full[s], (it / S) & 1)) {
+                    if (!wait(&full[s], (it / S) & 1)) {
                         ok = false;
                         break;
                     }
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint32_t st = smem_u32(smem + s * kPairStage);
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            mma_f8_pair(tmem_base + b * 256, desc_k_sw128(st) + 2 * kk,
-                                        desc_k_sw128(st + kABytes) + 2 * kk, idesc, kk != 0);
-                        mma_commit_both(&done[s]);
+                    for (int hf = 0; hf < 2; ++hf) {
+                        ok = ok && wait(&tempty[hf * 2 + b], ((it >> 1) & 1) ^ 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (elect_one()) {
+                            const uint32_t st = smem_u32(smem + s * kPairStage);
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk)
+                                mma_f8_pair(tmem_base + b * 256 + hf * 128,
+                                            desc_k_sw128(st) + 2 * kk,
+                                            desc_k_sw128(st + kABytes + hf * (kABytes / 2)) + 2 * kk,
+                                            idesc, kk != 0);
+                            mma_commit_both(&done[hf * S + s]);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
+                    if (!ok) break;
                 }
             }
             if (elect_one()) mma_commit_pair(smem_u32(final_bar));  // every MMA above is done
@@ -760,11 +767,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         }
     } else {
         // ---------------------------------------------------------- accumulation
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int q = warp & 3, h = (warp - 4) >> 2;
         const int r = q * 32 + lane;
-        const uint32_t lanes = tmem_base + (uint32_t(q * 32) << 16) + h * 32;
-        const uint32_t lead_tempty = cluster_addr(&tempty[0], 0);
+        // half h: columns [0, 64) are block 0's, [64, 128) block 1's
+        const uint32_t lanes = tmem_base + (uint32_t(q * 32) << 16) + h * 128;
+        const uint32_t lead_tempty = cluster_addr(&tempty[h * 2], 0);
+        uint64_t* const half_done = done + h * S;
         uint32_t it = 0, is = 0;
         bool ok = true;
         for (int u = first; u < total && ok; u += step) {
@@ -772,11 +781,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             decode<GLU, 256>(a, off, pref, KB, u, t);
             const int n = t.n - rank * 128;  // this CTA's positions
             const bool work = q * 32 < n, rv = r < n;
-            unsigned long long acc[2][16];  // columns [32 h, 32 h + 32) of either block
+            float acc[2][64];  // columns [64 h, 64 h + 64) of either block
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int j = 0; j < 16; ++j) acc[c][j] = 0ull;
+                for (int j = 0; j < 64; ++j) acc[c][j] = 0.0f;
             for (int kb = 0; kb < KB; ++kb, ++it) {
                 const uint32_t b = it & 1;
                 const int e = kb % kPairGroup;
@@ -786,26 +795,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     break;
                 }
                 const float* ps = sc + sl * (kPairScale / 4) + e * 256 + r;
-                const unsigned long long s0 = pair_of(ps[0]), s1 = pair_of(ps[128]);
-                if (!wait(&done[it % S], (it / S) & 1)) {
+                const float s0 = ps[0], s1 = ps[128];
+                if (!wait(&half_done[it % S], (it / S) & 1)) {
                     ok = false;
                     break;
                 }
                 if (work) {
                     tc_fence_after();
                     const uint32_t ta = lanes + b * 256;
-                    uint32_t d[2][16];
-                    tmem_ld16(ta, d[0]);
-                    tmem_ld_wait_reg16(d[0]);
+                    uint32_t d[64];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        if (c < 3)
-                            tmem_ld16(ta + ((c + 1) >> 1) * 128 + ((c + 1) & 1) * 16, d[(c + 1) & 1]);
+                    for (int c = 0; c < 2; ++c) {
+                        tmem_ld64(ta + c * 64, d);
+                        tmem_ld_wait_reg64(d);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            fma2(acc[c >> 1][(c & 1) * 8 + j], d[c & 1][2 * j], d[c & 1][2 * j + 1],
-                                 c < 2 ? s0 : s1);
-                        if (c < 3) tmem_ld_wait_reg16(d[(c + 1) & 1]);
+                        for (int j = 0; j < 64; ++j)
+                            acc[c][j] = fmaf(__uint_as_float(d[j]), c ? s1 : s0, acc[c][j]);
                     }
                     tc_fence_before();
                 }
@@ -820,39 +825,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             if (!ok) break;
             const size_t row = size_t(t.row0 + rank * 128 + r);
             if constexpr (GLU) {
-                // silu(g) * u of this thread's 32 columns; the block's other columns
-                // are the three other warps' of this quadrant
-                const int left = a.N - t.m0 - h * 32;  // columns before the end
-                uint32_t top = 0;
+                // silu(g) * u of this thread's 64 columns; the other 64 of the block are
+                // the other half's warp's
+                const int left = a.N - t.m0 - h * 64;  // columns before the end
+                float top = 0.0f;
+                uint32_t nan = 0;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    float m0 = 0.0f, m1 = 0.0f;
-                    if (2 * j < left) {  // N is a multiple of 16
-                        m0 = swiglu_fast(lo_f(acc[0][j]), lo_f(acc[1][j]));
-                        m1 = swiglu_fast(hi_f(acc[0][j]), hi_f(acc[1][j]));
-                    }
-                    const uint32_t b0 = __float_as_uint(m0), b1 = __float_as_uint(m1);
-                    top = max(top, max(b0 & 0x7fffffffu, b1 & 0x7fffffffu));
-                    acc[0][j] = (unsigned long long)b0 | ((unsigned long long)b1 << 32);
+                for (int j = 0; j < 64; ++j) {
+                    const float m = j < left ? swiglu_fast(acc[0][j], acc[1][j]) : 0.0f;
+                    top = fmaxf(top, fabsf(m));
+                    nan |= m != m;
+                    acc[0][j] = m;
                 }
-                red[h * 128 + r] = top;
-                named_bar_sync(1 + q, 128);
-                top = max(max(red[r], red[128 + r]), max(red[256 + r], red[384 + r]));
-                named_bar_sync(1 + q, 128);  // all have read before the next tile writes
+                red[h * 128 + r] = nan ? 0x7fc00000u : __float_as_uint(top);
+                named_bar_sync(1 + q, 64);
+                const uint32_t both = max(red[r], red[128 + r]);
+                named_bar_sync(1 + q, 64);  // both have read before the next tile writes
                 float inv;
-                const float s = block_scale(__uint_as_float(top), inv);
+                const float s = block_scale(__uint_as_float(both), inv);
                 if (rv) {
                     if (h == 0) a.mid_s[row * ((a.N + 127) / 128) + t.m0 / 128] = s;
-                    uint8_t* o = a.mid_q + row * a.N + t.m0 + h * 32;
+                    uint8_t* o = a.mid_q + row * a.N + t.m0 + h * 64;
 #pragma unroll
-                    for (int v = 0; v < 2; ++v) {
+                    for (int v = 0; v < 4; ++v) {
                         uint32_t w[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const unsigned long long p0 = acc[0][v * 8 + e * 2];
-                            const unsigned long long p1 = acc[0][v * 8 + e * 2 + 1];
-                            w[e] = pack4_e4m3(lo_f(p0) * inv, hi_f(p0) * inv, lo_f(p1) * inv,
-                                              hi_f(p1) * inv);
+                            const float* m = &acc[0][v * 16 + e * 4];
+                            w[e] = pack4_e4m3(m[0] * inv, m[1] * inv, m[2] * inv, m[3] * inv);
                         }
                         if (v * 16 < left)
                             *reinterpret_cast<uint4*>(o + v * 16) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -860,8 +860,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 }
             } else if (work) {
                 const long long p = t.row0 + rank * 128 + q * 32;
-                store32(a, p, n - q * 32, t.m0 + h * 32, acc[0]);
-                store32(a, p, n - q * 32, t.m0 + 128 + h * 32, acc[1]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    store32(a, p, n - q * 32, t.m0 + (c >> 1) * 128 + h * 64 + (c & 1) * 32,
+                            &acc[c >> 1][(c & 1) * 32]);
             }
         }
     }
