@@ -145,6 +145,15 @@ __device__ __forceinline__ void fma2(unsigned long long& acc, uint32_t d0, uint3
         : "+l"(acc)
         : "r"(d0), "r"(d1), "l"(s));
 }
+__device__ __forceinline__ void fma2(unsigned long long& acc, unsigned long long d,
+                                     unsigned long long s) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(d), "l"(s));
+}
+__device__ __forceinline__ unsigned long long pair_of(float v) {
+    unsigned long long p;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(p) : "f"(v));
+    return p;
+}
 __device__ __forceinline__ float lo_f(unsigned long long v) {
     return __uint_as_float(uint32_t(v));
 }
@@ -206,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem_base = *tmem_slot;
     const int total = pref[a.G];
     const auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return mbar_wait_for(bar, parity, abort_flag, kWaitNs);
+        return mbar_wait_for(smem_u32(bar), parity, abort_flag, kWaitNs);
     };
 
     if (warp < 4) {
@@ -501,7 +510,7 @@ __device__ __forceinline__ void transpose4(uint4 (&c)[4]) {
 // as 64-byte runs of four lanes, so that a store instruction touches 8 rows and
 // not 32 (which bounded the epilogue); others value by value.
 __device__ __forceinline__ void store32(const Fp8Args& a, long long row, int n, int col,
-                                        const float* v) {
+                                        const unsigned long long* v) {
     const int lane = threadIdx.x & 31, size = a.out_f32 ? 4 : 2;
     uint8_t* base = static_cast<uint8_t*>(a.out) + (row * a.N + col) * size;
     const bool whole = col + 32 <= a.N && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 &&
@@ -514,15 +523,14 @@ __device__ __forceinline__ void store32(const Fp8Args& a, long long row, int n, 
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (a.out_f32) {
-                    const float* f = v + half * 16 + 4 * j;
-                    c[j] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]),
-                                      __float_as_uint(f[2]), __float_as_uint(f[3]));
+                    const unsigned long long p = v[half * 8 + 2 * j], q = v[half * 8 + 2 * j + 1];
+                    c[j] = make_uint4(uint32_t(p), uint32_t(p >> 32), uint32_t(q), uint32_t(q >> 32));
                 } else {
                     uint32_t w[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const __nv_bfloat162 b =
-                            __floats2bfloat162_rn(v[8 * j + 2 * k], v[8 * j + 2 * k + 1]);
+                            __floats2bfloat162_rn(lo_f(v[4 * j + k]), hi_f(v[4 * j + k]));
                         w[k] = *reinterpret_cast<const uint32_t*>(&b);
                     }
                     c[j] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -542,8 +550,9 @@ __device__ __forceinline__ void store32(const Fp8Args& a, long long row, int n, 
 #pragma unroll
         for (int j = 0; j < 32; ++j)
             if (col + j < a.N) {
-                if (a.out_f32) reinterpret_cast<float*>(base)[j] = v[j];
-                else reinterpret_cast<__nv_bfloat16*>(base)[j] = __float2bfloat16_rn(v[j]);
+                const float y = j & 1 ? hi_f(v[j >> 1]) : lo_f(v[j >> 1]);
+                if (a.out_f32) reinterpret_cast<float*>(base)[j] = y;
+                else reinterpret_cast<__nv_bfloat16*>(base)[j] = __float2bfloat16_rn(y);
             }
     }
 }
@@ -557,21 +566,25 @@ __device__ __forceinline__ void store32(const Fp8Args& a, long long row, int n, 
 //
 // An accumulator lane is one position, so a thread needs two scales per block:
 // its position's times that of either weight block. Warp 2 writes these products
-// to a ring in shared memory, four blocks of K at a time.
+// to a ring in shared memory, eight blocks of K at a time.
 //
 // The MMA's N is cut in two halves of 128 (64 rows of either weight block: that
-// is what N = 128 takes from each CTA's shared memory), each with two buffers
-// and four warps of its own, 64 columns of both weight blocks a thread: a half's read-back then has the time of three
-// half MMAs (768 clocks) to be done, where one buffer of 256 left it 512.
-// warps 0-2 as above, 3 idle, 4-11 accumulation with the registers that the first
-// four give up: 4 * 32 * 56 + 8 * 32 * 224 of the launch's 384 * 168
+// is what N = 128 takes from each CTA's shared memory). Each half has two
+// buffers, an issuing warp and four accumulation warps (64 columns of both weight
+// blocks a thread) of its own. The chain MMA -> commit -> read-back -> release ->
+// MMA of one buffer costs about 1000 clocks, half of them barrier latencies (a
+// commit 200, a cluster arrive 120, a wait 50 each), against 515 for a block's
+// MMAs; two independent halves overlap their chains.
+//
+// Warps: 0 TMA producer, 1 and 3 MMA issuers of the halves (leader CTA; 1 owns
+// TMEM), 2 scales, 4-11 accumulation with the registers that the first four give up: 4 * 32 * 56 + 8 * 32 * 224 of the launch's 384 * 168
 constexpr int kPairThreads = 384;
 constexpr int kPairWarps = 8;
 constexpr int kPairStages = 6;
 constexpr int kPairStage = 2 * kABytes;  // 128 positions, 128 weight rows
 constexpr int kPairBar = 256;
 constexpr int kPairBox = 64;             // position rows of one TMA box
-constexpr int kPairGroup = 4;            // blocks of K per scale slot
+constexpr int kPairGroup = 8;            // blocks of K per scale slot
 constexpr int kPairSlots = 2;
 constexpr int kPairScale = kPairGroup * 2 * 128 * 4;  // bytes of a slot
 inline int pair_smem(int G) {
@@ -588,7 +601,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
                                                ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * kPairStage);
-    uint64_t* done = full + S;      // [half][stage] MMAs: sums ready (half 1: the stage is free)
+    uint64_t* done = full + S;        // [half][stage] MMAs: sums ready, operands read
     uint64_t* tempty = done + 2 * S;  // [half][buffer]
     uint64_t* sfull = tempty + 4;
     uint64_t* sempty = sfull + kPairSlots;
@@ -618,7 +631,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             mbar_init(&sfull[b], 1);
             mbar_init(&sempty[b], kPairWarps);
         }
-        mbar_init(final_bar, 1);
+        mbar_init(final_bar, 2);
         *abort_flag = 0;
         fence_mbar_init();
         if (a.clear_err && blockIdx.x == 0) *a.err = 0;
@@ -637,9 +650,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     // No barrier that the peer arrives on hands over data in ordinary memory (TMA
     // and the MMAs write and read shared memory, tcgen05 fences order the tensor
     // memory), so every wait orders this CTA's accesses only.
-    const auto wait = [&](uint64_t* bar, uint32_t parity) {
+    const auto wait = [&](uint32_t bar, uint32_t parity) {
         return mbar_wait_for(bar, parity, abort_flag, kWaitNs);
     };
+    const uint32_t full_at = smem_u32(full), done_at = smem_u32(done);
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -647,7 +661,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             // ------------------------------------------------------ TMA producer
             tma_prefetch_desc(&tmA);
             tma_prefetch_desc(&tmB);
-            uint32_t it = 0;
+            uint32_t s = 0, ph = 1, issued = 0;
             bool ok = true;
             for (int u = first; u < total && ok; u += step) {
                 Tile t;
@@ -656,65 +670,70 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 const int nb0 = (n0 + kPairBox - 1) / kPairBox, nb1 = (n1 + kPairBox - 1) / kPairBox;
                 const int nb = rank ? nb1 : nb0, row = t.row0 + rank * 128;
                 const int wrow = rank ? t.a1 : t.a0;
-                for (int kb = 0; kb < KB; ++kb, ++it) {
-                    const uint32_t s = it % S;
-                    if (!wait(&done[S + s], ((it / S) & 1) ^ 1)) {
+                const uint32_t bytes = 2 * kABytes + (nb0 + nb1) * kPairBox * 128;
+                for (int kb = 0; kb < KB; ++kb, ++issued) {
+                    if (!wait(done_at + s * 8, ph) || !wait(done_at + (S + s) * 8, ph)) {
                         ok = false;
                         break;
                     }
                     if (elect_one()) {
                         uint8_t* st = smem + s * kPairStage;
                         const uint32_t fb = cluster_addr(&full[s], 0);
-                        if (rank == 0)
-                            mbar_arrive_expect_tx(&full[s],
-                                                  2 * kABytes + (nb0 + nb1) * kPairBox * 128);
+                        if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
                         for (int j = 0; j < nb; ++j)
                             tma_load_2d_pair(st + j * kPairBox * 128, &tmB, fb, kb * 128,
                                              row + j * kPairBox);
                         tma_load_2d_pair(st + kABytes, &tmA, fb, kb * 128, wrow);
                     }
                     __syncwarp();
+                    if (++s == S) {
+                        s = 0;
+                        ph ^= 1;
+                    }
                 }
             }
             if (!ok && rank == 0) {  // every issued load lands before the pair leaves
-                const uint32_t from = it > uint32_t(S) ? it - S : 0;
-                for (uint32_t i = from; i < it; ++i) drain_wait(&full[i % S], (i / S) & 1);
+                const uint32_t from = issued > uint32_t(S) ? issued - S : 0;
+                for (uint32_t i = from; i < issued; ++i) drain_wait(&full[i % S], (i / S) & 1);
             }
-        } else if (warp == 1 && rank == 0) {
-            // ------------------------------------------------------ MMA issuer
-            const uint32_t idesc = idesc_e4m3_m256(128);
-            uint32_t it = 0;
-            bool ok = true;
-            for (int u = first; u < total && ok; u += step) {
-                for (int kb = 0; kb < KB; ++kb, ++it) {
-                    const uint32_t s = it % S, b = it & 1;
-                    if (!wait(&full[s], (it / S) & 1)) {
-                        ok = false;
-                        break;
-                    }
-#pragma unroll
-                    for (int hf = 0; hf < 2; ++hf) {
-                        ok = ok && wait(&tempty[hf * 2 + b], ((it >> 1) & 1) ^ 1);
-                        if (!ok) break;
+        } else if (warp != 2) {
+            // ------------------------------------------------------ MMA issuers
+            if (rank == 0) {
+                const int hf = warp >> 1;  // warp 1: half 0, warp 3: half 1
+                const uint32_t idesc = idesc_e4m3_m256(128);
+                const uint64_t ad = desc_k_sw128(smem_u32(smem));
+                const uint64_t bd = desc_k_sw128(smem_u32(smem) + kABytes + hf * (kABytes / 2));
+                const uint32_t te_at = smem_u32(tempty + hf * 2);
+                uint32_t s = 0, ph = 0, b = 0, bph = 1;
+                bool ok = true;
+                for (int u = first; u < total && ok; u += step) {
+                    for (int kb = 0; kb < KB; ++kb) {
+                        if (!wait(full_at + s * 8, ph) || !wait(te_at + b * 8, bph)) {
+                            ok = false;
+                            break;
+                        }
                         tc_fence_after();
                         if (elect_one()) {
-                            const uint32_t st = smem_u32(smem + s * kPairStage);
+                            const uint32_t d = tmem_base + b * 256 + hf * 128;
+                            const uint32_t o = s * (kPairStage >> 4);
 #pragma unroll
                             for (int kk = 0; kk < 4; ++kk)
-                                mma_f8_pair(tmem_base + b * 256 + hf * 128,
-                                            desc_k_sw128(st) + 2 * kk,
-                                            desc_k_sw128(st + kABytes + hf * (kABytes / 2)) + 2 * kk,
-                                            idesc, kk != 0);
+                                mma_f8_pair(d, ad + o + 2 * kk, bd + o + 2 * kk, idesc, kk != 0);
                             mma_commit_both(&done[hf * S + s]);
                         }
                         __syncwarp();
+                        if (++s == S) {
+                            s = 0;
+                            ph ^= 1;
+                        }
+                        bph ^= b;
+                        b ^= 1;
                     }
-                    if (!ok) break;
                 }
+                if (elect_one()) mma_commit_pair(smem_u32(final_bar));  // every MMA above is done
+                __syncwarp();
+                drain_wait(final_bar, 0);
             }
-            if (elect_one()) mma_commit_pair(smem_u32(final_bar));  // every MMA above is done
-            __syncwarp();
-            drain_wait(final_bar, 0);
         } else if (warp == 2) {
             // ------------------------------------------------------ scales
             const bool vec = KB % 4 == 0 && (reinterpret_cast<uintptr_t>(a.sx) & 15) == 0;
@@ -724,42 +743,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 Tile t;
                 decode<GLU, 256>(a, off, pref, KB, u, t);
                 const int n = min(128, t.n - rank * 128);
-                for (int kb = 0; kb < KB; kb += kPairGroup, ++is) {
-                    float x[4][kPairGroup], w0[kPairGroup], w1[kPairGroup];
-#pragma unroll
-                    for (int e = 0; e < kPairGroup; ++e) {
-                        const bool in = kb + e < KB;
-                        w0[e] = in ? t.s0[kb + e] : 0.0f;
-                        w1[e] = in ? t.s1[kb + e] : 0.0f;
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int r = j * 32 + lane;
-                        const float* p = a.sx + size_t(t.row0 + rank * 128 + (r < n ? r : 0)) * KB + kb;
-                        if (r >= n) {
-#pragma unroll
-                            for (int e = 0; e < kPairGroup; ++e) x[j][e] = 0.0f;
-                        } else if (vec) {
-                            const float4 v = *reinterpret_cast<const float4*>(p);
-                            x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < kPairGroup; ++e) x[j][e] = kb + e < KB ? p[e] : 0.0f;
-                        }
-                    }
+                for (int k0 = 0; k0 < KB; k0 += kPairGroup, ++is) {
                     const uint32_t q = is % kPairSlots;
-                    if (!wait(&sempty[q], ((is / kPairSlots) & 1) ^ 1)) {
-                        ok = false;
-                        break;
-                    }
-                    float* o = sc + q * (kPairScale / 4) + lane;
 #pragma unroll
-                    for (int e = 0; e < kPairGroup; ++e)
+                    for (int part = 0; part < kPairGroup; part += 4) {
+                        const int kb = k0 + part;
+                        float x[4][4], w0[4], w1[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const bool in = kb + e < KB;
+                            w0[e] = in ? t.s0[kb + e] : 0.0f;
+                            w1[e] = in ? t.s1[kb + e] : 0.0f;
+                        }
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            o[(e * 2) * 128 + j * 32] = x[j][e] * w0[e];
-                            o[(e * 2 + 1) * 128 + j * 32] = x[j][e] * w1[e];
+                            const int r = j * 32 + lane;
+                            const float* p =
+                                a.sx + size_t(t.row0 + rank * 128 + (r < n ? r : 0)) * KB + kb;
+                            if (r >= n || kb >= KB) {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) x[j][e] = 0.0f;
+                            } else if (vec) {
+                                const float4 v = *reinterpret_cast<const float4*>(p);
+                                x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) x[j][e] = kb + e < KB ? p[e] : 0.0f;
+                            }
                         }
+                        if (part == 0 &&
+                            !wait(smem_u32(&sempty[q]), ((is / kPairSlots) & 1) ^ 1)) {
+                            ok = false;
+                            break;
+                        }
+                        float* o = sc + q * (kPairScale / 4) + part * 256 + lane;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                o[e * 256 + j * 32] = x[j][e] * w0[e];
+                                o[e * 256 + 128 + j * 32] = x[j][e] * w1[e];
+                            }
+                    }
+                    if (!ok) break;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sfull[q]);
                 }
@@ -772,55 +798,70 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const int r = q * 32 + lane;
         // half h: columns [0, 64) are block 0's, [64, 128) block 1's
         const uint32_t lanes = tmem_base + (uint32_t(q * 32) << 16) + h * 128;
-        const uint32_t lead_tempty = cluster_addr(&tempty[h * 2], 0);
-        uint64_t* const half_done = done + h * S;
-        uint32_t it = 0, is = 0;
+        const uint32_t te_at = cluster_addr(&tempty[h * 2], 0);  // the leader's
+        const uint32_t ready_at = done_at + h * S * 8;
+        const uint32_t sf_at = smem_u32(sfull);
+        // ring positions: stage and its phase, buffer, scale slot and its phase
+        uint32_t s = 0, ph = 0, b = 0, sl = 0, sph = 0;
         bool ok = true;
         for (int u = first; u < total && ok; u += step) {
             Tile t;
             decode<GLU, 256>(a, off, pref, KB, u, t);
             const int n = t.n - rank * 128;  // this CTA's positions
             const bool work = q * 32 < n, rv = r < n;
-            float acc[2][64];  // columns [64 h, 64 h + 64) of either block
+            // columns [64 h, 64 h + 64) of either block, in pairs
+            unsigned long long acc[2][32];
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int j = 0; j < 64; ++j) acc[c][j] = 0.0f;
-            for (int kb = 0; kb < KB; ++kb, ++it) {
-                const uint32_t b = it & 1;
-                const int e = kb % kPairGroup;
-                const uint32_t sl = is % kPairSlots;
-                if (e == 0 && !wait(&sfull[sl], (is / kPairSlots) & 1)) {
-                    ok = false;
-                    break;
-                }
-                const float* ps = sc + sl * (kPairScale / 4) + e * 256 + r;
-                const float s0 = ps[0], s1 = ps[128];
-                if (!wait(&half_done[it % S], (it / S) & 1)) {
-                    ok = false;
-                    break;
-                }
-                if (work) {
-                    tc_fence_after();
-                    const uint32_t ta = lanes + b * 256;
-                    uint32_t d[64];
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        tmem_ld64(ta + c * 64, d);
-                        tmem_ld_wait_reg64(d);
-#pragma unroll
-                        for (int j = 0; j < 64; ++j)
-                            acc[c][j] = fmaf(__uint_as_float(d[j]), c ? s1 : s0, acc[c][j]);
-                    }
-                    tc_fence_before();
-                }
-                const bool last = e == kPairGroup - 1 || kb == KB - 1;  // of this scale slot
+                for (int j = 0; j < 32; ++j) acc[c][j] = 0ull;
+            const auto release = [&] {  // the buffer goes back
+                tc_fence_before();
                 __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive_remote_cta(lead_tempty + b * 8);
-                    if (last) mbar_arrive(&sempty[sl]);
+                if (lane == 0) mbar_arrive_remote_cta(te_at + b * 8);
+                b ^= 1;
+                if (++s == S) {
+                    s = 0;
+                    ph ^= 1;
                 }
-                if (last) ++is;
+            };
+            for (int k0 = 0; k0 < KB && ok; k0 += kPairGroup) {
+                if (!wait(sf_at + sl * 8, sph)) {
+                    ok = false;
+                    break;
+                }
+                const float* ps = sc + sl * (kPairScale / 4) + r;
+                const int ng = min(kPairGroup, KB - k0);
+                if (work) {
+#pragma unroll 1
+                    for (int e = 0; e < ng; ++e, ps += 256) {
+                        const unsigned long long s0 = pair_of(ps[0]), s1 = pair_of(ps[128]);
+                        if (!wait(ready_at + s * 8, ph)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t ta = lanes + b * 256;
+                        unsigned long long d[32];
+                        tmem_read64(ta, d);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) fma2(acc[0][j], d[j], s0);
+                        tmem_read64(ta + 64, d);
+                        release();  // read: the second block's multiply-adds can follow
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) fma2(acc[1][j], d[j], s1);
+                    }
+                } else {  // no position of this warp: it keeps step only
+#pragma unroll 1
+                    for (int e = 0; e < ng && ok; ++e) {
+                        ok = wait(ready_at + s * 8, ph);
+                        if (ok) release();
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sempty[sl]);
+                sph ^= sl;
+                sl ^= 1;
             }
             if (!ok) break;
             const size_t row = size_t(t.row0 + rank * 128 + r);
@@ -828,16 +869,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 // silu(g) * u of this thread's 64 columns; the other 64 of the block are
                 // the other half's warp's
                 const int left = a.N - t.m0 - h * 64;  // columns before the end
-                float top = 0.0f;
-                uint32_t nan = 0;
+                uint32_t top = 0;
 #pragma unroll
-                for (int j = 0; j < 64; ++j) {
-                    const float m = j < left ? swiglu_fast(acc[0][j], acc[1][j]) : 0.0f;
-                    top = fmaxf(top, fabsf(m));
-                    nan |= m != m;
-                    acc[0][j] = m;
+                for (int j = 0; j < 32; ++j) {
+                    float m0 = 0.0f, m1 = 0.0f;
+                    if (2 * j < left) {  // N is a multiple of 16
+                        m0 = swiglu_fast(lo_f(acc[0][j]), lo_f(acc[1][j]));
+                        m1 = swiglu_fast(hi_f(acc[0][j]), hi_f(acc[1][j]));
+                    }
+                    const uint32_t b0 = __float_as_uint(m0), b1 = __float_as_uint(m1);
+                    top = max(top, max(b0 & 0x7fffffffu, b1 & 0x7fffffffu));
+                    acc[0][j] = (unsigned long long)b0 | ((unsigned long long)b1 << 32);
                 }
-                red[h * 128 + r] = nan ? 0x7fc00000u : __float_as_uint(top);
+                red[h * 128 + r] = top;
                 named_bar_sync(1 + q, 64);
                 const uint32_t both = max(red[r], red[128 + r]);
                 named_bar_sync(1 + q, 64);  // both have read before the next tile writes
@@ -851,8 +895,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                         uint32_t w[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const float* m = &acc[0][v * 16 + e * 4];
-                            w[e] = pack4_e4m3(m[0] * inv, m[1] * inv, m[2] * inv, m[3] * inv);
+                            const unsigned long long p0 = acc[0][v * 8 + e * 2];
+                            const unsigned long long p1 = acc[0][v * 8 + e * 2 + 1];
+                            w[e] = pack4_e4m3(lo_f(p0) * inv, hi_f(p0) * inv, lo_f(p1) * inv,
+                                              hi_f(p1) * inv);
                         }
                         if (v * 16 < left)
                             *reinterpret_cast<uint4*>(o + v * 16) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -863,7 +909,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
                     store32(a, p, n - q * 32, t.m0 + (c >> 1) * 128 + h * 64 + (c & 1) * 32,
-                            &acc[c >> 1][(c & 1) * 32]);
+                            &acc[c >> 1][(c & 1) * 16]);
             }
         }
     }

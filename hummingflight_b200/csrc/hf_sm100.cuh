@@ -86,13 +86,22 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     return true;
 }
 
-// The same with a limit of its own for each wait: `limit` ns from the first
-// slow poll, whatever the kernel's run time.
-__device__ __forceinline__ bool mbar_wait_for(uint64_t* bar, uint32_t parity,
+// The same on a barrier's shared-memory address, with a limit of its own for
+// each wait: `limit` ns from the first slow poll, whatever the kernel's run time.
+__device__ __forceinline__ bool mbar_wait_for(uint32_t bar, uint32_t parity,
                                               volatile int* abort_flag, uint64_t limit) {
     uint32_t spins = 0;
     uint64_t deadline = 0;
-    while (!mbar_try_wait(bar, parity)) {
+    while (true) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.b32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (ok) return true;
         if ((++spins & 255u) == 0) {
             if (*abort_flag) return false;
             const uint64_t now = globaltimer();
@@ -103,7 +112,6 @@ __device__ __forceinline__ bool mbar_wait_for(uint64_t* bar, uint32_t parity,
             }
         }
     }
-    return true;
 }
 
 // ------------------------------------------------------------------ TMA (tiled 2-D, CTA-local)
@@ -215,42 +223,39 @@ __device__ __forceinline__ void tmem_ld_wait_regs(uint32_t (&a)[16], uint32_t (&
                  :
                  : "memory");
 }
-// 64 columns at once.
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+// 64 columns, waited for, as 32 pairs of floats (columns 2i and 2i + 1). Load,
+// wait and pairing are one statement: with the wait apart, its operands (which
+// keep the compiler from moving uses across it) cost a move for each register.
+__device__ __forceinline__ void tmem_read64(uint32_t taddr, unsigned long long (&v)[32]) {
     asm volatile(
+        "{\n\t"
+        ".reg .b32 r0, r1, r2, r3, r4, r5, r6, r7, r8, r9, r10, r11, r12, r13, r14, r15;\n\t"
+        ".reg .b32 r16, r17, r18, r19, r20, r21, r22, r23, r24, r25, r26, r27, r28, r29, r30, r31;\n\t"
+        ".reg .b32 r32, r33, r34, r35, r36, r37, r38, r39, r40, r41, r42, r43, r44, r45, r46, r47;\n\t"
+        ".reg .b32 r48, r49, r50, r51, r52, r53, r54, r55, r56, r57, r58, r59, r60, r61, r62, r63;\n\t"
         "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
-        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
-        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
-          "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
-          "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
-          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
-          "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
-          "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]),
-          "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]),
-          "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]),
-          "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-        : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_ld_wait_reg64(uint32_t (&a)[64]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]),
-                   "+r"(a[6]), "+r"(a[7]), "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]),
-                   "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15]), "+r"(a[16]), "+r"(a[17]),
-                   "+r"(a[18]), "+r"(a[19]), "+r"(a[20]), "+r"(a[21]), "+r"(a[22]), "+r"(a[23]),
-                   "+r"(a[24]), "+r"(a[25]), "+r"(a[26]), "+r"(a[27]), "+r"(a[28]), "+r"(a[29]),
-                   "+r"(a[30]), "+r"(a[31]), "+r"(a[32]), "+r"(a[33]), "+r"(a[34]), "+r"(a[35]),
-                   "+r"(a[36]), "+r"(a[37]), "+r"(a[38]), "+r"(a[39]), "+r"(a[40]), "+r"(a[41]),
-                   "+r"(a[42]), "+r"(a[43]), "+r"(a[44]), "+r"(a[45]), "+r"(a[46]), "+r"(a[47]),
-                   "+r"(a[48]), "+r"(a[49]), "+r"(a[50]), "+r"(a[51]), "+r"(a[52]), "+r"(a[53]),
-                   "+r"(a[54]), "+r"(a[55]), "+r"(a[56]), "+r"(a[57]), "+r"(a[58]), "+r"(a[59]),
-                   "+r"(a[60]), "+r"(a[61]), "+r"(a[62]), "+r"(a[63])
-                 :
-                 : "memory");
+        "r0, r1, r2, r3, r4, r5, r6, r7, r8, r9, r10, r11, r12, r13, r14, r15, "
+        "r16, r17, r18, r19, r20, r21, r22, r23, r24, r25, r26, r27, r28, r29, r30, r31, "
+        "r32, r33, r34, r35, r36, r37, r38, r39, r40, r41, r42, r43, r44, r45, r46, r47, "
+        "r48, r49, r50, r51, r52, r53, r54, r55, r56, r57, r58, r59, r60, r61, r62, r63}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;\n\t"
+        "mov.b64 %0, {r0, r1}; mov.b64 %1, {r2, r3}; mov.b64 %2, {r4, r5}; mov.b64 %3, {r6, r7};"
+        "mov.b64 %4, {r8, r9}; mov.b64 %5, {r10, r11}; mov.b64 %6, {r12, r13}; mov.b64 %7, {r14, r15};"
+        "mov.b64 %8, {r16, r17}; mov.b64 %9, {r18, r19}; mov.b64 %10, {r20, r21}; mov.b64 %11, {r22, r23};"
+        "mov.b64 %12, {r24, r25}; mov.b64 %13, {r26, r27}; mov.b64 %14, {r28, r29}; mov.b64 %15, {r30, r31};"
+        "mov.b64 %16, {r32, r33}; mov.b64 %17, {r34, r35}; mov.b64 %18, {r36, r37}; mov.b64 %19, {r38, r39};"
+        "mov.b64 %20, {r40, r41}; mov.b64 %21, {r42, r43}; mov.b64 %22, {r44, r45}; mov.b64 %23, {r46, r47};"
+        "mov.b64 %24, {r48, r49}; mov.b64 %25, {r50, r51}; mov.b64 %26, {r52, r53}; mov.b64 %27, {r54, r55};"
+        "mov.b64 %28, {r56, r57}; mov.b64 %29, {r58, r59}; mov.b64 %30, {r60, r61}; mov.b64 %31, {r62, r63};"
+        "}"
+        : "=l"(v[0]), "=l"(v[1]), "=l"(v[2]), "=l"(v[3]), "=l"(v[4]), "=l"(v[5]),
+          "=l"(v[6]), "=l"(v[7]), "=l"(v[8]), "=l"(v[9]), "=l"(v[10]), "=l"(v[11]),
+          "=l"(v[12]), "=l"(v[13]), "=l"(v[14]), "=l"(v[15]), "=l"(v[16]), "=l"(v[17]),
+          "=l"(v[18]), "=l"(v[19]), "=l"(v[20]), "=l"(v[21]), "=l"(v[22]), "=l"(v[23]),
+          "=l"(v[24]), "=l"(v[25]), "=l"(v[26]), "=l"(v[27]), "=l"(v[28]), "=l"(v[29]),
+          "=l"(v[30]), "=l"(v[31])
+        : "r"(taddr)
+        : "memory");
 }
 
 // Shared-memory matrix descriptor of a K-major tile stored as 128-byte rows
