@@ -745,30 +745,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 const int n = min(128, t.n - rank * 128);
                 for (int k0 = 0; k0 < KB; k0 += kPairGroup, ++is) {
                     const uint32_t q = is % kPairSlots;
-#pragma unroll
+                    float* o = sc + q * (kPairScale / 4) + lane;
+#pragma unroll 1
                     for (int part = 0; part < kPairGroup; part += 4) {
                         const int kb = k0 + part;
-                        float x[4][4], w0[4], w1[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const bool in = kb + e < KB;
-                            w0[e] = in ? t.s0[kb + e] : 0.0f;
-                            w1[e] = in ? t.s1[kb + e] : 0.0f;
-                        }
+                        float4 x[4];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const int r = j * 32 + lane;
-                            const float* p =
-                                a.sx + size_t(t.row0 + rank * 128 + (r < n ? r : 0)) * KB + kb;
-                            if (r >= n || kb >= KB) {
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) x[j][e] = 0.0f;
-                            } else if (vec) {
-                                const float4 v = *reinterpret_cast<const float4*>(p);
-                                x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) x[j][e] = kb + e < KB ? p[e] : 0.0f;
+                            x[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (r < n && kb < KB) {
+                                const float* p = a.sx + size_t(t.row0 + rank * 128 + r) * KB + kb;
+                                if (vec) {
+                                    x[j] = *reinterpret_cast<const float4*>(p);
+                                } else {
+                                    x[j].x = p[0];
+                                    if (kb + 1 < KB) x[j].y = p[1];
+                                    if (kb + 2 < KB) x[j].z = p[2];
+                                    if (kb + 3 < KB) x[j].w = p[3];
+                                }
                             }
                         }
                         if (part == 0 &&
@@ -776,14 +771,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                             ok = false;
                             break;
                         }
-                        float* o = sc + q * (kPairScale / 4) + part * 256 + lane;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
+                        for (int e = 0; e < 4; ++e) {
+                            const bool in = kb + e < KB;
+                            const float w0 = in ? t.s0[kb + e] : 0.0f;
+                            const float w1 = in ? t.s1[kb + e] : 0.0f;
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                o[e * 256 + j * 32] = x[j][e] * w0[e];
-                                o[e * 256 + 128 + j * 32] = x[j][e] * w1[e];
+                                const float v = e == 0 ? x[j].x : e == 1 ? x[j].y : e == 2 ? x[j].z : x[j].w;
+                                o[e * 256 + j * 32] = v * w0;
+                                o[e * 256 + 128 + j * 32] = v * w1;
                             }
+                        }
+                        o += 4 * 256;
                     }
                     if (!ok) break;
                     __syncwarp();
