@@ -3,32 +3,38 @@
 // expert segments (hf_route_logits). topKScores (compute/moe_router.h:29-57) is
 // the case of a sigmoid, one group and k <= 8.
 //
-// One warp per token; lane i holds experts i, i + 32, ... . Scores become
-// order-preserving integer codes (0: not in the choice; 1: NaN; then the
-// numbers), so one round of the choice is a scan of the lane's codes, a
-// redux.sync and, among equal codes, the lowest id.
+// One warp per token; lane i holds experts i, i + 32, ... . Keys become
+// order-preserving integers (0: not in the choice; then NaN; then the numbers)
+// whose lowest bits are replaced by the expert's place in its lane, inverted:
+// one integer maximum then finds the best key and, among equal ones, the lowest
+// id. A lane sorts its keys once (min / max network); a round of the choice is a
+// redux.sync over the lanes' first keys, and the winner moves its list up.
 //
 // Which expert ranks before which is decided as in 64-bit arithmetic, without
-// paying for it: without a bias the score is monotone in the logit, so the
-// logits' own codes rank exactly. With a bias the round runs on fp32 keys
-// whose error is bounded, and a token whose consecutive picks (or whose last
-// kept and first dropped group) are closer than twice that bound is redone on
-// 64-bit keys. At 256 experts that is about one token in a few hundred.
+// paying for it. Without a bias the score is monotone in the logit, so the
+// logits rank exactly (up to the replaced bits). With a bias the keys are fp32
+// sums whose error is bounded. Where consecutive picks are closer than the bound
+// the choice goes on until one is clearly below, and the candidates (one a lane)
+// are ranked again by their 64-bit keys: at 256 experts about one token in two
+// hundred. A token whose last kept and first dropped group are that close is
+// redone in 64 bits from its logits.
 //
 // The permutation: tokens are cut into blocks; a block keeps, per expert, one
 // bit per token, so a slot's rank in its segment is a popcount, whatever the
-// order of the atomics. Up to 128 tokens one block does everything; beyond, a
+// order of the atomics. Up to 16 tokens one block does everything; beyond, a
 // second launch adds the counts of the blocks before its own.
 #include "hf_internal.cuh"
 
 #include <math.h>
+
+#include <algorithm>
 
 namespace hf {
 namespace {
 
 constexpr int kMaxRouteK = 32;      // one lane per pick
 constexpr int kMaxRouteGroups = 32;
-constexpr int kOneBlockT = 128;     // tokens one block routes and permutes in one launch
+constexpr int kOneBlockT = 16;      // tokens one block routes and permutes in one launch
 constexpr size_t kWsAlign = 256;
 
 struct LogitArgs {
@@ -47,22 +53,28 @@ struct LogitArgs {
 };
 
 // ------------------------------------------------------------------ codes
+// -inf is 0x007fffff (and 0x000f... in 64 bits); NaN takes kNanCode below it,
+// above the place bits.
+constexpr uint32_t kNanCode = 0x40u;
 __device__ __forceinline__ uint32_t code_of(float v) {
-    if (v != v) return 1u;
     const uint32_t b = __float_as_uint(v + 0.0f);  // -0 ranks as +0
-    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+    const uint32_t c = b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u);
+    return v == v ? c : kNanCode;
 }
+// Of a code with its place bits cleared: -inf's own code is then the lowest NaN
+// pattern, so everything up to it reads as -inf.
 __device__ __forceinline__ float value_of(uint32_t c) {
-    if (c <= 1u) return c ? __uint_as_float(0x7fc00000u) : -INFINITY;
+    if (c <= 0x007fffffu) return c == kNanCode ? __uint_as_float(0x7fc00000u) : -INFINITY;
     return __uint_as_float((c & 0x80000000u) ? (c & 0x7fffffffu) : ~c);
 }
 __device__ __forceinline__ unsigned long long code_of(double v) {
-    if (v != v) return 1ull;
+    if (v != v) return kNanCode;
     const unsigned long long b = (unsigned long long)__double_as_longlong(v + 0.0);
     return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
 }
 __device__ __forceinline__ double value_of(unsigned long long c) {
-    if (c <= 1ull) return c ? __longlong_as_double(0x7ff8000000000000ll) : double(-INFINITY);
+    if (c <= 0x000fffffffffffffull)
+        return c == kNanCode ? __longlong_as_double(0x7ff8000000000000ll) : double(-INFINITY);
     return __longlong_as_double((long long)((c >> 63) ? (c & 0x7fffffffffffffffull) : ~c));
 }
 __device__ __forceinline__ uint32_t warp_max(uint32_t c) { return __reduce_max_sync(~0u, c); }
@@ -73,79 +85,111 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long c) {
     return ((unsigned long long)mh << 32) | ml;
 }
 
-// How far a is above b beyond the roundings of two fp32 sums (2^-24 of each, and
-// as much again of the parts added): negative when they could be either way.
-__device__ __forceinline__ float above(float a, float b) {
-    return (a - b) - 0x1p-22f * (fabsf(a) + fabsf(b));
-}
-__device__ __forceinline__ double above(double a, double b) { return a - b; }
-
-// The lane holding the lowest id among the lanes whose best code is `m`; every
-// lane gets that id.
-template <typename C>
-__device__ __forceinline__ int lowest_id(C best, C m, int id) {
-    const unsigned cand = __ballot_sync(~0u, best == m);
-    if ((cand & (cand - 1u)) == 0u) return __shfl_sync(~0u, id, __ffs(cand) - 1);
-    return __reduce_min_sync(~0u, best == m ? id : 0x7fffffff);
-}
+// Low bits of a code that hold the expert's place j in its lane (as NPL - 1 - j).
+template <int NPL>
+struct Place {
+    static constexpr int kBits = NPL == 1 ? 0 : NPL == 2 ? 1 : NPL == 4 ? 2 : NPL == 8 ? 3
+                                 : NPL == 16 ? 4 : 5;
+    static constexpr uint32_t kMask = (1u << kBits) - 1u;
+};
 
 template <int NPL, typename C>
-__device__ __forceinline__ void lane_best(const C (&c)[NPL], int lane, C& best, int& id) {
-    best = 0;
-    id = lane;
+__device__ __forceinline__ C packed(C code, int j) {
+    return (code & ~C(Place<NPL>::kMask)) | C(NPL - 1 - j);
+}
+template <int NPL, typename C>
+__device__ __forceinline__ auto value_at(C packed_code) {
+    return value_of(packed_code & ~C(Place<NPL>::kMask));
+}
+
+// How far the key of code a is above that of code b, beyond what the fp32 sums
+// (2^-23 of each) and the replaced bits (2^(kBits - 23)) may hide: not positive
+// when either could be the larger. On 64-bit keys the replaced bits are far below
+// any difference of interest.
+template <int NPL>
+__device__ __forceinline__ float beyond(float diff, float size) {
+    constexpr float kRel = float(2 + (1 << Place<NPL>::kBits)) * 0x1p-23f;
+    return diff - kRel * size;
+}
+template <int NPL>
+__device__ __forceinline__ double beyond(double diff, double) {
+    return diff;
+}
+template <int NPL, typename C>
+__device__ __forceinline__ auto above(C a, C b) {
+    const auto x = value_at<NPL>(a), y = value_at<NPL>(b);
+    return beyond<NPL>(x - y, fabs(x) + fabs(y));
+}
+
+// Descending sort of a lane's codes: Batcher's merge exchange.
+template <int NPL, typename C>
+__device__ __forceinline__ void sort_lane(C (&c)[NPL]) {
 #pragma unroll
-    for (int j = 0; j < NPL; ++j)
-        if (c[j] > best) {  // strict: the lane's lowest id on equal codes
-            best = c[j];
-            id = j * 32 + lane;
-        }
+    for (int p = 1; p < NPL; p <<= 1)
+#pragma unroll
+        for (int k = p; k >= 1; k >>= 1)
+#pragma unroll
+            for (int j = k % p; j + k < NPL; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < NPL && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const C hi = max(c[i + j], c[i + j + k]), lo = min(c[i + j], c[i + j + k]);
+                        c[i + j] = hi;
+                        c[i + j + k] = lo;
+                    }
 }
 
 // Drops the experts of the groups that are not kept (their codes become 0).
-// `gc` are the codes whose values are summed for a group's score. *gap: how far
-// the last kept group is above the best dropped one.
+// `gc` are the packed codes whose values are summed for a group's score; lane g
+// scans group g's codes in the warp's scratch `scr` [E], from a place of its own
+// so that groups of 32 do not meet in one bank. *gap: how far the last kept group
+// is above the best dropped one.
 template <int NPL, typename C, typename F>
 __device__ __forceinline__ void keep_groups(C (&c)[NPL], const C (&gc)[NPL], const LogitArgs& a,
-                                            int lane, F* gap) {
+                                            int lane, C* scr, F* gap) {
     const int gs = a.E / a.n_group;
-    C mine = 0;  // lane g: the code of group g's score
-#pragma unroll 1
-    for (int g = 0; g < a.n_group; ++g) {
-        C t[NPL], best;
-        int id;
+    __syncwarp();
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) {
-            const int e = j * 32 + lane;
-            t[j] = (e >= g * gs && e < (g + 1) * gs) ? gc[j] : C(0);
+    for (int j = 0; j < NPL; ++j)
+        if (j * 32 + lane < a.E) scr[j * 32 + lane] = gc[j];
+    __syncwarp();
+    C b1 = 0, b2 = 0, code = 0;  // the best two keys of group `lane`, its score's code
+    F size = 0;                  // and the magnitudes that were added
+    if (lane < a.n_group) {
+        const C* g = scr + lane * gs;
+        int i = lane % gs;
+#pragma unroll 4
+        for (int q = 0; q < gs; ++q) {
+            // places differ inside a lane's codes only: equal keys of two lanes may
+            // be equal codes, and count twice all the same
+            const C v = g[i];
+            b2 = max(b2, min(b1, v));
+            b1 = max(b1, v);
+            if (++i == gs) i = 0;
         }
-        lane_best(t, lane, best, id);
-        const C m1 = warp_max(best);
-        F s = value_of(m1);
+        F s = value_at<NPL>(b1);
+        size = fabs(s);
         if (a.group_top == 2 && gs > 1) {
-            const int w = lowest_id(best, m1, id);
-#pragma unroll
-            for (int j = 0; j < NPL; ++j)
-                if (j * 32 + lane == w) t[j] = 0;
-            lane_best(t, lane, best, id);
-            s = s + value_of(warp_max(best));
+            const F s2 = value_at<NPL>(b2);
+            s = s + s2;
+            size = size + fabs(s2);
         }
-        if (lane == g) mine = code_of(s);
+        code = code_of(s);
     }
     // rank of lane's group: the groups before it
     int rank = 0;
-#pragma unroll 1
+#pragma unroll 4
     for (int g = 0; g < a.n_group; ++g) {
-        const C o = __shfl_sync(~0u, mine, g);
-        rank += (o > mine) || (o == mine && g < lane);
+        const C o = __shfl_sync(~0u, code, g);
+        rank += (o > code) || (o == code && g < lane);
     }
     const bool in = lane < a.n_group && rank < a.topk_group;
     const unsigned kept = __ballot_sync(~0u, in);
-    if (a.topk_group < a.n_group) {
-        const unsigned last = __ballot_sync(~0u, lane < a.n_group && rank == a.topk_group - 1);
-        const unsigned next = __ballot_sync(~0u, lane < a.n_group && rank == a.topk_group);
-        *gap = above(value_of(__shfl_sync(~0u, mine, __ffs(last) - 1)),
-                     value_of(__shfl_sync(~0u, mine, __ffs(next) - 1)));
-    }
+    const unsigned last = __ballot_sync(~0u, lane < a.n_group && rank == a.topk_group - 1);
+    const unsigned next = __ballot_sync(~0u, lane < a.n_group && rank == a.topk_group);
+    const int ll = __ffs(last) - 1, ln = __ffs(next) - 1;
+    *gap = beyond<NPL>(value_of(__shfl_sync(~0u, code, ll)) - value_of(__shfl_sync(~0u, code, ln)),
+                       __shfl_sync(~0u, size, ll) + __shfl_sync(~0u, size, ln));
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
         const int e = j * 32 + lane;
@@ -153,27 +197,44 @@ __device__ __forceinline__ void keep_groups(C (&c)[NPL], const C (&gc)[NPL], con
     }
 }
 
-// The k best codes in rank order: lane r gets the r-th pick's id. *gap: the
-// smallest distance of consecutive ones (the first one left out included).
-template <int NPL, typename C, typename F>
-__device__ __forceinline__ int pick(C (&c)[NPL], int k, int lane, F* gap) {
-    int mine = 0;
-    F prev = 0;
-#pragma unroll 1
-    for (int r = 0; r <= k; ++r) {
-        C best;
-        int id;
-        lane_best(c, lane, best, id);
-        const C m = warp_max(best);
-        if (m == 0) break;  // after k picks of k experts
-        if (r) *gap = fmin(*gap, above(prev, value_of(m)));  // fmin passes over NaN (inf - inf)
-        if (r == k) break;
-        prev = value_of(m);
-        const int w = lowest_id(best, m, id);
-        if (lane == r) mine = w;
+// Takes the best code of the warp out of the lanes' sorted lists: its packed code
+// (0 when none is left), and the id in *id.
+template <int NPL, typename C>
+__device__ __forceinline__ C take_best(C (&c)[NPL], int lane, int* id) {
+    const C m = warp_max(c[0]);
+    // equal codes have equal places, so the lowest lane has the lowest id
+    const int w = __ffs(__ballot_sync(~0u, c[0] == m)) - 1;
+    *id = (NPL - 1 - int(uint32_t(m) & Place<NPL>::kMask)) * 32 + w;
+    const bool mine = lane == w;
 #pragma unroll
-        for (int j = 0; j < NPL; ++j)
-            if (j * 32 + lane == w) c[j] = 0;
+    for (int j = 0; j + 1 < NPL; ++j) c[j] = mine ? c[j + 1] : c[j];
+    if (mine) c[NPL - 1] = 0;
+    return m;
+}
+
+// Whether code b (<= a) is not clearly below a: the codes are equal but for the
+// place (`exact`), or not more than tol apart; a NaN difference (inf - inf)
+// counts as close.
+template <int NPL, typename C, typename F>
+__device__ __forceinline__ bool is_close(C a, C b, bool exact, F tol) {
+    const C place = C(Place<NPL>::kMask);
+    return exact ? (a | place) == (b | place) : !(above<NPL>(a, b) > tol);
+}
+
+// Ranks n candidates (lane r < n: an id and its code) by code and id: lane r
+// gets the id of rank r.
+__device__ __forceinline__ int rank_again(unsigned long long code, int id, int n, int lane) {
+    int rank = 0, mine = 0;
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+        const unsigned long long o = __shfl_sync(~0u, code, i);
+        const int oid = __shfl_sync(~0u, id, i);
+        rank += o > code || (o == code && oid < id);
+    }
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+        const int ri = __shfl_sync(~0u, rank, i), oid = __shfl_sync(~0u, id, i);
+        if (ri == lane) mine = oid;
     }
     return mine;
 }
@@ -189,113 +250,170 @@ __device__ __forceinline__ float warp_max_f(float v) {
     return v;
 }
 
-// The choice on 64-bit keys (rare: out of line, so that the common path keeps
-// its registers).
-template <int NPL>
-__device__ __noinline__ int pick_exact(const LogitArgs& a, int t, int lane) {
-    unsigned long long c[NPL];
-    double mx = -INFINITY, sum = 0.0;
-    if (a.score == HF_SCORE_SOFTMAX) {
-        float m = -INFINITY;
-        for (int e = lane; e < a.E; e += 32) m = fmaxf(m, load_logit(a, size_t(t) * a.E + e));
-        mx = warp_max_f(m);
-        for (int e = lane; e < a.E; e += 32) {
-            const double l = load_logit(a, size_t(t) * a.E + e);
-            sum += l == -INFINITY ? 0.0 : exp(l - mx);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+// Maximum of token t's logits, and in 64 bits the sum of their exponentials.
+__device__ __forceinline__ double softmax_sum(const LogitArgs& a, int t, int lane, double* mx) {
+    float m = -INFINITY;
+    for (int e = lane; e < a.E; e += 32) m = fmaxf(m, load_logit(a, size_t(t) * a.E + e));
+    *mx = warp_max_f(m);
+    double sum = 0.0;
+#pragma unroll 1
+    for (int e = lane; e < a.E; e += 32) {
+        const double l = load_logit(a, size_t(t) * a.E + e);
+        sum += l == -INFINITY ? 0.0 : exp(l - *mx);
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    return sum;
+}
+
+__device__ __forceinline__ double key64(const LogitArgs& a, int t, int e, double mx, double sum) {
+    const double l = load_logit(a, size_t(t) * a.E + e);
+    double p;
+    if (a.score == HF_SCORE_SIGMOID) p = 1.0 / (1.0 + exp(-l));
+    else p = l == -INFINITY ? 0.0 : exp(l - mx) / sum;
+    return p + (a.bias ? double(a.bias[e]) : 0.0);
+}
+
+// The candidates' order by logit, or by 64-bit key.
+__device__ __noinline__ int refine(const LogitArgs& a, int t, int lane, int id, int n) {
+    unsigned long long code;
+    if (a.bias == nullptr) {
+        code = code_of(load_logit(a, size_t(t) * a.E + id));
+    } else {
+        double mx = 0.0, sum = 1.0;
+        if (a.score == HF_SCORE_SOFTMAX) sum = softmax_sum(a, t, lane, &mx);
+        code = code_of(key64(a, t, id, mx, sum));
+    }
+    return rank_again(code, id, n, lane);
+}
+
+// The whole choice in 64 bits (groups too close to tell apart, more candidates
+// than lanes).
+template <int NPL>
+__device__ __noinline__ int pick_exact(const LogitArgs& a, int t, int lane,
+                                       unsigned long long* scr) {
+    unsigned long long c[NPL];
+    double mx = 0.0, sum = 1.0;
+    if (a.score == HF_SCORE_SOFTMAX) sum = softmax_sum(a, t, lane, &mx);
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
         const int e = j * 32 + lane;
-        c[j] = 0;
-        if (e < a.E) {
-            const double l = load_logit(a, size_t(t) * a.E + e);
-            double p;
-            if (a.score == HF_SCORE_SIGMOID) p = 1.0 / (1.0 + exp(-l));
-            else p = l == -INFINITY ? 0.0 : exp(l - mx) / sum;
-            c[j] = code_of(p + (a.bias ? double(a.bias[e]) : 0.0));
-        }
+        c[j] = e < a.E ? packed<NPL>(code_of(key64(a, t, e, mx, sum)), j) : 0ull;
     }
-    double gap = INFINITY;
-    if (a.topk_group < a.n_group) keep_groups(c, c, a, lane, &gap);
-    return pick(c, a.k, lane, &gap);
+    double gap;
+    if (a.topk_group < a.n_group) keep_groups(c, c, a, lane, scr, &gap);
+    if (a.bias == nullptr) {  // by logit, whose codes lose nothing in 64 bits
+#pragma unroll
+        for (int j = 0; j < NPL; ++j)
+            if (c[j])
+                c[j] = ((unsigned long long)code_of(load_logit(a, size_t(t) * a.E + j * 32 + lane))
+                        << 32) | (unsigned long long)(NPL - 1 - j);
+    }
+    sort_lane(c);
+    int mine = 0;
+#pragma unroll 1
+    for (int r = 0; r < a.k; ++r) {
+        int id;
+        take_best(c, lane, &id);
+        if (lane == r) mine = id;
+    }
+    return mine;
 }
 
 // Scores, choice and weights of token t. Lane r < k returns its pick's id.
 template <int NPL>
-__device__ __forceinline__ int route_token(const LogitArgs& a, int t, int lane) {
-    float s[NPL];
-    uint32_t c[NPL];
-#pragma unroll
-    for (int j = 0; j < NPL; ++j) {
-        const int e = j * 32 + lane;
-        s[j] = e < a.E ? load_logit(a, size_t(t) * a.E + e) : -INFINITY;
-        c[j] = e < a.E ? code_of(s[j]) : 0u;
-    }
-    if (a.score == HF_SCORE_SIGMOID) {
-#pragma unroll
-        for (int j = 0; j < NPL; ++j) s[j] = __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-s[j])));
-    } else {
-        float m = s[0];
-#pragma unroll
-        for (int j = 1; j < NPL; ++j) m = fmaxf(m, s[j]);
-        m = warp_max_f(m);
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < NPL; ++j) {
-            s[j] = s[j] == -INFINITY ? 0.0f : expf(s[j] - m);
-            sum += s[j];
-        }
-        sum = warp_sum(sum);
-        const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);  // 0: every logit is -inf
-#pragma unroll
-        for (int j = 0; j < NPL; ++j) s[j] = __fmul_rn(s[j], inv);
-    }
-    // The bound on a fp32 score's error, for scores up to smax. Sigmoid: expf
-    // 2^-22, the sum, the quotient: < 2^-21 smax. Softmax: the exponent's
-    // rounding (|x e^-x| <= 0.37, 2^-24 each), expf, a sum of 1024 terms in
-    // NPL + 5 roundings, the reciprocal and product: < 2^-18 smax. Two keys can
-    // be off by twice that (tol), two groups' sums of two by four times; the
-    // roundings of the sums themselves are above()'s.
+__device__ __forceinline__ int route_token(const LogitArgs& a, const float (&bias)[NPL], int t,
+                                           int lane, unsigned long long* scr) {
     const bool by_logit = a.bias == nullptr;
     const bool limited = a.topk_group < a.n_group;
-    float tol = 0.0f;
-    float gap = INFINITY, ggap = INFINITY;
+    const bool softmax = a.score == HF_SCORE_SOFTMAX;
+    float l[NPL];
+    uint32_t c[NPL];
+#pragma unroll
+    for (int j = 0; j < NPL; ++j)
+        l[j] = j * 32 + lane < a.E ? load_logit(a, size_t(t) * a.E + j * 32 + lane) : -INFINITY;
+    float top = l[0];
+#pragma unroll
+    for (int j = 1; j < NPL; ++j) top = fmaxf(top, l[j]);
+    top = warp_max_f(top);
+    const float m = top == -INFINITY ? 0.0f : top;  // exp(-inf - 0) = 0
+    float inv = 1.0f;
+    if (softmax) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) sum += __expf(l[j] - m);
+        sum = warp_sum(sum);
+        inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);  // 0: every logit is -inf
+    }
+    float tol = 0.0f, ggap = INFINITY;
     if (!by_logit || (limited && a.group_top == 2)) {
+        // Keys on the fast exponential (2 + 1.2 |x| units of 2^-23). Bounds on a
+        // score's error, for the largest score smax. Sigmoid: s (1 - s) times the
+        // exponential's, which is largest at the largest logit, and the sum and
+        // quotient: < smax (2^-21 + 2^-22 |top|, the latter where top < 0).
+        // Softmax: the exponent's rounding and the exponential's stay below 3 units
+        // (e^-x (2 + 1.2 x) <= 2), the sum's error below 3 and NPL + 5 roundings:
+        // < 2^-18 smax. Two keys can be off by twice that (tol), two groups' sums
+        // of two by four times; the roundings of the sums are above()'s.
         uint32_t key[NPL];
-        float smax = 0.0f;
 #pragma unroll
         for (int j = 0; j < NPL; ++j) {
-            const int e = j * 32 + lane;
-            key[j] = 0u;
-            if (e < a.E) {
-                const float v = by_logit ? s[j] : __fadd_rn(s[j], a.bias[e]);
-                key[j] = code_of(v);
-                smax = fmaxf(smax, s[j]);
-            }
+            const float s = softmax ? __expf(l[j] - m) * inv
+                                    : __fdividef(1.0f, 1.0f + __expf(-l[j]));
+            key[j] = j * 32 + lane < a.E ? packed<NPL>(code_of(s + bias[j]), j) : 0u;
         }
-        tol = warp_max_f(smax) * (a.score == HF_SCORE_SIGMOID ? 0x1p-20f : 0x1p-17f);
-        if (!by_logit) {
+        if (softmax) tol = inv * 0x1p-17f;
+        else tol = __fdividef(1.0f, 1.0f + __expf(-top)) *
+                   (0x1p-20f + fmaxf(-top, 0.0f) * 0x1p-21f);
 #pragma unroll
-            for (int j = 0; j < NPL; ++j) c[j] = key[j];
-        }
-        if (limited) keep_groups(c, key, a, lane, &ggap);
-    } else if (limited) {
-        keep_groups(c, c, a, lane, &ggap);
-        ggap = INFINITY;  // the logits rank exactly
+        for (int j = 0; j < NPL; ++j)
+            c[j] = !by_logit ? key[j]
+                             : j * 32 + lane < a.E ? packed<NPL>(code_of(l[j]), j) : 0u;
+        if (limited) keep_groups(c, key, a, lane, reinterpret_cast<uint32_t*>(scr), &ggap);
+    } else {
+#pragma unroll
+        for (int j = 0; j < NPL; ++j)
+            c[j] = j * 32 + lane < a.E ? packed<NPL>(code_of(l[j]), j) : 0u;
+        if (limited) keep_groups(c, c, a, lane, reinterpret_cast<uint32_t*>(scr), &ggap);
     }
-    int mine = pick(c, a.k, lane, &gap);
-    // not (gap > tol): a NaN or infinite difference is decided on 64-bit keys too
-    if (!(ggap > 2.0f * tol) || (!by_logit && !(gap > tol))) mine = pick_exact<NPL>(a, t, lane);
+    sort_lane(c);
+    int mine = 0;
+    uint32_t mc = 0;  // lane r < k: the r-th pick and its code
+#pragma unroll 1
+    for (int r = 0; r < a.k; ++r) {
+        int id;
+        const uint32_t m1 = take_best(c, lane, &id);
+        if (lane == r) {
+            mine = id;
+            mc = m1;
+        }
+    }
+    uint32_t left = warp_max(c[0]);  // the first one left out (0: none)
+    // Logits rank exactly but for the replaced bits, which bf16 logits leave 0.
+    const bool ranked = by_logit && a.bf16;
+    const uint32_t before = __shfl_up_sync(~0u, mc, 1);
+    bool close = lane > 0 && lane < a.k && is_close<NPL>(before, mc, by_logit, tol);
+    uint32_t last = __shfl_sync(~0u, mc, a.k - 1);
+    bool open = left && is_close<NPL>(last, left, by_logit, tol);
+    if (limited && !(ggap > 2.0f * tol) && !(ranked && a.group_top == 1)) {
+        mine = pick_exact<NPL>(a, t, lane, scr);
+    } else if (!ranked && (__any_sync(~0u, close) || open)) {
+        int n = a.k;  // candidates: on until one is clearly below
+        while (open && n < 32) {
+            int id;
+            last = take_best(c, lane, &id);
+            if (lane == n) mine = id;
+            ++n;
+            left = warp_max(c[0]);
+            open = left && is_close<NPL>(last, left, by_logit, tol);
+        }
+        mine = open ? pick_exact<NPL>(a, t, lane, scr) : refine(a, t, lane, mine, n);
+    }
 
-    float ws = 0.0f;  // the pick's score: from the lane that holds it
-#pragma unroll
-    for (int j = 0; j < NPL; ++j) {
-        const float v = __shfl_sync(~0u, s[j], mine & 31);
-        if (j == (mine >> 5)) ws = v;
-    }
+    // the picks' scores once more, accurately
+    const float lp = load_logit(a, size_t(t) * a.E + (lane < a.k ? mine : 0));
+    float ws = softmax ? __fmul_rn(expf(lp - m), inv)
+                       : __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-lp)));
     if (lane >= a.k) ws = 0.0f;
     float sum = 0.0f;  // rank order, as topKScores sums
 #pragma unroll 1
@@ -380,11 +498,12 @@ __device__ __forceinline__ void set_masks(const LogitArgs& a, uint32_t* masks, i
     }
 }
 
+// ids: of the block's tokens [nt x k]
 __device__ __forceinline__ void scatter(const LogitArgs& a, const uint32_t* masks, const int* base,
-                                        int t0, int nt, int words) {
+                                        const int* ids, int t0, int nt, int words) {
     for (int i = threadIdx.x; i < nt * a.k; i += blockDim.x) {
-        const int slot = t0 * a.k + i, e = a.ids[slot];
-        a.perm[base[e] + mask_rank(masks + e * words, i / a.k)] = slot;
+        const int e = ids[i];
+        a.perm[base[e] + mask_rank(masks + e * words, i / a.k)] = t0 * a.k + i;
     }
 }
 
@@ -393,18 +512,28 @@ __device__ __forceinline__ void scatter(const LogitArgs& a, const uint32_t* mask
 template <int NPL, int THREADS>
 __global__ void __launch_bounds__(THREADS) k_route_logits(LogitArgs a) {
     extern __shared__ __align__(16) uint32_t sm[];
-    const int words = a.tb / 32;
-    uint32_t* masks = sm;                                         // [E][words]
-    int* total = reinterpret_cast<int*>(sm + size_t(a.E) * words);  // [E]
+    const int words = (a.tb + 31) / 32;
+    // groups: a scratch row of 64-bit codes per warp, in front
+    auto* scr = reinterpret_cast<unsigned long long*>(sm) + size_t(threadIdx.x >> 5) * a.E;
+    uint32_t* masks = sm + (a.topk_group < a.n_group ? size_t(blockDim.x >> 5) * a.E * 2 : 0);
+    int* total = reinterpret_cast<int*>(masks + size_t(a.E) * words);  // [E]; masks [E][words]
     int* base = total + a.E;                                      // [E]
     const int t0 = blockIdx.x * a.tb, nt = min(a.tb, a.T - t0);
+    int* s_ids = base + a.E;                                      // [tb][k] (one block)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     griddep_launch_dependents();
+    float bias[NPL];
+#pragma unroll
+    for (int j = 0; j < NPL; ++j)
+        bias[j] = a.bias && j * 32 + lane < a.E ? a.bias[j * 32 + lane] : 0.0f;
     for (int i = threadIdx.x; i < a.E * words; i += blockDim.x) masks[i] = 0u;
     __syncthreads();
-    for (int tl = warp; tl < nt; tl += THREADS / 32) {
-        const int id = route_token<NPL>(a, t0 + tl, lane);
-        if (lane < a.k) atomicOr(&masks[id * words + (tl >> 5)], 1u << (tl & 31));
+    for (int tl = warp; tl < nt; tl += int(blockDim.x >> 5)) {
+        const int id = route_token<NPL>(a, bias, t0 + tl, lane, scr);
+        if (lane < a.k) {
+            atomicOr(&masks[id * words + (tl >> 5)], 1u << (tl & 31));
+            if (gridDim.x == 1) s_ids[tl * a.k + lane] = id;
+        }
     }
     __syncthreads();
     for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
@@ -417,12 +546,12 @@ __global__ void __launch_bounds__(THREADS) k_route_logits(LogitArgs a) {
     if (gridDim.x > 1) return;
     __syncthreads();
     segment_bases(a, total, base, true);
-    scatter(a, masks, base, t0, nt, words);
+    scatter(a, masks, base, s_ids, t0, nt, words);
 }
 
 __global__ void __launch_bounds__(1024) k_route_scatter(LogitArgs a, int nb) {
     extern __shared__ __align__(16) uint32_t sm[];
-    const int words = a.tb / 32;
+    const int words = (a.tb + 31) / 32;
     uint32_t* masks = sm;
     int* total = reinterpret_cast<int*>(sm + size_t(a.E) * words);
     int* base = total + a.E;
@@ -451,7 +580,7 @@ __global__ void __launch_bounds__(1024) k_route_scatter(LogitArgs a, int nb) {
     set_masks(a, masks, t0, nt, words);
     __syncthreads();
     segment_bases(a, total, base, b == 0);
-    scatter(a, masks, base, t0, nt, words);
+    scatter(a, masks, base, a.ids + size_t(t0) * a.k, t0, nt, words);
 }
 
 __global__ void k_route_empty(LogitArgs a) {
@@ -461,13 +590,14 @@ __global__ void k_route_empty(LogitArgs a) {
     }
 }
 
-// Tokens per block: 128 routed by one block; else 32 while that leaves at most
-// two blocks per SM (a block's warps then have one token each), 128, and 512
-// where the second launch would add up too many blocks' counts.
+// Tokens per block: all of up to 16 tokens in one; else the smallest power of two
+// from 8 on that leaves at most one block per SM, 512 at most (the second launch
+// adds up the counts of all blocks).
 int tokens_per_block(int T) {
     if (T <= kOneBlockT) return kOneBlockT;
-    if (T <= 2 * 148 * 32) return 32;
-    return T <= 65536 ? 128 : 512;
+    int tb = 8;
+    while (tb < 512 && (T + tb - 1) / tb > 148) tb *= 2;
+    return tb;
 }
 
 int blocks_of(int T) {
@@ -485,14 +615,18 @@ hf_status launch(const LogitArgs& a, cudaStream_t st) {
     // registers: NPL scores and codes per lane (and 64-bit ones in the rare path)
     constexpr int kThreads = NPL <= 8 ? 1024 : 256;
     const int nb = blocks_of(a.T);
-    const int smem = a.E * (a.tb / 32 + 2) * 4;
+    const int smem = a.E * ((a.tb + 31) / 32 + 2) * 4;
     const auto kern = k_route_logits<NPL, kThreads>;
-    HF_CUDA(ensure_smem(reinterpret_cast<const void*>(kern), smem));
-    kern<<<nb, kThreads, smem, st>>>(a);
+    // a warp per token, eight at least (they also count and permute)
+    const int threads = std::min(kThreads, std::max(8, std::min(a.T, a.tb)) * 32);
+    const int own = smem + (nb == 1 ? a.T * a.k * 4 : 0) +
+                    (a.topk_group < a.n_group ? threads / 32 * a.E * 8 : 0);
+    HF_CUDA(ensure_smem(reinterpret_cast<const void*>(kern), own));
+    kern<<<nb, threads, own, st>>>(a);
     HF_CUDA(cudaGetLastError());
     if (nb > 1) {
         HF_CUDA(ensure_smem(reinterpret_cast<const void*>(k_route_scatter), smem));
-        HF_CUDA(launch_pdl(k_route_scatter, dim3(nb), dim3(1024), size_t(smem), st, a, nb));
+        HF_CUDA(launch_pdl(k_route_scatter, dim3(nb), dim3(nb > 16 ? 1024 : 256), size_t(smem), st, a, nb));
     }
     return HF_OK;
 }

@@ -383,7 +383,7 @@ def _route_spec(E, top_k, score, n_group, topk_group, group_top, scale, norm):
 
 
 def route_workspace_size(T: int, num_experts: int, top_k: int) -> int:
-    """Bytes of scratch of route_logits over T tokens (0 up to 128 tokens)."""
+    """Bytes of scratch of route_logits over T tokens (0 up to 16 tokens)."""
     spec = _route_spec(num_experts, top_k, "sigmoid", 1, 1, 1, 1.0, True)
     return int(_lib.lib().hf_route_workspace_size(T, ctypes.byref(spec)))
 

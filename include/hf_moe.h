@@ -338,7 +338,7 @@ HF_API size_t hf_route_workspace_size(int T, const hf_route_spec* spec);
  * routing->topk_ids [T x k], topk_weights [T x k], counts [E+1], offsets [E+2]
  * and perm [T*k] (the shared group E is empty); all five are required, margins
  * and slot_out must be NULL. T = 0 writes zero counts and offsets. workspace:
- * device scratch of hf_route_workspace_size bytes (0 and NULL up to 128 tokens),
+ * device scratch of hf_route_workspace_size bytes (0 and NULL up to 16 tokens),
  * 256-byte aligned, used in stream order only. Asynchronous on `stream`. */
 HF_API hf_status hf_route_logits(const void* logits, hf_dtype dtype, const float* bias, int T,
                                  const hf_route_spec* spec, const hf_moe_routing* routing,

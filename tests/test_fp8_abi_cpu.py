@@ -55,9 +55,9 @@ def test_route_refusals():
         assert L.hf_last_error(), b
     assert L.hf_route_logits(P, 1, None, 4, None, None, None, 0, None) == _lib.HF_ERR_ARG
     assert L.hf_route_logits(P, 1, None, 4, spec(), None, None, 0, None) == _lib.HF_ERR_ARG
-    assert L.hf_route_workspace_size(128, spec()) == 0
-    assert L.hf_route_workspace_size(129, spec()) > 0
-    assert L.hf_route_workspace_size(129, spec(top_k=0)) == 0
+    assert L.hf_route_workspace_size(16, spec()) == 0
+    assert L.hf_route_workspace_size(17, spec()) > 0
+    assert L.hf_route_workspace_size(17, spec(top_k=0)) == 0
 
 
 def test_quantize_refusals():
