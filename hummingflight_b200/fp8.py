@@ -9,12 +9,19 @@ falls back to the CPU.
 """
 from __future__ import annotations
 
+import functools
+
+import torch
 
 from . import _lib
-from ._lib import HfError, HfMoeRouting, call
-from .moe import _ACT, _dtype_code, _ptr, _stream, _torch, check_tensor, on_device, scratch
+from ._lib import HF_BF16, HF_F32, HfError, HfMoeRouting, call
+from .moe import _ACT, _ptr, _stream, check_tensor, on_device, scratch
 
 BLOCK = 128
+_Q = (torch.float8_e4m3fn, torch.uint8)
+_X = (torch.bfloat16, torch.float32)
+_F32 = (torch.float32,)
+_I32 = (torch.int32,)
 
 
 def blocks(n: int) -> int:
@@ -22,33 +29,26 @@ def blocks(n: int) -> int:
     return (n + BLOCK - 1) // BLOCK
 
 
-def _q_types():
-    torch = _torch()
-    return (torch.float8_e4m3fn, torch.uint8)
-
-
-def _act_types():
-    torch = _torch()
-    return (torch.bfloat16, torch.float32)
+def _code(dtype) -> int:
+    return HF_F32 if dtype == torch.float32 else HF_BF16
 
 
 def quantize(x, q=None, scales=None, stream=None):
     """Rows x [T x K] (device, bf16 or fp32; the rows may lie apart) -> e4m3
     [T x K] and power-of-two fp32 scales [T x ceil(K/128)]. K a multiple of 16."""
-    torch = _torch()
     T, K = x.shape
-    check_tensor("x", x, _act_types(), (T, K), rows=True)
+    check_tensor("x", x, _X, (T, K), rows=True)
     dev = x.device
     if q is None:
         q = torch.empty((T, K), dtype=torch.float8_e4m3fn, device=dev)
     else:
-        check_tensor("q", q, _q_types(), (T, K), dev)
+        check_tensor("q", q, _Q, (T, K), dev)
     if scales is None:
         scales = torch.empty((T, blocks(K)), dtype=torch.float32, device=dev)
     else:
-        check_tensor("scales", scales, (torch.float32,), (T, blocks(K)), dev)
+        check_tensor("scales", scales, _F32, (T, blocks(K)), dev)
     with on_device(dev, stream) as s:
-        call("hf_fp8_quantize", x.data_ptr(), _dtype_code(x), _pitch(x), T, K, q.data_ptr(),
+        call("hf_fp8_quantize", x.data_ptr(), _code(x.dtype), _pitch(x), T, K, q.data_ptr(),
              scales.data_ptr(), s)
     return q, scales
 
@@ -58,6 +58,7 @@ def _pitch(x):
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
+@functools.lru_cache(maxsize=256)
 def gemm_workspace_size(T: int, N: int, K: int) -> int:
     return int(_lib.lib().hf_fp8_gemm_workspace_size(T, N, K))
 
@@ -68,27 +69,27 @@ def gemm(xq, sx, wq, sw, out=None, out_dtype: str = "bf16", workspace=None, stre
     ceil(K/128)] -> [T x N] bf16 or fp32 (the type of `out` when given).
     `workspace`: uint8 scratch of gemm_workspace_size bytes, kept by callers that
     check :func:`status`."""
-    torch = _torch()
     T, K = xq.shape
     N = wq.shape[0]
     dev = xq.device
-    check_tensor("xq", xq, _q_types(), (T, K))
-    check_tensor("sx", sx, (torch.float32,), (T, blocks(K)), dev)
-    check_tensor("wq", wq, _q_types(), (N, K), dev)
-    check_tensor("sw", sw, (torch.float32,), (blocks(N), blocks(K)), dev)
+    check_tensor("xq", xq, _Q, (T, K))
+    check_tensor("sx", sx, _F32, (T, blocks(K)), dev)
+    check_tensor("wq", wq, _Q, (N, K), dev)
+    check_tensor("sw", sw, _F32, (blocks(N), blocks(K)), dev)
     if out is None:
         out = torch.empty((T, N), dtype=torch.float32 if out_dtype == "f32" else torch.bfloat16,
                           device=dev)
     else:
-        check_tensor("out", out, _act_types(), (T, N), dev)
+        check_tensor("out", out, _X, (T, N), dev)
     with on_device(dev, stream) as s:
-        need = int(_lib.lib().hf_fp8_gemm_workspace_size(T, N, K))
+        need = gemm_workspace_size(T, N, K)
         workspace = scratch(workspace, need, dev)
         call("hf_fp8_gemm", xq.data_ptr(), sx.data_ptr(), wq.data_ptr(), sw.data_ptr(), T, N, K,
-             out.data_ptr(), _dtype_code(out), _ptr(workspace), need, s)
+             out.data_ptr(), _code(out.dtype), None if workspace is None else workspace.data_ptr(), need, s)
     return out
 
 
+@functools.lru_cache(maxsize=256)
 def moe_experts_workspace_size(T: int, top_k: int, num_experts: int, hidden: int, inter: int,
                                out_dtype: str = "bf16") -> int:
     return int(_lib.lib().hf_fp8_moe_experts_workspace_size(T, top_k, num_experts, hidden, inter,
@@ -105,37 +106,38 @@ def moe_experts(x, experts, scales, routing: dict, resid=None, out=None, out_dty
     scales: fp32 [E x 3*ceil(I/128)*ceil(H/128)] in the same order; routing: the
     dict of route_logits or MoELayer.route (topk_weights, offsets and perm are
     read); resid: [T x H] of out's type, may be `out`."""
-    torch = _torch()
     T, H = x.shape
     dev = x.device
     E = experts.shape[0]
     w = routing["topk_weights"]
     k = w.shape[1]
     I = experts.shape[1] // (3 * H)
-    check_tensor("x", x, _act_types(), (T, H), rows=True)
-    check_tensor("experts", experts, _q_types(), (E, 3 * I * H), dev)
-    check_tensor("scales", scales, (torch.float32,), (E, 3 * blocks(I) * blocks(H)), dev)
-    check_tensor("topk_weights", w, (torch.float32,), (T, k), dev)
+    check_tensor("x", x, _X, (T, H), rows=True)
+    check_tensor("experts", experts, _Q, (E, 3 * I * H), dev)
+    check_tensor("scales", scales, _F32, (E, 3 * blocks(I) * blocks(H)), dev)
+    check_tensor("topk_weights", w, _F32, (T, k), dev)
     offsets, perm = routing["offsets"], routing["perm"]
-    for name, t, least in (("offsets", offsets, E + 1), ("perm", perm, T * k)):
-        check_tensor(name, t, (torch.int32,), t.shape, dev)
-        if t.numel() < least:
-            raise ValueError(f"{name}: {t.numel()} entries, {least} are needed")
+    check_tensor("offsets", offsets, _I32, offsets.shape, dev)
+    check_tensor("perm", perm, _I32, perm.shape, dev)
+    if offsets.numel() < E + 1 or perm.numel() < T * k:
+        raise ValueError(f"offsets, perm: {offsets.numel()} and {perm.numel()} entries, {E + 1} "
+                         f"and {T * k} are needed")
     if out is None:
         out = torch.empty((T, H), dtype=torch.float32 if out_dtype == "f32" else torch.bfloat16,
                           device=dev)
     else:
-        check_tensor("out", out, _act_types(), (T, H), dev)
+        check_tensor("out", out, _X, (T, H), dev)
     if resid is not None:
         check_tensor("resid", resid, (out.dtype,), (T, H), dev)
     r = HfMoeRouting(None, w.data_ptr(), None, None, offsets.data_ptr(), perm.data_ptr(), None)
-    code = _dtype_code(out)
+    code = _code(out.dtype)
     with on_device(dev, stream) as s:
-        need = int(_lib.lib().hf_fp8_moe_experts_workspace_size(T, k, E, H, I, code))
+        need = moe_experts_workspace_size(T, k, E, H, I, "f32" if code == HF_F32 else "bf16")
         workspace = scratch(workspace, need, dev)
         call("hf_fp8_moe_experts", experts.data_ptr(), scales.data_ptr(), E, H, I, x.data_ptr(),
-             _dtype_code(x), _pitch(x), T, k, r, _ptr(resid), out.data_ptr(), code,
-             _ptr(workspace), need, s)
+             _code(x.dtype), _pitch(x), T, k, r,
+             None if resid is None else resid.data_ptr(), out.data_ptr(), code,
+             None if workspace is None else workspace.data_ptr(), need, s)
     return out
 
 

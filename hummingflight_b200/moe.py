@@ -77,19 +77,38 @@ def _host_u16(a):
 def check_tensor(name, t, dtypes, shape, device=None, rows=False):
     """Raises ValueError unless `t` is a contiguous tensor of one of the dtypes
     and the shape (rows: its rows may lie apart), on `device`."""
+    if (t.dtype in dtypes and t.shape == shape
+            and (device is None or t.get_device() == device.index)
+            and (t.is_contiguous() or (rows and t.dim() == 2 and t.stride(1) == 1))):
+        return
     if t.dtype not in dtypes:
         raise ValueError(f"{name}: dtype {t.dtype} is not one of {', '.join(map(str, dtypes))}")
     if t.shape != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)} is not {tuple(shape)}")
     if device is not None and t.device != device:
         raise ValueError(f"{name}: on {t.device}, not on {device}")
-    if not t.is_contiguous() and not (rows and t.dim() == 2 and t.stride(1) == 1):
-        raise ValueError(f"{name}: must be contiguous")
+    raise ValueError(f"{name}: must be contiguous")
+
+
+def _get_device() -> int:
+    return _torch().cuda.current_device()
+
+
+def _set_device(index: int) -> None:
+    _torch().cuda.set_device(index)
+
+
+def _raw_stream(index: int) -> int:
+    """Handle of the device's current stream (without the Stream object around
+    it, which costs more than a small kernel's launch)."""
+    return _torch()._C._cuda_getCurrentRawStream(index)
 
 
 class on_device:
     """The context a call on `device` runs in: makes the device current when it
     is not, and gives the stream (the device's current one unless given)."""
+
+    __slots__ = ("_index", "_stream", "_back")
 
     def __init__(self, device, stream=None):
         if device.type != "cuda":
@@ -97,15 +116,15 @@ class on_device:
         self._index, self._stream, self._back = device.index, stream, None
 
     def __enter__(self):
-        torch = _torch()
-        if self._index is not None and torch.cuda.current_device() != self._index:
-            self._back = torch.cuda.current_device()
-            torch.cuda.set_device(self._index)
-        return (self._stream or torch.cuda.current_stream()).cuda_stream
+        current = _get_device()
+        if current != self._index:
+            _set_device(self._index)
+            self._back = current
+        return _raw_stream(self._index) if self._stream is None else self._stream.cuda_stream
 
     def __exit__(self, *exc):
         if self._back is not None:
-            _torch().cuda.set_device(self._back)
+            _set_device(self._back)
 
 
 def scratch(workspace, need: int, device):
@@ -382,6 +401,7 @@ def _route_spec(E, top_k, score, n_group, topk_group, group_top, scale, norm):
     return HfRouteSpec(E, top_k, _SCORES[score], n_group, topk_group, group_top, scale, int(norm))
 
 
+@functools.lru_cache(maxsize=256)
 def route_workspace_size(T: int, num_experts: int, top_k: int) -> int:
     """Bytes of scratch of route_logits over T tokens (0 up to 16 tokens)."""
     spec = _route_spec(num_experts, top_k, "sigmoid", 1, 1, 1, 1.0, True)
@@ -402,33 +422,35 @@ def route_logits(logits, bias=None, top_k: int = 8, score: str = "sigmoid", n_gr
     hummingflight_b200.fp8.moe_experts takes. `out`: such a dict to write into."""
     torch = _torch()
     T, E = logits.shape
+    f32, i32 = (torch.float32,), (torch.int32,)
     check_tensor("logits", logits, (torch.float32, torch.bfloat16), (T, E))
     dev = logits.device
     if bias is not None:
-        check_tensor("bias", bias, (torch.float32,), (E,), dev)
+        check_tensor("bias", bias, f32, (E,), dev)
     spec = _route_spec(E, top_k, score, n_group, topk_group, group_top, routed_scaling_factor,
                        bool(norm_topk_prob))
-    i32 = torch.int32
     if out is None:
-        out = dict(topk_ids=torch.empty((T, top_k), dtype=i32, device=dev),
+        out = dict(topk_ids=torch.empty((T, top_k), dtype=torch.int32, device=dev),
                    topk_weights=torch.empty((T, top_k), dtype=torch.float32, device=dev),
-                   counts=torch.empty(E + 1, dtype=i32, device=dev),
-                   offsets=torch.empty(E + 2, dtype=i32, device=dev),
-                   perm=torch.empty(T * top_k, dtype=i32, device=dev))
-    else:
-        check_tensor("topk_ids", out["topk_ids"], (i32,), (T, top_k), dev)
-        check_tensor("topk_weights", out["topk_weights"], (torch.float32,), (T, top_k), dev)
-        check_tensor("counts", out["counts"], (i32,), (E + 1,), dev)
-        check_tensor("offsets", out["offsets"], (i32,), (E + 2,), dev)
-        check_tensor("perm", out["perm"], (i32,), (T * top_k,), dev)
-    r = HfMoeRouting(out["topk_ids"].data_ptr(), out["topk_weights"].data_ptr(), None,
-                     out["counts"].data_ptr(), out["offsets"].data_ptr(), out["perm"].data_ptr(),
-                     None)
+                   counts=torch.empty(E + 1, dtype=torch.int32, device=dev),
+                   offsets=torch.empty(E + 2, dtype=torch.int32, device=dev),
+                   perm=torch.empty(T * top_k, dtype=torch.int32, device=dev))
+    ids, w, counts, offsets, perm = (out["topk_ids"], out["topk_weights"], out["counts"],
+                                     out["offsets"], out["perm"])
+    check_tensor("topk_ids", ids, i32, (T, top_k), dev)
+    check_tensor("topk_weights", w, f32, (T, top_k), dev)
+    check_tensor("counts", counts, i32, (E + 1,), dev)
+    check_tensor("offsets", offsets, i32, (E + 2,), dev)
+    check_tensor("perm", perm, i32, (T * top_k,), dev)
+    r = HfMoeRouting(ids.data_ptr(), w.data_ptr(), None, counts.data_ptr(), offsets.data_ptr(),
+                     perm.data_ptr(), None)
     with on_device(dev, stream) as s:
-        need = int(_lib.lib().hf_route_workspace_size(T, spec))
-        workspace = scratch(workspace, need, dev)
-        call("hf_route_logits", logits.data_ptr(), _dtype_code(logits), _ptr(bias), T, spec, r,
-             _ptr(workspace), need, s)
+        need = route_workspace_size(T, E, top_k)
+        workspace = scratch(workspace, need, dev) if need else None
+        call("hf_route_logits", logits.data_ptr(),
+             HF_F32 if logits.dtype == torch.float32 else HF_BF16,
+             None if bias is None else bias.data_ptr(), T, spec, r,
+             None if workspace is None else workspace.data_ptr(), need, s)
     return out
 
 

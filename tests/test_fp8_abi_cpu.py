@@ -169,9 +169,9 @@ def test_calls_run_on_the_device_of_their_tensors(monkeypatch):
         def __init__(self, n):
             self.cuda_stream = n
 
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: cur[0])
-    monkeypatch.setattr(torch.cuda, "set_device", lambda d: (log.append(d), cur.__setitem__(0, d)))
-    monkeypatch.setattr(torch.cuda, "current_stream", lambda: Stream(100 + cur[0]))
+    monkeypatch.setattr(moe, "_get_device", lambda: cur[0])
+    monkeypatch.setattr(moe, "_set_device", lambda d: (log.append(d), cur.__setitem__(0, d)))
+    monkeypatch.setattr(moe, "_raw_stream", lambda i: 100 + i)
     with moe.on_device(torch.device("cuda", 1)) as s:
         assert s == 101 and cur[0] == 1
     assert cur[0] == 0 and log == [1, 0]
