@@ -187,7 +187,9 @@ hf_status hf_fp8_quantize(const void* x, hf_dtype x_dtype, long long ldx, int T,
 }
 
 size_t hf_fp8_gemm_workspace_size(int T, int N, int K) {
-    return T <= 0 || N <= 0 || K <= 0 ? 0 : kAlign;
+    if (T <= 0 || N <= 0 || K <= 0) return 0;
+    const Fp8Split sp = fp8_split(T, N, K);
+    return kAlign + (sp.n > 1 ? up(size_t(sp.n) * T * N * sizeof(float)) : 0);
 }
 
 hf_status hf_fp8_gemm(const uint8_t* xq, const float* sx, const uint8_t* wq, const float* sw, int T,
@@ -219,7 +221,8 @@ hf_status hf_fp8_gemm(const uint8_t* xq, const float* sx, const uint8_t* wq, con
     a.out_f32 = out_dtype == HF_F32;
     a.err = static_cast<int*>(workspace);
     a.clear_err = 1;
-    return launch_fp8_product(a, false, as_cuda(stream));
+    return launch_fp8_gemm(a, reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kAlign),
+                           as_cuda(stream));
 }
 
 size_t hf_fp8_moe_experts_workspace_size(int T, int top_k, int E, int H, int I,
@@ -299,6 +302,8 @@ hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E,
     a.rows = n;
     a.N = I;
     a.K = H;
+    a.nsplit = 1;
+    a.kbper = hb;
     a.mid_q = ws + L.mq;
     a.mid_s = reinterpret_cast<float*>(ws + L.ms);
     a.err = qa.err;
@@ -311,6 +316,7 @@ hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E,
     a.sw = scales + 2ll * ib * hb;
     a.N = H;
     a.K = I;
+    a.kbper = ib;
     a.out = ws + L.y;
     a.out_f32 = f32;
     HF_TRY(launch_fp8_product(a, false, st));

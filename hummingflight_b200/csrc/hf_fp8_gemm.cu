@@ -38,6 +38,7 @@ using namespace sm100;
 
 constexpr int kThreads = 384;
 constexpr int kAccWarps = 8;
+constexpr int kNarrowRows = 64;  // positions per segment up to which the weights are the MMA's M
 constexpr int kScaleSlots = 4;
 constexpr uint32_t kABytes = 128 * 128;  // 128 weight rows x 128 bytes
 constexpr uint64_t kWaitNs = 2000ull * 1000 * 1000;
@@ -65,6 +66,8 @@ struct Cfg {
 struct Tile {
     int row0, n;      // first position, positions
     int m0;           // first weight row of block 0 in its matrix
+    int kb0, kb1;     // blocks of K
+    long long out0;   // first output row (behind the planes of earlier runs of K)
     int a0, a1;       // TMA rows of the two blocks
     const float* s0;  // weight scales of the two blocks, [kb]
     const float* s1;
@@ -115,11 +118,22 @@ __device__ __forceinline__ void load_plan(const Fp8Args& a, int MB, int* off, in
 template <bool GLU, int BN>
 __device__ __forceinline__ void decode(const Fp8Args& a, const int* off, const int* pref, int KB,
                                        int u, Tile& t) {
+    t.kb0 = 0;
+    t.kb1 = KB;
+    t.out0 = 0;
+    if (!GLU && a.nsplit > 1) {  // runs of K of one tile are adjacent
+        const int ks = u % a.nsplit;
+        u /= a.nsplit;
+        t.kb0 = ks * a.kbper;
+        t.kb1 = min(KB, t.kb0 + a.kbper);
+        t.out0 = (long long)ks * a.rows;
+    }
     const int g = find_segment(pref, a.G, u);
     const int c = off[g + 1] - off[g];
     const int nt = (c + BN - 1) / BN, nw = (c + nt - 1) / nt;  // equal widths
     const int local = u - pref[g], mi = local / nt, ni = local % nt;
     t.row0 = off[g] + ni * nw;
+    t.out0 += t.row0;
     t.n = min(nw, c - ni * nw);
     t.m0 = mi * (GLU ? 128 : 256);
     t.a0 = g * a.a_stride + a.a_base + t.m0;
@@ -213,7 +227,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    const int total = pref[a.G];
+    const int total = pref[a.G] * (GLU ? 1 : a.nsplit);
+    griddep_launch_dependents();
     const auto wait = [&](uint64_t* bar, uint32_t parity) {
         return mbar_wait_for(smem_u32(bar), parity, abort_flag, kWaitNs);
     };
@@ -229,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 Tile t;
                 decode<GLU, BN>(a, off, pref, KB, u, t);
                 const int nb = (t.n + C::kBoxB - 1) / C::kBoxB;
-                for (int kb = 0; kb < KB; ++kb, ++it) {
+                for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
                     const uint32_t s = it % S;
                     if (!wait(&done[s], ((it / S) & 1) ^ 1)) {
                         ok = false;
@@ -259,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 Tile t;
                 decode<GLU, BN>(a, off, pref, KB, u, t);
                 const uint32_t idesc = idesc_e4m3_m128(uint32_t(t.n + 15) & ~15u);
-                for (int kb = 0; kb < KB; ++kb, ++it) {
+                for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
                     const uint32_t s = it % S, b = it % NB;
                     if (!wait(&tempty[b], ((it / NB) & 1) ^ 1) || !wait(&full[s], (it / S) & 1)) {
                         ok = false;
@@ -291,17 +306,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
                 Tile t;
                 decode<GLU, BN>(a, off, pref, KB, u, t);
-                float x[PL], w0 = t.s0[0], w1 = t.s1[0];
+                float x[PL], w0 = t.s0[t.kb0], w1 = t.s1[t.kb0];
                 const float* xp[PL];
 #pragma unroll
                 for (int j = 0; j < PL; ++j) {
                     const int c = j * 32 + lane;
                     xp[j] = c < t.n ? a.sx + size_t(t.row0 + c) * KB : nullptr;
-                    x[j] = xp[j] ? xp[j][0] : 0.0f;
+                    x[j] = xp[j] ? xp[j][t.kb0] : 0.0f;
                 }
-                for (int kb = 0; kb < KB; ++kb, ++it) {
+                for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
                     float xn[PL], v0 = 0.0f, v1 = 0.0f;  // the next block's, in flight
-                    const bool more = kb + 1 < KB;
+                    const bool more = kb + 1 < t.kb1;
 #pragma unroll
                     for (int j = 0; j < PL; ++j) xn[j] = more && xp[j] ? xp[j][kb + 1] : 0.0f;
                     if (more) {
@@ -347,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < CH; ++i)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) g[i][j] = v[i][j] = 0ull;
-            for (int kb = 0; kb < KB; ++kb, ++it) {
+            for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
                 const uint32_t b = it % NB, sl = it % kScaleSlots;
                 if (!wait(&done[it % S], (it / S) & 1) ||
                     !wait(&sfull[sl], (it / kScaleSlots) & 1)) {
@@ -456,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             if (i < nc && c < t.n) {
                                 const float y0 = e ? hi_f(g[i][j]) : lo_f(g[i][j]);
                                 const float y1 = e ? hi_f(v[i][j]) : lo_f(v[i][j]);
-                                const size_t o = size_t(t.row0 + c) * a.N + t.m0 + r;
+                                const size_t o = size_t(t.out0 + c) * a.N + t.m0 + r;
                                 const bool r0 = t.m0 + r < a.N, r1 = t.m0 + 128 + r < a.N;
                                 if (a.out_f32) {
                                     float* y = static_cast<float*>(a.out) + o;
@@ -646,7 +661,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     cluster_sync();  // the peer's barriers exist before any remote arrive
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    const int total = pref[a.G];
+    const int total = pref[a.G] * (GLU ? 1 : a.nsplit);
+    griddep_launch_dependents();
     // No barrier that the peer arrives on hands over data in ordinary memory (TMA
     // and the MMAs write and read shared memory, tcgen05 fences order the tensor
     // memory), so every wait orders this CTA's accesses only.
@@ -671,7 +687,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 const int nb = rank ? nb1 : nb0, row = t.row0 + rank * 128;
                 const int wrow = rank ? t.a1 : t.a0;
                 const uint32_t bytes = 2 * kABytes + (nb0 + nb1) * kPairBox * 128;
-                for (int kb = 0; kb < KB; ++kb, ++issued) {
+                for (int kb = t.kb0; kb < t.kb1; ++kb, ++issued) {
                     if (!wait(done_at + s * 8, ph) || !wait(done_at + (S + s) * 8, ph)) {
                         ok = false;
                         break;
@@ -707,7 +723,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 uint32_t s = 0, ph = 0, b = 0, bph = 1;
                 bool ok = true;
                 for (int u = first; u < total && ok; u += step) {
-                    for (int kb = 0; kb < KB; ++kb) {
+                    const int k0 = GLU ? 0 : u % a.nsplit * a.kbper;
+                    const int nk = GLU ? KB : min(KB - k0, a.kbper);
+                    for (int kb = 0; kb < nk; ++kb) {
                         if (!wait(full_at + s * 8, ph) || !wait(te_at + b * 8, bph)) {
                             ok = false;
                             break;
@@ -736,14 +754,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             }
         } else if (warp == 2) {
             // ------------------------------------------------------ scales
-            const bool vec = KB % 4 == 0 && (reinterpret_cast<uintptr_t>(a.sx) & 15) == 0;
+            const bool vec = KB % 4 == 0 && (GLU || a.kbper % 4 == 0) && (reinterpret_cast<uintptr_t>(a.sx) & 15) == 0;
             uint32_t is = 0;
             bool ok = true;
             for (int u = first; u < total && ok; u += step) {
                 Tile t;
                 decode<GLU, 256>(a, off, pref, KB, u, t);
                 const int n = min(128, t.n - rank * 128);
-                for (int k0 = 0; k0 < KB; k0 += kPairGroup, ++is) {
+                for (int k0 = t.kb0; k0 < t.kb1; k0 += kPairGroup, ++is) {
                     const uint32_t q = is % kPairSlots;
                     float* o = sc + q * (kPairScale / 4) + lane;
 #pragma unroll 1
@@ -825,13 +843,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     ph ^= 1;
                 }
             };
-            for (int k0 = 0; k0 < KB && ok; k0 += kPairGroup) {
+            for (int k0 = t.kb0; k0 < t.kb1 && ok; k0 += kPairGroup) {
                 if (!wait(sf_at + sl * 8, sph)) {
                     ok = false;
                     break;
                 }
                 const float* ps = sc + sl * (kPairScale / 4) + r;
-                const int ng = min(kPairGroup, KB - k0);
+                const int ng = min(kPairGroup, t.kb1 - k0);
                 if (work) {
 #pragma unroll 1
                     for (int e = 0; e < ng; ++e, ps += 256) {
@@ -905,7 +923,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     }
                 }
             } else if (work) {
-                const long long p = t.row0 + rank * 128 + q * 32;
+                const long long p = t.out0 + rank * 128 + q * 32;
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
                     store32(a, p, n - q * 32, t.m0 + (c >> 1) * 128 + h * 64 + (c & 1) * 32,
@@ -979,9 +997,99 @@ hf_status launch_one(const Fp8Args& a, cudaStream_t st) {
 
 }  // namespace
 
+// The runs of K of one product: with fewer tiles than the GPU has places for
+// (148 CTAs, or 74 pairs), each tile's blocks of K are dealt to several CTAs that
+// write fp32 planes, which a second launch adds in order. The number that
+// minimises rounds x (blocks + 2 to fill the pipeline) + the sum pass; a block
+// takes about 0.75 us where the weights stream from memory (0.6 us on a pair).
+Fp8Split fp8_split(int T, int N, int K) {
+    const int KB = (K + kFp8Block - 1) / kFp8Block;
+    const bool pair = T > kNarrowRows;
+    const long long tiles = (long long)((N + 255) / 256) * (pair ? (T + 255) / 256 : 1);
+    const int slots = pair ? 74 : 148, mult = pair ? 4 : 1;
+    Fp8Split best{1, KB};
+    double least = 1e30;
+    for (int n = 1; n <= 16 && n <= KB; ++n) {
+        const int per = ((KB + n - 1) / n + mult - 1) / mult * mult;
+        if ((KB + per - 1) / per != n) continue;  // no empty run
+        const double rounds = double((tiles * n + slots - 1) / slots);
+        const double sum = n == 1 ? 0.0 : (2.0 + n * 8e-6 * T * N / 5.0) / 0.7;
+        const double cost = rounds * (per + 2) + sum;
+        if (cost < least) {
+            least = cost;
+            best = Fp8Split{n, per};
+        }
+    }
+    return best;
+}
+
+__global__ void __launch_bounds__(256) k_sum_planes(const float* planes, int n, long long count,
+                                                    void* out, int out_f32) {
+    griddep_wait();
+    const long long quads = count / 4, rest = count - quads * 4;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i < quads) {
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int s = 0; s < n; ++s) {
+            const float* p = planes + s * count + i * 4;
+            float4 v;
+            if (count % 4 == 0) {
+                v = *reinterpret_cast<const float4*>(p);
+            } else {
+                v = make_float4(p[0], p[1], p[2], p[3]);
+            }
+            y.x += v.x; y.y += v.y; y.z += v.z; y.w += v.w;
+        }
+        const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+        const float r[4] = {y.x, y.y, y.z, y.w};
+        if (out_f32) {
+            float* o = static_cast<float*>(out) + i * 4;
+            if (vec) *reinterpret_cast<float4*>(o) = y;
+            else
+                for (int e = 0; e < 4; ++e) o[e] = r[e];
+        } else {
+            __nv_bfloat16* o = static_cast<__nv_bfloat16*>(out) + i * 4;
+            if (vec) {
+                const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y);
+                const __nv_bfloat162 b = __floats2bfloat162_rn(y.z, y.w);
+                *reinterpret_cast<uint2*>(o) = make_uint2(*reinterpret_cast<const uint32_t*>(&a),
+                                                          *reinterpret_cast<const uint32_t*>(&b));
+            } else {
+                for (int e = 0; e < 4; ++e) o[e] = __float2bfloat16_rn(r[e]);
+            }
+        }
+    } else if (i < quads + rest) {
+        const long long c = quads * 4 + (i - quads);
+        float y = 0.0f;
+        for (int s = 0; s < n; ++s) y += planes[s * count + c];
+        if (out_f32) static_cast<float*>(out)[c] = y;
+        else static_cast<__nv_bfloat16*>(out)[c] = __float2bfloat16_rn(y);
+    }
+}
+
+hf_status launch_fp8_gemm(const Fp8Args& args, float* planes, cudaStream_t st) {
+    Fp8Args a = args;
+    const Fp8Split sp = fp8_split(a.rows, a.N, a.K);
+    a.nsplit = sp.n;
+    a.kbper = sp.per;
+    if (sp.n > 1) {
+        a.out = planes;
+        a.out_f32 = 1;
+    }
+    HF_TRY(launch_fp8_product(a, false, st));
+    if (sp.n > 1) {
+        const long long count = (long long)a.rows * a.N, n = count / 4 + count % 4;
+        HF_CUDA(launch_pdl(k_sum_planes, dim3(unsigned((n + 255) / 256)), dim3(256), 0, st,
+                           static_cast<const float*>(planes), sp.n, count, args.out,
+                           args.out_f32));
+    }
+    return HF_OK;
+}
+
 hf_status launch_fp8_product(const Fp8Args& a, bool glu, cudaStream_t st) {
     const int avg = (a.rows + a.G - 1) / a.G;
-    if (avg > 64) return glu ? launch_pair<true>(a, st) : launch_pair<false>(a, st);
+    if (avg > kNarrowRows) return glu ? launch_pair<true>(a, st) : launch_pair<false>(a, st);
     if (avg > 32) return glu ? launch_one<true, 64>(a, st) : launch_one<false, 64>(a, st);
     if (avg > 16) return glu ? launch_one<true, 32>(a, st) : launch_one<false, 32>(a, st);
     return glu ? launch_one<true, 16>(a, st) : launch_one<false, 16>(a, st);

@@ -85,8 +85,8 @@ def check_tensor(name, t, dtypes, shape, device=None, rows=False):
         raise ValueError(f"{name}: dtype {t.dtype} is not one of {', '.join(map(str, dtypes))}")
     if t.shape != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)} is not {tuple(shape)}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name}: on {t.device}, not on {device}")
+    if device is not None and (t.device != device or device.type != "cuda"):
+        raise ValueError(f"{name}: on {t.device}, not on the CUDA device of the other tensors")
     raise ValueError(f"{name}: must be contiguous")
 
 
