@@ -17,60 +17,204 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 int blocks128(int n) { return (n + kFp8Block - 1) / kFp8Block; }
 
 // ------------------------------------------------------------------ quantise
-// 16 threads own one block of 128 columns, 8 columns each.
+// One pass bound by memory: 16 threads own a block of 128 columns, 8 columns
+// (16 or 32 bytes) each, so the maximum is four shuffles and every load and store
+// is whole sectors; a thread has kQuantBatch blocks' loads in flight.
+// 16384 x 6144 bf16: @QT16384@.
 struct QuantArgs {
     const void* x;
     long long ldx;
     int rows, K, nb;
     uint8_t* q;
     float* s;
-    // gather (experts): the row of slot perm[p]'s token goes to position p;
-    // null: row t of x to row t of q
+    // experts: the row of slot perm[p]'s token goes to position p, pos[slot] = p
     const int32_t* perm;
     int k, n_tok;
-    int32_t* pos;  // [slots] position of each slot
-    int* err;      // error word, cleared by the first block
+    int32_t* pos;
+    int* err;  // error word, cleared by the first block
+};
+constexpr int kQuantBatch = 4;
+
+// 8 columns as they lie in memory.
+template <bool XF32>
+struct Raw8 {
+    uint4 v[XF32 ? 2 : 1];
+    __device__ __forceinline__ void load(const void* x, long long i) {
+        if constexpr (XF32) {
+            const float* p = static_cast<const float*>(x) + i;
+            v[0] = ld_stream_u4(p);
+            v[1] = ld_stream_u4(p + 4);
+        } else {
+            v[0] = ld_stream_u4(static_cast<const uint16_t*>(x) + i);
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < (XF32 ? 2 : 1); ++i) v[i] = make_uint4(0, 0, 0, 0);
+    }
 };
 
+// A thread's 8 columns of a block: values and scale. The 16 threads of `half`
+// call it together. Magnitudes order as their bits (NaN above Inf), bf16 ones two
+// to a register.
+template <bool XF32>
+__device__ __forceinline__ uint2 quantize8(const Raw8<XF32>& r, unsigned half, float* scale) {
+    uint32_t m;
+    float f[8];
+    if constexpr (XF32) {
+        const uint4 a = r.v[0], b = r.v[1];
+        const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            f[j] = __uint_as_float(u[j]);
+            m = max(m, u[j] & 0x7fffffffu);
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(half, m, o));
+    } else {
+        const uint4 a = r.v[0];
+        unpack8(a, f);
+        m = __vmaxu2(__vmaxu2(a.x & 0x7fff7fffu, a.y & 0x7fff7fffu),
+                     __vmaxu2(a.z & 0x7fff7fffu, a.w & 0x7fff7fffu));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(half, m, o));
+        m = max(m & 0xffff0000u, m << 16);
+    }
+    float inv;
+    *scale = block_scale(__uint_as_float(m), inv);
+    return make_uint2(pack4_e4m3(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
+                      pack4_e4m3(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+}
+
+// Rows one behind the other and whole blocks: the blocks are one array.
+template <bool XF32>
+__global__ void __launch_bounds__(256) k_quantize_flat(const void* x, long long blocks, uint8_t* q,
+                                                       float* s) {
+    const int sub = threadIdx.x & 15;
+    const unsigned half = 0xffffu << (threadIdx.x & 16);
+    const long long step = (long long)gridDim.x * 16;
+    for (long long i0 = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); i0 < blocks;
+         i0 += step * kQuantBatch) {
+        Raw8<XF32> r[kQuantBatch];
+#pragma unroll
+        for (int u = 0; u < kQuantBatch; ++u)
+            if (i0 + u * step < blocks) r[u].load(x, (i0 + u * step) * kFp8Block + sub * 8);
+#pragma unroll
+        for (int u = 0; u < kQuantBatch; ++u) {
+            const long long i = i0 + u * step;
+            if (i >= blocks) break;  // the 16 threads of a block agree
+            float sc;
+            reinterpret_cast<uint2*>(q)[i * 16 + sub] = quantize8(r[u], half, &sc);
+            if (sub == 0) s[i] = sc;
+        }
+    }
+}
+
+// Any pitch, ragged last blocks, gathered rows.
 template <bool XF32>
 __global__ void __launch_bounds__(256) k_quantize(QuantArgs a) {
+    griddep_launch_dependents();
     if (a.err && blockIdx.x == 0 && threadIdx.x == 0) *a.err = 0;
     const int sub = threadIdx.x & 15;
     const unsigned half = 0xffffu << (threadIdx.x & 16);
-    const long long blocks = (long long)a.rows * a.nb;
-    for (long long i = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); i < blocks;
-         i += (long long)gridDim.x * 16) {
-        const int p = int(i / a.nb), b = int(i % a.nb);
+    const long long blocks = (long long)a.rows * a.nb, step = (long long)gridDim.x * 16;
+    for (long long i = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); i < blocks; i += step) {
+        int p, b;
+        if (blocks < 0x7fffffffll) {  // 32-bit division
+            p = int(unsigned(i) / unsigned(a.nb));
+            b = int(unsigned(i) - unsigned(p) * unsigned(a.nb));
+        } else {
+            p = int(i / a.nb);
+            b = int(i - (long long)p * a.nb);
+        }
+        const int c = b * kFp8Block + sub * 8;
         int row = p;
         if (a.perm) {
             const int slot = a.perm[p];
-            if (slot < 0 || slot / a.k >= a.n_tok) continue;
             row = slot / a.k;
-            if (b == 0 && sub == 0) a.pos[slot] = p;
+            if (slot < 0 || row >= a.n_tok) continue;  // the 16 threads agree
+            if (c == 0) a.pos[slot] = p;
         }
-        const int c = b * kFp8Block + sub * 8;
-        float v[8] = {};
-        if (c < a.K) load8<XF32>(a.x, row * a.ldx + c, v);
-        uint32_t m = 0;  // magnitudes order as their bits; NaN is above Inf
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(half, m, o));
-        float inv;
-        const float s = block_scale(__uint_as_float(m), inv);
-        if (c < a.K)
-            *reinterpret_cast<uint2*>(a.q + size_t(p) * a.K + c) =
-                make_uint2(pack4_e4m3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
-                           pack4_e4m3(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
+        Raw8<XF32> r;
+        if (c < a.K) r.load(a.x, row * a.ldx + c);
+        else r.zero();
+        float s;
+        const uint2 q = quantize8(r, half, &s);
+        if (c < a.K) *reinterpret_cast<uint2*>(a.q + size_t(p) * a.K + c) = q;
         if (sub == 0) a.s[size_t(p) * a.nb + b] = s;
     }
 }
 
+// pos[perm[p]] = p. What perm does not name keeps what the workspace holds; its
+// readers check the range.
+__global__ void __launch_bounds__(256) k_positions(const int32_t* perm, int n, int32_t* pos,
+                                                   int* err) {
+    const int p = blockIdx.x * 256 + threadIdx.x;
+    if (p == 0) *err = 0;
+    if (p >= n) return;
+    const int slot = perm[p];
+    if (slot >= 0 && slot < n) pos[slot] = p;
+}
+
+// Token-major gather of large batches: a block of a token's row is read and
+// quantised once and written to the positions of its k slots (k times fewer reads
+// than position by position).
+template <bool XF32>
+__global__ void __launch_bounds__(256) k_quantize_tokens(QuantArgs a) {
+    const int sub = threadIdx.x & 15;
+    const unsigned half = 0xffffu << (threadIdx.x & 16);
+    const int t = blockIdx.x, n = a.n_tok * a.k;
+    __shared__ int32_t at[kMaxK];
+    if (int(threadIdx.x) < a.k) at[threadIdx.x] = a.pos[t * a.k + threadIdx.x];
+    __syncthreads();
+    for (int b0 = threadIdx.x >> 4; b0 < a.nb; b0 += 16 * kQuantBatch) {
+        Raw8<XF32> r[kQuantBatch];
+#pragma unroll
+        for (int u = 0; u < kQuantBatch; ++u) {
+            const int c = (b0 + u * 16) * kFp8Block + sub * 8;
+            if (c < a.K) r[u].load(a.x, t * a.ldx + c);
+            else r[u].zero();
+        }
+#pragma unroll
+        for (int u = 0; u < kQuantBatch; ++u) {
+            const int b = b0 + u * 16, c = b * kFp8Block + sub * 8;
+            if (b >= a.nb) continue;
+            float s;
+            const uint2 q = quantize8(r[u], half, &s);
+            for (int i = 0; i < a.k; ++i) {
+                const int p = at[i];
+                if (unsigned(p) >= unsigned(n)) continue;
+                if (c < a.K) *reinterpret_cast<uint2*>(a.q + size_t(p) * a.K + c) = q;
+                if (sub == 0) a.s[size_t(p) * a.nb + b] = s;
+            }
+        }
+    }
+}
+
+// Positions from which the experts' gather goes by tokens: @GATHER@.
+constexpr int kTokenMajor = 4096;
+
 hf_status launch_quantize(const QuantArgs& a, bool f32, int dev, cudaStream_t st) {
-    const long long groups = ((long long)a.rows * a.nb + 15) / 16;
-    const int grid = int(std::min<long long>(groups, num_sms(dev) * 16));
-    if (f32) k_quantize<true><<<grid, 256, 0, st>>>(a);
-    else k_quantize<false><<<grid, 256, 0, st>>>(a);
+    if (a.perm && a.rows >= kTokenMajor && a.k > 1) {
+        k_positions<<<(a.rows + 255) / 256, 256, 0, st>>>(a.perm, a.rows, a.pos, a.err);
+        HF_CUDA(cudaGetLastError());
+        if (f32) k_quantize_tokens<true><<<a.n_tok, 256, 0, st>>>(a);
+        else k_quantize_tokens<false><<<a.n_tok, 256, 0, st>>>(a);
+        HF_CUDA(cudaGetLastError());
+        return HF_OK;
+    }
+    const long long blocks = (long long)a.rows * a.nb;
+    const long long most = num_sms(dev) * 8ll;
+    if (!a.perm && a.ldx == a.K && a.K % kFp8Block == 0) {
+        const int grid = int(std::min((blocks + 15) / 16, most));
+        if (f32) k_quantize_flat<true><<<grid, 256, 0, st>>>(a.x, blocks, a.q, a.s);
+        else k_quantize_flat<false><<<grid, 256, 0, st>>>(a.x, blocks, a.q, a.s);
+    } else {
+        const int grid = int(std::min((blocks + 15) / 16, 2 * most));
+        if (f32) k_quantize<true><<<grid, 256, 0, st>>>(a);
+        else k_quantize<false><<<grid, 256, 0, st>>>(a);
+    }
     HF_CUDA(cudaGetLastError());
     return HF_OK;
 }
@@ -78,50 +222,67 @@ hf_status launch_quantize(const QuantArgs& a, bool f32, int dev, cudaStream_t st
 // ------------------------------------------------------------------ combine
 // out[t] = resid[t] + sum_i w[t, i] y[pos(t, i)], rank order, fp32: the
 // reference's separate multiply and add per pick.
-template <bool F32>
-__device__ __forceinline__ void load4(const void* p, size_t i, float (&v)[4]) {
-    if constexpr (F32) {
-        const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    } else {
-        const uint2 a = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
-        v[0] = bf16lo(a.x); v[1] = bf16hi(a.x); v[2] = bf16lo(a.y); v[3] = bf16hi(a.y);
-    }
+__device__ __forceinline__ void unpack(const uint4 v, float (&f)[4]) {
+    f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y);
+    f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
 }
+__device__ __forceinline__ void unpack(const uint4 v, float (&f)[8]) { unpack8(v, f); }
 
+// A thread takes 16 bytes of a token's columns, all of its picks' loads in flight
+// before the first is used. T = 16384, k = 8, H = 6144, bf16: @COMBINE@.
 template <bool F32>
 __global__ void __launch_bounds__(256) k_fp8_combine(const void* y, const int32_t* pos,
                                                      const float* w, int T, int k, int H,
                                                      const void* resid, void* out) {
-    const long long n = (long long)T * (H / 4);
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-        const int t = int(i / (H / 4)), c = int(i % (H / 4)) * 4;
-        float acc[4] = {}, v[4];
-        for (int j = 0; j < k; ++j) {
-            const float wj = w[size_t(t) * k + j];
-            const unsigned at = unsigned(pos[size_t(t) * k + j]);
-            if (at >= unsigned(T * k)) continue;  // a slot that perm does not name
-            load4<F32>(y, size_t(at) * H + c, v);
+    constexpr int V = F32 ? 4 : 8, kBatch = 8;
+    const int t = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * V;
+    griddep_wait();
+    if (c >= H) return;
+    float acc[V] = {};
+    for (int j0 = 0; j0 < k; j0 += kBatch) {
+        uint4 v[kBatch];
+        float wj[kBatch];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) acc[q] = __fadd_rn(acc[q], __fmul_rn(wj, v[q]));
+        for (int j = 0; j < kBatch; ++j) {
+            unsigned at = ~0u;
+            if (j0 + j < k) at = unsigned(pos[size_t(t) * k + j0 + j]);
+            // a slot that perm does not name counts as 0
+            const bool in = at < unsigned(T * k);
+            wj[j] = in ? w[size_t(t) * k + j0 + j] : 0.0f;
+            v[j] = in ? ld_nc_u4(static_cast<const char*>(y) +
+                                 (size_t(at) * H + c) * (F32 ? 4 : 2))
+                      : make_uint4(0, 0, 0, 0);
         }
-        const size_t o = size_t(t) * H + c;
-        if (resid) {
-            load4<F32>(resid, o, v);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) acc[q] = __fadd_rn(v[q], acc[q]);
-        }
-        if constexpr (F32) {
-            *reinterpret_cast<float4*>(static_cast<float*>(out) + o) =
-                make_float4(acc[0], acc[1], acc[2], acc[3]);
-        } else {
-            const __nv_bfloat162 a = __floats2bfloat162_rn(acc[0], acc[1]);
-            const __nv_bfloat162 b = __floats2bfloat162_rn(acc[2], acc[3]);
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + o) =
-                make_uint2(*reinterpret_cast<const uint32_t*>(&a),
-                           *reinterpret_cast<const uint32_t*>(&b));
+        for (int j = 0; j < kBatch; ++j) {
+            if (j0 + j >= k) break;
+            float f[V];
+            unpack(v[j], f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] = __fadd_rn(acc[e], __fmul_rn(wj[j], f[e]));
         }
     }
+    const size_t o = (size_t(t) * H + c) * (F32 ? 4 : 2);
+    if (resid) {
+        float f[V];
+        unpack(*reinterpret_cast<const uint4*>(static_cast<const char*>(resid) + o), f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] = __fadd_rn(f[e], acc[e]);
+    }
+    uint4 r;
+    if constexpr (F32) {
+        r = make_uint4(__float_as_uint(acc[0]), __float_as_uint(acc[1]), __float_as_uint(acc[2]),
+                       __float_as_uint(acc[3]));
+    } else {
+        uint32_t b[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(acc[2 * e], acc[2 * e + 1]);
+            b[e] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        r = make_uint4(b[0], b[1], b[2], b[3]);
+    }
+    *reinterpret_cast<uint4*>(static_cast<char*>(out) + o) = r;
 }
 
 // ------------------------------------------------------------------ workspaces
@@ -320,14 +481,13 @@ hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E,
     a.out = ws + L.y;
     a.out_f32 = f32;
     HF_TRY(launch_fp8_product(a, false, st));
-    const int grid = num_sms(dev) * 8;
-    if (f32)
-        k_fp8_combine<true><<<grid, 256, 0, st>>>(ws + L.y, qa.pos, r->topk_weights, T, top_k, H,
-                                                  resid, out);
-    else
-        k_fp8_combine<false><<<grid, 256, 0, st>>>(ws + L.y, qa.pos, r->topk_weights, T, top_k, H,
-                                                   resid, out);
-    HF_CUDA(cudaGetLastError());
+    const int v = f32 ? 4 : 8;
+    const dim3 grid(unsigned(T), unsigned((H / v + 255) / 256));
+    const void* y = ws + L.y;
+    const int32_t* pos = qa.pos;
+    const float* w = r->topk_weights;
+    HF_CUDA(launch_pdl(f32 ? k_fp8_combine<true> : k_fp8_combine<false>, grid, dim3(256), 0, st, y,
+                       pos, w, T, top_k, H, resid, out));
     return HF_OK;
 }
 

@@ -48,19 +48,6 @@ __device__ __forceinline__ float block_scale(float m, float& inv) {
     return __uint_as_float(uint32_t(se) << 23);
 }
 
-// 8 consecutive activations as fp32.
-template <bool XF32>
-__device__ __forceinline__ void load8(const void* x, long long i, float (&v)[8]) {
-    if constexpr (XF32) {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + i);
-        const float4 a = __ldg(p), b = __ldg(p + 1);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-        unpack8(ld_nc_u4(static_cast<const uint16_t*>(x) + i), v);
-    }
-}
-
 // ------------------------------------------------------------------ products
 // Rows of e4m3 activations (positions) against weight rows. One group (offsets
 // null: all rows) or G groups: group g multiplies positions [offsets[g],
