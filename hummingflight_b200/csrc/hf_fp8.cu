@@ -57,34 +57,39 @@ struct Raw8 {
 // A thread's 8 columns of a block: values and scale. The 16 threads of `half`
 // call it together. Magnitudes order as their bits (NaN above Inf), bf16 ones two
 // to a register.
-template <bool XF32>
-__device__ __forceinline__ uint2 quantize8(const Raw8<XF32>& r, unsigned half, float* scale) {
-    uint32_t m;
-    float f[8];
-    if constexpr (XF32) {
-        const uint4 a = r.v[0], b = r.v[1];
-        const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        m = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            f[j] = __uint_as_float(u[j]);
-            m = max(m, u[j] & 0x7fffffffu);
-        }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(half, m, o));
-    } else {
-        const uint4 a = r.v[0];
-        unpack8(a, f);
-        m = __vmaxu2(__vmaxu2(a.x & 0x7fff7fffu, a.y & 0x7fff7fffu),
-                     __vmaxu2(a.z & 0x7fff7fffu, a.w & 0x7fff7fffu));
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(half, m, o));
-        m = max(m & 0xffff0000u, m << 16);
-    }
+__device__ __forceinline__ uint2 scaled8(const float (&f)[8], uint32_t m, float* scale) {
     float inv;
     *scale = block_scale(__uint_as_float(m), inv);
     return make_uint2(pack4_e4m3(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
                       pack4_e4m3(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+}
+__device__ __forceinline__ uint2 quantize8(const float (&f)[8], unsigned half, float* scale) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(f[j]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(half, m, o));
+    return scaled8(f, m, scale);
+}
+template <bool XF32>
+__device__ __forceinline__ uint2 quantize8(const Raw8<XF32>& r, unsigned half, float* scale) {
+    float f[8];
+    if constexpr (XF32) {
+        const uint4 a = r.v[0], b = r.v[1];
+        const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(u[j]);
+        return quantize8(f, half, scale);
+    } else {
+        const uint4 a = r.v[0];
+        unpack8(a, f);
+        uint32_t m = __vmaxu2(__vmaxu2(a.x & 0x7fff7fffu, a.y & 0x7fff7fffu),
+                     __vmaxu2(a.z & 0x7fff7fffu, a.w & 0x7fff7fffu));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(half, m, o));
+        m = max(m & 0xffff0000u, m << 16);
+        return scaled8(f, m, scale);
+    }
 }
 
 // Rows one behind the other and whole blocks: the blocks are one array.
@@ -115,6 +120,7 @@ __global__ void __launch_bounds__(256) k_quantize_flat(const void* x, long long 
 template <bool XF32>
 __global__ void __launch_bounds__(256) k_quantize(QuantArgs a) {
     griddep_launch_dependents();
+    griddep_wait();
     if (a.err && blockIdx.x == 0 && threadIdx.x == 0) *a.err = 0;
     const int sub = threadIdx.x & 15;
     const unsigned half = 0xffffu << (threadIdx.x & 16);
@@ -212,11 +218,46 @@ hf_status launch_quantize(const QuantArgs& a, bool f32, int dev, cudaStream_t st
         else k_quantize_flat<false><<<grid, 256, 0, st>>>(a.x, blocks, a.q, a.s);
     } else {
         const int grid = int(std::min((blocks + 15) / 16, 2 * most));
-        if (f32) k_quantize<true><<<grid, 256, 0, st>>>(a);
-        else k_quantize<false><<<grid, 256, 0, st>>>(a);
+        HF_CUDA(launch_pdl(f32 ? k_quantize<true> : k_quantize<false>, dim3(unsigned(grid)),
+                           dim3(256), 0, st, a));
     }
     HF_CUDA(cudaGetLastError());
     return HF_OK;
+}
+
+// The intermediate of few positions, whose gate/up product ran in several runs of
+// K: silu(g) * u of the summed planes [n x rows x 2 I] (gate columns, then up),
+// quantised. 16 threads a block of 128 columns.
+__global__ void __launch_bounds__(256) k_swiglu_planes(const float* planes, int n, int rows, int I,
+                                                       int nb, uint8_t* q, float* s) {
+    griddep_launch_dependents();
+    const int sub = threadIdx.x & 15;
+    const unsigned half = 0xffffu << (threadIdx.x & 16);
+    const int i = blockIdx.x * 16 + (threadIdx.x >> 4);
+    griddep_wait();
+    if (i >= rows * nb) return;  // the 16 threads of a block agree
+    const int p = i / nb, b = i % nb, c = b * kFp8Block + sub * 8;
+    float f[8] = {};
+    if (c < I) {
+        float g[8] = {}, u[8] = {};
+#pragma unroll 4
+        for (int r = 0; r < n; ++r) {
+            const float4* v = reinterpret_cast<const float4*>(
+                planes + (size_t(r) * rows + p) * 2 * I + c);
+            const float4* w = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(v) + I);
+            const float4 a0 = v[0], a1 = v[1], b0 = w[0], b1 = w[1];
+            g[0] += a0.x; g[1] += a0.y; g[2] += a0.z; g[3] += a0.w;
+            g[4] += a1.x; g[5] += a1.y; g[6] += a1.z; g[7] += a1.w;
+            u[0] += b0.x; u[1] += b0.y; u[2] += b0.z; u[3] += b0.w;
+            u[4] += b1.x; u[5] += b1.y; u[6] += b1.z; u[7] += b1.w;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = swiglu(g[j], u[j]);
+    }
+    float sc;
+    const uint2 v = quantize8(f, half, &sc);
+    if (c < I) *reinterpret_cast<uint2*>(q + size_t(p) * I + c) = v;
+    if (sub == 0) s[size_t(p) * nb + b] = sc;
 }
 
 // ------------------------------------------------------------------ combine
@@ -230,27 +271,29 @@ __device__ __forceinline__ void unpack(const uint4 v, float (&f)[8]) { unpack8(v
 
 // A thread takes 16 bytes of a token's columns, all of its picks' loads in flight
 // before the first is used. T = 16384, k = 8, H = 6144, bf16: @COMBINE@.
-template <bool F32>
-__global__ void __launch_bounds__(256) k_fp8_combine(const void* y, const int32_t* pos,
+// Y32: the expert outputs are fp32, in n planes (runs of K) that are added in order.
+template <bool Y32, bool F32>
+__global__ void __launch_bounds__(256) k_fp8_combine(const void* y, int n, const int32_t* pos,
                                                      const float* w, int T, int k, int H,
                                                      const void* resid, void* out) {
-    constexpr int V = F32 ? 4 : 8, kBatch = 8;
+    constexpr int V = Y32 ? 4 : 8, kBatch = 8;
     const int t = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * V;
     griddep_wait();
     if (c >= H) return;
+    const unsigned rows = unsigned(T) * unsigned(k);
     float acc[V] = {};
     for (int j0 = 0; j0 < k; j0 += kBatch) {
         uint4 v[kBatch];
         float wj[kBatch];
+        unsigned at[kBatch];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            unsigned at = ~0u;
-            if (j0 + j < k) at = unsigned(pos[size_t(t) * k + j0 + j]);
-            // a slot that perm does not name counts as 0
-            const bool in = at < unsigned(T * k);
+            at[j] = j0 + j < k ? unsigned(pos[size_t(t) * k + j0 + j]) : ~0u;
+            // a position out of range (perm does not name the slot) counts as 0
+            const bool in = at[j] < rows;
             wj[j] = in ? w[size_t(t) * k + j0 + j] : 0.0f;
             v[j] = in ? ld_nc_u4(static_cast<const char*>(y) +
-                                 (size_t(at) * H + c) * (F32 ? 4 : 2))
+                                 (size_t(at[j]) * H + c) * (Y32 ? 4 : 2))
                       : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
@@ -258,53 +301,101 @@ __global__ void __launch_bounds__(256) k_fp8_combine(const void* y, const int32_
             if (j0 + j >= k) break;
             float f[V];
             unpack(v[j], f);
+            if constexpr (Y32) {
+                for (int r = 1; r < n && at[j] < rows; ++r) {
+                    float g[V];
+                    unpack(ld_nc_u4(static_cast<const float*>(y) +
+                                    (size_t(r) * rows + at[j]) * H + c), g);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) f[e] += g[e];
+                }
+            }
 #pragma unroll
             for (int e = 0; e < V; ++e) acc[e] = __fadd_rn(acc[e], __fmul_rn(wj[j], f[e]));
         }
     }
-    const size_t o = (size_t(t) * H + c) * (F32 ? 4 : 2);
-    if (resid) {
-        float f[V];
-        unpack(*reinterpret_cast<const uint4*>(static_cast<const char*>(resid) + o), f);
-#pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] = __fadd_rn(f[e], acc[e]);
-    }
-    uint4 r;
+    const size_t o = size_t(t) * H + c;
     if constexpr (F32) {
-        r = make_uint4(__float_as_uint(acc[0]), __float_as_uint(acc[1]), __float_as_uint(acc[2]),
-                       __float_as_uint(acc[3]));
-    } else {
-        uint32_t b[4];
+        static_assert(Y32, "fp32 outputs come from fp32 expert outputs");
+        if (resid) {
+            float f[V];
+            unpack(*reinterpret_cast<const uint4*>(static_cast<const float*>(resid) + o), f);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < V; ++e) acc[e] = __fadd_rn(f[e], acc[e]);
+        }
+        *reinterpret_cast<float4*>(static_cast<float*>(out) + o) =
+            make_float4(acc[0], acc[1], acc[2], acc[3]);
+    } else {
+        uint32_t b[V / 2];
+        if (resid) {
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) {
+                const uint32_t h = reinterpret_cast<const uint32_t*>(
+                    static_cast<const uint16_t*>(resid) + o)[e];
+                acc[2 * e] = __fadd_rn(bf16lo(h), acc[2 * e]);
+                acc[2 * e + 1] = __fadd_rn(bf16hi(h), acc[2 * e + 1]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e) {
             const __nv_bfloat162 h = __floats2bfloat162_rn(acc[2 * e], acc[2 * e + 1]);
             b[e] = *reinterpret_cast<const uint32_t*>(&h);
         }
-        r = make_uint4(b[0], b[1], b[2], b[3]);
+        uint16_t* d = static_cast<uint16_t*>(out) + o;
+        if constexpr (V == 8) *reinterpret_cast<uint4*>(d) = make_uint4(b[0], b[1], b[2], b[3]);
+        else *reinterpret_cast<uint2*>(d) = make_uint2(b[0], b[1]);
     }
-    *reinterpret_cast<uint4*>(static_cast<char*>(out) + o) = r;
+}
+
+hf_status launch_fp8_combine(const void* y, int n, const int32_t* pos, const float* w, int T, int k,
+                             int H, const void* resid, void* out, bool f32, cudaStream_t st) {
+    const bool y32 = f32 || n > 1;
+    const int v = y32 ? 4 : 8;
+    const dim3 grid(unsigned(T), unsigned((H / v + 255) / 256));
+    HF_CUDA(launch_pdl(f32 ? k_fp8_combine<true, true>
+                           : y32 ? k_fp8_combine<true, false> : k_fp8_combine<false, false>,
+                       grid, dim3(256), 0, st, y, n, pos, w, T, k, H, resid, out));
+    return HF_OK;
 }
 
 // ------------------------------------------------------------------ workspaces
+// Runs of K of the experts' products: few positions make few tiles (at most one
+// per position and row block of the weights); beyond this number the tiles fill
+// the GPU.
+constexpr int kFewPositions = 64;
+
 struct ExpertsWs {
-    size_t pos, xq, sx, mq, ms, y, total;
+    Fp8Split up, down;  // runs of the gate/up and down products
+    bool few;           // the gate/up product writes planes, one for each run
+    size_t pos, xq, sx, gu, mq, ms, y, total;
 };
 
-ExpertsWs experts_ws(int T, int k, int H, int I, bool f32) {
+ExpertsWs experts_ws(int T, int k, int E, int H, int I, bool f32) {
     ExpertsWs w{};
     const size_t n = size_t(T) * k;
+    w.up = Fp8Split{1, blocks128(H)};
+    w.down = Fp8Split{1, blocks128(I)};
+    if (n <= kFewPositions) {
+        const long long active = std::min<long long>(n, E);
+        w.down = fp8_split(active * ((H + 255) / 256), false, I, 4.0 * n * H);
+        if (I % kFp8Block == 0) {  // gate and up rows then have one run of scale blocks
+            w.up = fp8_split(active * (I / 128), false, H, 8.0 * n * I);
+            w.few = w.up.n > 1;
+        }
+    }
     size_t o = kAlign;  // the error word
     const auto take = [&](size_t bytes) {
         const size_t at = o;
-        o += up(bytes);
+        o += hf::up(bytes);
         return at;
     };
     w.pos = take(n * 4);
     w.xq = take(n * H);
     w.sx = take(n * blocks128(H) * 4);
+    w.gu = take(w.few ? size_t(w.up.n) * n * 2 * I * 4 : 0);
     w.mq = take(n * I);
     w.ms = take(n * blocks128(I) * 4);
-    w.y = take(n * H * (f32 ? 4 : 2));
+    w.y = take(size_t(w.down.n) * n * H * (f32 || w.down.n > 1 ? 4 : 2));
     w.total = o;
     return w;
 }
@@ -349,7 +440,7 @@ hf_status hf_fp8_quantize(const void* x, hf_dtype x_dtype, long long ldx, int T,
 
 size_t hf_fp8_gemm_workspace_size(int T, int N, int K) {
     if (T <= 0 || N <= 0 || K <= 0) return 0;
-    const Fp8Split sp = fp8_split(T, N, K);
+    const Fp8Split sp = fp8_gemm_split(T, N, K);
     return kAlign + (sp.n > 1 ? up(size_t(sp.n) * T * N * sizeof(float)) : 0);
 }
 
@@ -389,7 +480,7 @@ hf_status hf_fp8_gemm(const uint8_t* xq, const float* sx, const uint8_t* wq, con
 size_t hf_fp8_moe_experts_workspace_size(int T, int top_k, int E, int H, int I,
                                          hf_dtype out_dtype) {
     if (T <= 0 || top_k <= 0 || E <= 0 || H <= 0 || I <= 0) return 0;
-    return experts_ws(T, top_k, H, I, out_dtype == HF_F32).total;
+    return experts_ws(T, top_k, E, H, I, out_dtype == HF_F32).total;
 }
 
 hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E, int H, int I,
@@ -418,7 +509,7 @@ hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E,
     if (reinterpret_cast<uintptr_t>(workspace) % kAlign)
         return fail(HF_ERR_ARG, f + ": workspace must be 256-byte aligned");
     const bool f32 = out_dtype == HF_F32;
-    const ExpertsWs L = experts_ws(T, top_k, H, I, f32);
+    const ExpertsWs L = experts_ws(T, top_k, E, H, I, f32);
     if (workspace_bytes < L.total)
         return fail(HF_ERR_ARG, f + ": workspace smaller than hf_fp8_moe_experts_workspace_size");
     if (resid && resid != out) {
@@ -457,38 +548,45 @@ hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E,
     a.a_stride = 3 * I;
     a.sw = scales;
     a.sw_stride = 3ll * ib * hb;
-    a.sw_up = (long long)ib * hb;
     a.offsets = r->offsets;
     a.G = E;
     a.rows = n;
-    a.N = I;
     a.K = H;
-    a.nsplit = 1;
-    a.kbper = hb;
-    a.mid_q = ws + L.mq;
-    a.mid_s = reinterpret_cast<float*>(ws + L.ms);
+    a.nsplit = L.up.n;  // 1 unless few
+    a.kbper = L.up.per;
     a.err = qa.err;
-    HF_TRY(launch_fp8_product(a, true, st));
-    a.xq = a.mid_q;
-    a.sx = a.mid_s;
+    uint8_t* mq = ws + L.mq;
+    float* ms = reinterpret_cast<float*>(ws + L.ms);
+    if (L.few) {
+        float* gu = reinterpret_cast<float*>(ws + L.gu);
+        a.N = 2 * I;
+        a.out = gu;
+        a.out_f32 = 1;
+        HF_TRY(launch_fp8_product(a, false, st));
+        HF_CUDA(launch_pdl(k_swiglu_planes, dim3(unsigned((n * ib + 15) / 16)), dim3(256), 0, st,
+                           static_cast<const float*>(gu), L.up.n, n, I, ib, mq, ms));
+    } else {
+        a.N = I;
+        a.sw_up = (long long)ib * hb;
+        a.mid_q = mq;
+        a.mid_s = ms;
+        HF_TRY(launch_fp8_product(a, true, st));
+    }
+    a.xq = mq;
+    a.sx = ms;
     a.a_rows = 3ll * E * H;
     a.a_stride = 3 * H;
     a.a_base = 2 * H;
     a.sw = scales + 2ll * ib * hb;
     a.N = H;
     a.K = I;
-    a.kbper = ib;
+    a.nsplit = L.down.n;
+    a.kbper = L.down.per;
     a.out = ws + L.y;
-    a.out_f32 = f32;
+    a.out_f32 = f32 || L.down.n > 1;
     HF_TRY(launch_fp8_product(a, false, st));
-    const int v = f32 ? 4 : 8;
-    const dim3 grid(unsigned(T), unsigned((H / v + 255) / 256));
-    const void* y = ws + L.y;
-    const int32_t* pos = qa.pos;
-    const float* w = r->topk_weights;
-    HF_CUDA(launch_pdl(f32 ? k_fp8_combine<true> : k_fp8_combine<false>, grid, dim3(256), 0, st, y,
-                       pos, w, T, top_k, H, resid, out));
-    return HF_OK;
+    return launch_fp8_combine(ws + L.y, L.down.n, qa.pos, r->topk_weights, T, top_k, H, resid, out,
+                              f32, st);
 }
 
 hf_status hf_fp8_status(const void* workspace, hf_stream stream) {

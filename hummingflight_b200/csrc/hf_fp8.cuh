@@ -65,8 +65,8 @@ struct Fp8Args {
     // product: out [rows x N], bf16 or f32
     void* out;
     int out_f32;
-    // runs of K (one group): run s takes blocks [s * kbper, ...) and writes rows
-    // [s * rows, ...) of out
+    // runs of K: run s takes blocks [s * kbper, ...) and writes rows [s * rows, ...)
+    // of out (fp32 when there are several)
     int nsplit, kbper;
     // gate/up: the up rows follow the N gate rows, their scales sw_up floats
     // further; silu(g) * u quantised into mid_q [rows x N], mid_s [rows x ceil(N/128)]
@@ -77,11 +77,12 @@ struct Fp8Args {
     int clear_err;          // the first kernel of a call clears it
 };
 hf_status launch_fp8_product(const Fp8Args& a, bool glu, cudaStream_t st);
-// One group, with its runs of K chosen by size; planes: fp32 [n x T x N] when n > 1.
 struct Fp8Split {
-    int n, per;
+    int n, per;  // runs, blocks of K in each
 };
-Fp8Split fp8_split(int T, int N, int K);
+Fp8Split fp8_split(long long tiles, bool pair, int K, double plane_bytes);
+// One group, with its runs of K chosen by size; planes: fp32 [n x T x N] when n > 1.
+Fp8Split fp8_gemm_split(int T, int N, int K);
 hf_status launch_fp8_gemm(const Fp8Args& a, float* planes, cudaStream_t st);
 
 }  // namespace hf

@@ -216,12 +216,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(final_bar, 1);
         *abort_flag = 0;
         fence_mbar_init();
-        if (a.clear_err && blockIdx.x == 0) *a.err = 0;
     }
     if (warp == 1) {
         tmem_alloc(tmem_slot, C::kTmemCols);
         tmem_relinquish();
     }
+    griddep_wait();  // the rows, the offsets, the workspace's earlier users
+    if (a.clear_err && blockIdx.x == 0 && threadIdx.x == 0) *a.err = 0;
     load_plan<BN>(a, MB, off, pref);
     tc_fence_before();
     __syncthreads();
@@ -649,12 +650,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         mbar_init(final_bar, 2);
         *abort_flag = 0;
         fence_mbar_init();
-        if (a.clear_err && blockIdx.x == 0) *a.err = 0;
     }
     if (warp == 1) {
         tmem_alloc_pair(tmem_slot, 512);
         tmem_relinquish_pair();
     }
+    griddep_wait();  // the rows, the offsets, the workspace's earlier users
+    if (a.clear_err && blockIdx.x == 0 && threadIdx.x == 0) *a.err = 0;
     load_plan<256>(a, MB, off, pref);
     tc_fence_before();
     __syncthreads();
@@ -974,8 +976,8 @@ hf_status launch_pair(const Fp8Args& a, cudaStream_t st) {
     CUtensorMap A, B;
     HF_TRY(make_map_u8(&A, a.w, a.K, a.a_rows, a.K, 128));
     HF_TRY(make_map_u8(&B, a.xq, a.K, a.rows, a.K, kPairBox));
-    kern<<<pair_grid(kp, pair_smem(kMaxExperts), dev), kPairThreads, smem, st>>>(A, B, a);
-    HF_CUDA(cudaGetLastError());
+    HF_CUDA(launch_pdl(kern, dim3(unsigned(pair_grid(kp, pair_smem(kMaxExperts), dev))),
+                       dim3(kPairThreads), size_t(smem), st, A, B, a));
     return HF_OK;
 }
 
@@ -990,22 +992,19 @@ hf_status launch_one(const Fp8Args& a, cudaStream_t st) {
     CUtensorMap A, B;
     HF_TRY(make_map_u8(&A, a.w, a.K, a.a_rows, a.K, 128));
     HF_TRY(make_map_u8(&B, a.xq, a.K, a.rows, a.K, C::kBoxB));
-    kern<<<num_sms(dev), kThreads, smem, st>>>(A, B, a);
-    HF_CUDA(cudaGetLastError());
+    HF_CUDA(launch_pdl(kern, dim3(unsigned(num_sms(dev))), dim3(kThreads), size_t(smem), st, A, B, a));
     return HF_OK;
 }
 
 }  // namespace
 
-// The runs of K of one product: with fewer tiles than the GPU has places for
-// (148 CTAs, or 74 pairs), each tile's blocks of K are dealt to several CTAs that
-// write fp32 planes, which a second launch adds in order. The number that
-// minimises rounds x (blocks + 2 to fill the pipeline) + the sum pass; a block
-// takes about 0.75 us where the weights stream from memory (0.6 us on a pair).
-Fp8Split fp8_split(int T, int N, int K) {
+// The runs of K of a product: with few tiles for the GPU's places (148 CTAs, or
+// 74 pairs), each tile's blocks of K are dealt to several CTAs that write fp32
+// planes, which the next launch adds in order. The number that minimises
+// rounds x (blocks + 0.5 for the tile's end) + the planes' traffic; a block takes
+// about 0.7 us where the weights stream from memory.
+Fp8Split fp8_split(long long tiles, bool pair, int K, double plane_bytes) {
     const int KB = (K + kFp8Block - 1) / kFp8Block;
-    const bool pair = T > kNarrowRows;
-    const long long tiles = (long long)((N + 255) / 256) * (pair ? (T + 255) / 256 : 1);
     const int slots = pair ? 74 : 148, mult = pair ? 4 : 1;
     Fp8Split best{1, KB};
     double least = 1e30;
@@ -1013,14 +1012,21 @@ Fp8Split fp8_split(int T, int N, int K) {
         const int per = ((KB + n - 1) / n + mult - 1) / mult * mult;
         if ((KB + per - 1) / per != n) continue;  // no empty run
         const double rounds = double((tiles * n + slots - 1) / slots);
-        const double sum = n == 1 ? 0.0 : (2.0 + n * 8e-6 * T * N / 5.0) / 0.7;
-        const double cost = rounds * (per + 2) + sum;
+        // written and read once at about 5 TB/s, and a launch
+        const double sum = n == 1 ? 0.0 : (2.0 + n * plane_bytes * 2.0 / 5e6) / 0.7;
+        const double cost = rounds * (per + 0.5) + sum;
         if (cost < least) {
             least = cost;
             best = Fp8Split{n, per};
         }
     }
     return best;
+}
+
+Fp8Split fp8_gemm_split(int T, int N, int K) {
+    const bool pair = T > kNarrowRows;
+    return fp8_split((long long)((N + 255) / 256) * (pair ? (T + 255) / 256 : 1), pair, K,
+                     4.0 * T * N);
 }
 
 __global__ void __launch_bounds__(256) k_sum_planes(const float* planes, int n, long long count,
@@ -1070,7 +1076,7 @@ __global__ void __launch_bounds__(256) k_sum_planes(const float* planes, int n, 
 
 hf_status launch_fp8_gemm(const Fp8Args& args, float* planes, cudaStream_t st) {
     Fp8Args a = args;
-    const Fp8Split sp = fp8_split(a.rows, a.N, a.K);
+    const Fp8Split sp = fp8_gemm_split(a.rows, a.N, a.K);
     a.nsplit = sp.n;
     a.kbper = sp.per;
     if (sp.n > 1) {
