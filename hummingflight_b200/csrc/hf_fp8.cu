@@ -20,7 +20,7 @@ int blocks128(int n) { return (n + kFp8Block - 1) / kFp8Block; }
 // One pass bound by memory: 16 threads own a block of 128 columns, 8 columns
 // (16 or 32 bytes) each, so the maximum is four shuffles and every load and store
 // is whole sectors; a thread has kQuantBatch blocks' loads in flight.
-// 16384 x 6144 bf16: @QT16384@.
+// 16384 x 6144 bf16: 57 us, 5.3 TB/s of 6.5 measured.
 struct QuantArgs {
     const void* x;
     long long ldx;
@@ -198,8 +198,10 @@ __global__ void __launch_bounds__(256) k_quantize_tokens(QuantArgs a) {
     }
 }
 
-// Positions from which the experts' gather goes by tokens: @GATHER@.
-constexpr int kTokenMajor = 4096;
+// Positions from which the experts' gather goes by tokens. H = 6144, k = 8, us by
+// positions and by tokens (two launches): 512 positions 4.8 and 6.6, 2048: 12.7
+// and 7.9, 8192: 43.8 and 16.3, 32768: 161 and 45.
+constexpr int kTokenMajor = 1024;
 
 hf_status launch_quantize(const QuantArgs& a, bool f32, int dev, cudaStream_t st) {
     if (a.perm && a.rows >= kTokenMajor && a.k > 1) {
@@ -270,7 +272,7 @@ __device__ __forceinline__ void unpack(const uint4 v, float (&f)[4]) {
 __device__ __forceinline__ void unpack(const uint4 v, float (&f)[8]) { unpack8(v, f); }
 
 // A thread takes 16 bytes of a token's columns, all of its picks' loads in flight
-// before the first is used. T = 16384, k = 8, H = 6144, bf16: @COMBINE@.
+// before the first is used. T = 16384, k = 8, H = 6144, bf16: 299 us, 6.0 TB/s.
 // Y32: the expert outputs are fp32, in n planes (runs of K) that are added in order.
 template <bool Y32, bool F32>
 __global__ void __launch_bounds__(256) k_fp8_combine(const void* y, int n, const int32_t* pos,
@@ -362,7 +364,7 @@ hf_status launch_fp8_combine(const void* y, int n, const int32_t* pos, const flo
 // Runs of K of the experts' products: few positions make few tiles (at most one
 // per position and row block of the weights); beyond this number the tiles fill
 // the GPU.
-constexpr int kFewPositions = 64;
+constexpr int kFewPositions = 512;
 
 struct ExpertsWs {
     Fp8Split up, down;  // runs of the gate/up and down products

@@ -38,7 +38,13 @@ using namespace sm100;
 
 constexpr int kThreads = 384;
 constexpr int kAccWarps = 8;
-constexpr int kNarrowRows = 64;  // positions per segment up to which the weights are the MMA's M
+// Mean positions per segment up to which the weights are the MMA's M, and up to
+// which a tile takes 32 positions instead of 64. 32 experts of 6144 x 2048, the
+// three kernels' us: mean 4: 226 (32), 234 (64), 378 (pair); 48: 274, 279, 386;
+// 64: 277, 293, 384; 96: 392, 389, 394; 128: 490, 420, 394. One matrix, 64
+// rows x 12288 -> 6144: 24.6 (32), 22.3 (64).
+constexpr int kNarrowRows = 96;
+constexpr int kNarrow32 = 48;
 constexpr int kScaleSlots = 4;
 constexpr uint32_t kABytes = 128 * 128;  // 128 weight rows x 128 bytes
 constexpr uint64_t kWaitNs = 2000ull * 1000 * 1000;
@@ -48,9 +54,9 @@ template <int BN>
 struct Cfg {
     static constexpr int kStageBytes = 2 * kABytes + BN * 128;
     static constexpr int kCols = 2 * BN;                     // TMEM columns of one buffer
-    static constexpr int kBufs = 512 / kCols >= 4 ? 4 : 2;
+    static constexpr int kBufs = 4;
     static constexpr uint32_t kTmemCols = kBufs * kCols;     // a power of two, 128..512
-    static constexpr int kBoxB = BN < 32 ? BN : 32;          // position rows of one TMA box
+    static constexpr int kBoxB = 32;                         // position rows of one TMA box
     static constexpr int kScaleBytes = kScaleSlots * 2 * BN * 4;
     static constexpr int kRedBytes = 5 * BN * 4;             // maxima of 4 quadrants, 1 / scale
     static constexpr int kBarBytes = 512;
@@ -181,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const Fp8Args a) {
     using C = Cfg<BN>;
     constexpr int S = C::kStages, NB = C::kBufs;
-    constexpr int CH = BN >= 32 ? BN / 32 : 1;  // 16-column chunks of one accumulation warp
+    constexpr int CH = BN / 32;  // 16-column chunks of one accumulation warp
     extern __shared__ __align__(1024) uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
                                                ~uintptr_t(1023));
@@ -301,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             drain_wait(final_bar, 0);
         } else if (warp == 2) {
             // ------------------------------------------------------ scales
-            constexpr int PL = (BN + 31) / 32;
+            constexpr int PL = BN / 32;
             uint32_t it = 0;
             bool ok = true;
             for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
@@ -333,10 +339,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int j = 0; j < PL; ++j) {
                         const int c = j * 32 + lane;
-                        if (c < BN) {
-                            p[c] = x[j] * w0;
-                            p[BN + c] = x[j] * w1;
-                        }
+                        p[c] = x[j] * w0;
+                        p[BN + c] = x[j] * w1;
                         x[j] = xn[j];
                     }
                     w0 = v0;
@@ -1025,8 +1029,8 @@ Fp8Split fp8_split(long long tiles, bool pair, int K, double plane_bytes) {
 
 Fp8Split fp8_gemm_split(int T, int N, int K) {
     const bool pair = T > kNarrowRows;
-    return fp8_split((long long)((N + 255) / 256) * (pair ? (T + 255) / 256 : 1), pair, K,
-                     4.0 * T * N);
+    const int bn = pair ? 256 : T > kNarrow32 ? 64 : 32;
+    return fp8_split((long long)((N + 255) / 256) * ((T + bn - 1) / bn), pair, K, 4.0 * T * N);
 }
 
 __global__ void __launch_bounds__(256) k_sum_planes(const float* planes, int n, long long count,
@@ -1096,9 +1100,8 @@ hf_status launch_fp8_gemm(const Fp8Args& args, float* planes, cudaStream_t st) {
 hf_status launch_fp8_product(const Fp8Args& a, bool glu, cudaStream_t st) {
     const int avg = (a.rows + a.G - 1) / a.G;
     if (avg > kNarrowRows) return glu ? launch_pair<true>(a, st) : launch_pair<false>(a, st);
-    if (avg > 32) return glu ? launch_one<true, 64>(a, st) : launch_one<false, 64>(a, st);
-    if (avg > 16) return glu ? launch_one<true, 32>(a, st) : launch_one<false, 32>(a, st);
-    return glu ? launch_one<true, 16>(a, st) : launch_one<false, 16>(a, st);
+    if (avg > kNarrow32) return glu ? launch_one<true, 64>(a, st) : launch_one<false, 64>(a, st);
+    return glu ? launch_one<true, 32>(a, st) : launch_one<false, 32>(a, st);
 }
 
 }  // namespace hf

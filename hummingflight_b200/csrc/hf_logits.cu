@@ -621,11 +621,12 @@ hf_status launch(const LogitArgs& a, cudaStream_t st) {
     const int threads = std::min(kThreads, std::max(8, std::min(a.T, a.tb)) * 32);
     const int own = smem + (nb == 1 ? a.T * a.k * 4 : 0) +
                     (a.topk_group < a.n_group ? threads / 32 * a.E * 8 : 0);
-    HF_CUDA(ensure_smem(reinterpret_cast<const void*>(kern), own));
+    if (own > 48 * 1024) HF_CUDA(ensure_smem(reinterpret_cast<const void*>(kern), own));
     kern<<<nb, threads, own, st>>>(a);
     HF_CUDA(cudaGetLastError());
     if (nb > 1) {
-        HF_CUDA(ensure_smem(reinterpret_cast<const void*>(k_route_scatter), smem));
+        if (smem > 48 * 1024)
+            HF_CUDA(ensure_smem(reinterpret_cast<const void*>(k_route_scatter), smem));
         HF_CUDA(launch_pdl(k_route_scatter, dim3(nb), dim3(nb > 16 ? 1024 : 256), size_t(smem), st, a, nb));
     }
     return HF_OK;

@@ -42,7 +42,9 @@ HF_API hf_status hf_fp8_quantize(const void* x, hf_dtype x_dtype, long long ldx,
  * [T x ceil(K/128)] (any values, not only powers of two); wq: e4m3 [N x K];
  * sw: fp32 [ceil(N/128) x ceil(K/128)]; out: [T x N] of out_dtype. K a multiple
  * of 16, any T and N; xq, wq and the workspace 16-byte (workspace: 256-byte)
- * aligned. The single-token form reads the weight once on the CUDA cores. */
+ * aligned. Sums of up to 128 products are taken by the tensor cores in fp32; with
+ * few output tiles K is cut into runs whose fp32 partial sums lie in the workspace
+ * and are added in order, so equal calls give equal bits. */
 HF_API size_t hf_fp8_gemm_workspace_size(int T, int N, int K);
 HF_API hf_status hf_fp8_gemm(const uint8_t* xq, const float* sx, const uint8_t* wq, const float* sw,
                              int T, int N, int K, void* out, hf_dtype out_dtype, void* workspace,

@@ -80,7 +80,10 @@ def test_quantize_rows_apart_and_out():
 # ------------------------------------------------------------------ product
 GEMM = [(1, 1, 16), (1, 128, 128), (1, 1000, 2064), (2, 257, 144), (7, 384, 1024), (16, 130, 256),
         (17, 64, 4112), (31, 1, 512), (33, 513, 640), (64, 640, 384), (100, 129, 1040),
-        (128, 256, 128), (129, 300, 272), (333, 1000, 528), (515, 260, 160)]
+        (128, 256, 128), (129, 300, 272), (333, 1000, 528), (515, 260, 160),
+        (97, 384, 2048), (49, 200, 1024),
+        # more tiles than CTAs or CTA pairs: several a CTA
+        (40, 40100, 256), (300, 10000, 272)]
 
 
 @pytest.mark.parametrize("T,N,K", GEMM)
@@ -182,7 +185,12 @@ def make_routing(rng, T, E, k, skew=1.0, only=None):
 EXPERTS = [  # T, E, k, H, I
     (1, 4, 2, 256, 128), (1, 1, 1, 16, 16), (1, 8, 8, 400, 144), (2, 16, 4, 256, 256),
     (5, 8, 3, 528, 272), (16, 33, 6, 384, 128), (40, 8, 2, 512, 384), (64, 16, 4, 144, 400),
-    (130, 4, 2, 640, 256), (257, 3, 3, 256, 160), (300, 2, 1, 272, 512)]
+    (130, 4, 2, 640, 256), (257, 3, 3, 256, 160), (300, 2, 1, 272, 512),
+    # runs of K of the gate/up product (whole blocks of I) and of the down product
+    (1, 4, 2, 4096, 256), (3, 6, 2, 2048, 384), (2, 4, 2, 2048, 272), (1, 2, 2, 256, 2048),
+    # many picks; many tiles; tokens enough for the token-major gather
+    (4, 40, 32, 128, 128), (100, 40, 2, 256, 512), (1000, 16, 2, 256, 1024),
+    (2100, 4, 2, 272, 128)]
 
 
 @pytest.mark.parametrize("T,E,k,H,I", EXPERTS)
@@ -299,3 +307,74 @@ def test_routing_of_the_bf16_layer_is_taken():
                          r["topk_weights"].double().cpu().numpy(), 128)
     assert (np.abs(y.double().cpu().numpy() - ref) <= tol).all()
     L.close()
+
+
+def test_experts_whose_offsets_pass_32_bits():
+    """The last expert's block starts beyond 2^32 bytes; the other experts' bytes are
+    left as they came (never read)."""
+    need_gpu()
+    from hummingflight_b200 import fp8
+    rng = np.random.default_rng(8)
+    E, H, I, T = 400, 2048, 1792, 3
+    n, nb = I * H, R.blocks(I) * R.blocks(H)
+    q = torch.empty((E, 3 * n), dtype=torch.uint8, device="cuda")
+    s = torch.empty((E, 3 * nb), device="cuda")
+    assert (E - 1) * 3 * n > 2 ** 32
+    one, os, full = make_experts(rng, 1, H, I)
+    q[E - 1], s[E - 1] = one[0], os[0]
+    off = torch.zeros(E + 2, dtype=torch.int32, device="cuda")
+    off[E:] = T
+    routing = dict(topk_weights=torch.full((T, 1), 0.75, device="cuda"), offsets=off,
+                   perm=torch.arange(T, dtype=torch.int32, device="cuda"))
+    for rows_ in (T, 100):
+        routing.update(topk_weights=torch.full((rows_, 1), 0.75, device="cuda"),
+                       perm=torch.arange(rows_, dtype=torch.int32, device="cuda"))
+        off[E:] = rows_
+        x, xd = rows(rng, rows_, H, "bf16")
+        y = fp8.moe_experts(x.cuda(), q, s, routing)
+        ref, tol = R.experts(xd, full, np.zeros((rows_, 1), int), np.full((rows_, 1), 0.75), I)
+        assert (np.abs(y.double().cpu().numpy() - ref) <= tol).all()
+
+
+def test_experts_bad_permutation_stays_in_bounds():
+    """Entries and offsets out of range: the call returns, and rows that are named
+    properly keep their values."""
+    need_gpu()
+    from hummingflight_b200 import fp8
+    rng = np.random.default_rng(3)
+    for T in (6, 1200):
+        E, k, H, I = 4, 1, 256, 128
+        q, s, _ = make_experts(rng, E, H, I)
+        x = rows(rng, T, H, "bf16")[0].cuda()
+        r = dict(topk_weights=torch.ones((T, k), device="cuda"),
+                 offsets=torch.tensor([0, T, T, T, T, T], dtype=torch.int32, device="cuda"),
+                 perm=torch.arange(T, dtype=torch.int32, device="cuda"))
+        good = fp8.moe_experts(x, q, s, r).clone()
+        r["perm"][2], r["perm"][3] = -5, 2 ** 30
+        ws = torch.full((fp8.moe_experts_workspace_size(T, k, E, H, I),), 255, dtype=torch.uint8,
+                        device="cuda")
+        y = fp8.moe_experts(x, q, s, r, workspace=ws)
+        keep = [t for t in range(T) if t not in (2, 3)]
+        assert torch.equal(y[keep], good[keep])
+        r["offsets"].copy_(torch.tensor([-7, T + 100, 2 ** 30, 5, -1, T], dtype=torch.int32))
+        fp8.moe_experts(x, q, s, r, workspace=ws)
+        fp8.status(ws)
+
+
+def test_two_streams_at_once():
+    """Independent calls that overlap on two streams, each with its own workspace."""
+    need_gpu()
+    from hummingflight_b200 import fp8
+    rng = np.random.default_rng(11)
+    T, E, k, H, I = 200, 8, 2, 512, 256
+    q, s, _ = make_experts(rng, E, H, I)
+    a, _, _ = make_routing(rng, T, E, k)
+    b, _, _ = make_routing(rng, T, E, k)
+    x = rows(rng, T, H, "bf16")[0].cuda()
+    want = [fp8.moe_experts(x, q, s, r).clone() for r in (a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(10):
+        got = [fp8.moe_experts(x, q, s, r, stream=st) for r, st in zip((a, b), streams)]
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
