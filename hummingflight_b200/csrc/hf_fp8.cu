@@ -494,6 +494,8 @@ hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E,
     if (E < 1 || E > kMaxExperts) return fail(HF_ERR_ARG, f + ": E must be in 1..1024");
     if (H <= 0 || I <= 0 || H % 16 || I % 16)
         return fail(HF_ERR_ARG, f + ": H and I must be positive multiples of 16");
+    if (3ll * E * std::max(H, I) > 0x7fffffffll)
+        return fail(HF_ERR_ARG, f + ": 3 * E * max(H, I) must be below 2^31");
     if (top_k < 1 || top_k > kMaxK) return fail(HF_ERR_ARG, f + ": top_k must be in 1..32");
     if (T < 0 || (long long)T * top_k > 0x7fffffffll)
         return fail(HF_ERR_ARG, f + ": T >= 0 and T * top_k below 2^31");

@@ -35,6 +35,7 @@ namespace {
 constexpr int kMaxRouteK = 32;      // one lane per pick
 constexpr int kMaxRouteGroups = 32;
 constexpr int kOneBlockT = 16;      // tokens one block routes and permutes in one launch
+constexpr int kScanBlocks = 512;    // blocks of tokens from which their counts are scanned first
 constexpr size_t kWsAlign = 256;
 
 struct LogitArgs {
@@ -549,7 +550,24 @@ __global__ void __launch_bounds__(THREADS) k_route_logits(LogitArgs a) {
     scatter(a, masks, base, s_ids, t0, nt, words);
 }
 
-__global__ void __launch_bounds__(1024) k_route_scatter(LogitArgs a, int nb) {
+// Very long batches: blk becomes its exclusive prefix over the blocks (row nb: the
+// totals), so that the scatter need not add up every block's counts.
+__global__ void __launch_bounds__(32) k_route_scan(LogitArgs a, int nb) {
+    const int e = blockIdx.x * 32 + threadIdx.x;
+    if (e >= a.E) return;
+    int run = 0;
+#pragma unroll 8
+    for (int q = 0; q < nb; ++q) {
+        int32_t* p = a.blk + size_t(q) * a.E + e;
+        const int c = *p;
+        *p = run;
+        run += c;
+    }
+    a.blk[size_t(nb) * a.E + e] = run;
+}
+
+// `scanned`: after k_route_scan.
+__global__ void __launch_bounds__(1024) k_route_scatter(LogitArgs a, int nb, int scanned) {
     extern __shared__ __align__(16) uint32_t sm[];
     const int words = (a.tb + 31) / 32;
     uint32_t* masks = sm;
@@ -564,7 +582,12 @@ __global__ void __launch_bounds__(1024) k_route_scatter(LogitArgs a, int nb) {
     // are spread over the block; integer sums, any order
     const int cols = min(a.E, int(blockDim.x)), slices = int(blockDim.x) / cols;
     const int slice = int(threadIdx.x) / cols;
-    if (slice < slices) {
+    if (scanned) {
+        for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
+            total[e] = a.blk[size_t(nb) * a.E + e];
+            base[e] = a.blk[size_t(b) * a.E + e];
+        }
+    } else if (slice < slices) {
         for (int e = int(threadIdx.x) % cols; e < a.E; e += cols) {
             int all = 0, before = 0;
 #pragma unroll 8
@@ -607,7 +630,7 @@ int blocks_of(int T) {
 
 size_t ws_bytes(int T, int E) {
     if (T <= kOneBlockT) return 0;
-    return (size_t(blocks_of(T)) * E * sizeof(int32_t) + kWsAlign - 1) / kWsAlign * kWsAlign;
+    return (size_t(blocks_of(T) + 1) * E * sizeof(int32_t) + kWsAlign - 1) / kWsAlign * kWsAlign;
 }
 
 template <int NPL>
@@ -627,7 +650,13 @@ hf_status launch(const LogitArgs& a, cudaStream_t st) {
     if (nb > 1) {
         if (smem > 48 * 1024)
             HF_CUDA(ensure_smem(reinterpret_cast<const void*>(k_route_scatter), smem));
-        HF_CUDA(launch_pdl(k_route_scatter, dim3(nb), dim3(nb > 16 ? 1024 : 256), size_t(smem), st, a, nb));
+        const int scan = nb > kScanBlocks;
+        if (scan) {
+            k_route_scan<<<(a.E + 31) / 32, 32, 0, st>>>(a, nb);
+            HF_CUDA(cudaGetLastError());
+        }
+        HF_CUDA(launch_pdl(k_route_scatter, dim3(nb), dim3(nb > 16 ? 1024 : 256), size_t(smem), st,
+                           a, nb, scan));
     }
     return HF_OK;
 }

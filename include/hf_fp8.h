@@ -65,10 +65,10 @@ HF_API hf_status hf_fp8_gemm(const uint8_t* xq, const float* sx, const uint8_t* 
  * hf_route_logits or hf_moe_route for the same T and k (a shared segment behind
  * the routed ones is left out; topk_ids is not read); offsets, perm entries out
  * of range are skipped. resid: device [T x H] of out_dtype or NULL, may be out
- * itself. out: device [T x H] of out_dtype; the expert outputs are kept in the
- * same type until the combine. The shared expert, or a dense MLP, is the call
+ * itself. out: device [T x H] of out_dtype; the expert outputs y_i are kept in
+ * the same type until the combine (bf16 outputs: y_i rounded once more). The shared expert, or a dense MLP, is the call
  * with E = 1, k = 1 and the routed output as resid. H and I multiples of 16,
- * k in 1..32, E in 1..1024, T * k below 2^31; pointers 16-byte aligned, the
+ * k in 1..32, E in 1..1024, T * k and 3 * E * max(H, I) below 2^31; pointers 16-byte aligned, the
  * workspace 256-byte. A workspace serves any number of layers in stream order. */
 HF_API size_t hf_fp8_moe_experts_workspace_size(int T, int top_k, int E, int H, int I,
                                                 hf_dtype out_dtype);

@@ -105,7 +105,7 @@ def test_experts_refusals():
         return L.hf_fp8_moe_experts(*{**ok, **kw}.values())
 
     for b in (dict(E=0), dict(E=1025), dict(H=0), dict(H=248), dict(I=0), dict(I=120), dict(T=-1),
-              dict(k=0), dict(k=33), dict(T=1 << 30, k=4), dict(xt=4), dict(ot=4), dict(w=None),
+              dict(k=0), dict(k=33), dict(T=1 << 30, k=4), dict(E=1024, H=1 << 20), dict(xt=4), dict(ot=4), dict(w=None),
               dict(s=None), dict(x=None), dict(out=None), dict(ws=None), dict(r=None),
               dict(r=_lib.HfMoeRouting(None, None, None, None, P, P, None)),
               dict(r=_lib.HfMoeRouting(None, P, None, None, None, P, None)),

@@ -70,12 +70,12 @@ def test_matches_plain_form(T, E, k, score, bias, ng, tg, gt, norm, dtype):
     check(l, b, k, score, ng, tg, gt, 2.5, norm)
 
 
-@pytest.mark.parametrize("T", [9473, 70000])
-def test_long_batches(T):
-    """Several blocks of 128 and of 512 tokens."""
+@pytest.mark.parametrize("T,E", [(1190, 40), (9473, 8), (70000, 8), (270000, 3)])
+def test_long_batches(T, E):
+    """Blocks of 16, 64 and 512 tokens, and so many that their counts are scanned."""
     need_gpu()
     g = torch.Generator().manual_seed(T)
-    check(torch.randn((T, 8), generator=g).cuda(), None, 2, "softmax")
+    check(torch.randn((T, E), generator=g).cuda(), None, 2, "softmax")
 
 
 def test_empty_batch():
