@@ -330,9 +330,17 @@ __device__ __forceinline__ int route_token(const LogitArgs& a, const float (&bia
     const bool softmax = a.score == HF_SCORE_SOFTMAX;
     float l[NPL];
     uint32_t c[NPL];
+    // (uniform branches around whole loops: a choice inside one is made per expert)
+    if (a.bf16) {
+        const uint16_t* p = static_cast<const uint16_t*>(a.logits) + size_t(t) * a.E + lane;
 #pragma unroll
-    for (int j = 0; j < NPL; ++j)
-        l[j] = j * 32 + lane < a.E ? load_logit(a, size_t(t) * a.E + j * 32 + lane) : -INFINITY;
+        for (int j = 0; j < NPL; ++j)
+            l[j] = j * 32 + lane < a.E ? bf16_to_f32(p[j * 32]) : -INFINITY;
+    } else {
+        const float* p = static_cast<const float*>(a.logits) + size_t(t) * a.E + lane;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) l[j] = j * 32 + lane < a.E ? p[j * 32] : -INFINITY;
+    }
     float top = l[0];
 #pragma unroll
     for (int j = 1; j < NPL; ++j) top = fmaxf(top, l[j]);
@@ -356,21 +364,32 @@ __device__ __forceinline__ int route_token(const LogitArgs& a, const float (&bia
         // (e^-x (2 + 1.2 x) <= 2), the sum's error below 3 and NPL + 5 roundings:
         // < 2^-18 smax. Two keys can be off by twice that (tol), two groups' sums
         // of two by four times; the roundings of the sums are above()'s.
+        float s[NPL];
+        if (softmax) {
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) s[j] = fmaf(__expf(l[j] - m), inv, bias[j]);
+            tol = inv * 0x1p-17f;
+        } else {
+#pragma unroll
+            for (int j = 0; j < NPL; ++j)
+                s[j] = __fdividef(1.0f, 1.0f + __expf(-l[j])) + bias[j];
+            tol = __fdividef(1.0f, 1.0f + __expf(-top)) *
+                  (0x1p-20f + fmaxf(-top, 0.0f) * 0x1p-21f);
+        }
         uint32_t key[NPL];
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) {
-            const float s = softmax ? __expf(l[j] - m) * inv
-                                    : __fdividef(1.0f, 1.0f + __expf(-l[j]));
-            key[j] = j * 32 + lane < a.E ? packed<NPL>(code_of(s + bias[j]), j) : 0u;
-        }
-        if (softmax) tol = inv * 0x1p-17f;
-        else tol = __fdividef(1.0f, 1.0f + __expf(-top)) *
-                   (0x1p-20f + fmaxf(-top, 0.0f) * 0x1p-21f);
-#pragma unroll
         for (int j = 0; j < NPL; ++j)
-            c[j] = !by_logit ? key[j]
-                             : j * 32 + lane < a.E ? packed<NPL>(code_of(l[j]), j) : 0u;
-        if (limited) keep_groups(c, key, a, lane, reinterpret_cast<uint32_t*>(scr), &ggap);
+            key[j] = j * 32 + lane < a.E ? packed<NPL>(code_of(s[j]), j) : 0u;
+        if (by_logit) {
+#pragma unroll
+            for (int j = 0; j < NPL; ++j)
+                c[j] = j * 32 + lane < a.E ? packed<NPL>(code_of(l[j]), j) : 0u;
+            keep_groups(c, key, a, lane, reinterpret_cast<uint32_t*>(scr), &ggap);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) c[j] = key[j];
+            if (limited) keep_groups(c, c, a, lane, reinterpret_cast<uint32_t*>(scr), &ggap);
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < NPL; ++j)
@@ -413,8 +432,9 @@ __device__ __forceinline__ int route_token(const LogitArgs& a, const float (&bia
 
     // the picks' scores once more, accurately
     const float lp = load_logit(a, size_t(t) * a.E + (lane < a.k ? mine : 0));
-    float ws = softmax ? __fmul_rn(expf(lp - m), inv)
-                       : __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-lp)));
+    float ws;
+    if (softmax) ws = __fmul_rn(expf(lp - m), inv);
+    else ws = __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-lp)));
     if (lane >= a.k) ws = 0.0f;
     float sum = 0.0f;  // rank order, as topKScores sums
 #pragma unroll 1
@@ -566,6 +586,39 @@ __global__ void __launch_bounds__(32) k_route_scan(LogitArgs a, int nb) {
     a.blk[size_t(nb) * a.E + e] = run;
 }
 
+// Per-expert tokens of all blocks, and of those before b. Threads cover (slice of
+// blocks, V experts); integer sums, any order.
+template <int V>
+__device__ __forceinline__ void add_counts(const LogitArgs& a, int nb, int b, int* total, int* base) {
+    const int cols = min(a.E / V, int(blockDim.x)), slices = int(blockDim.x) / cols;
+    const int slice = int(threadIdx.x) / cols;
+    if (slice >= slices) return;
+    for (int c = int(threadIdx.x) % cols; c < a.E / V; c += cols) {
+        int all[V] = {}, before[V] = {};
+#pragma unroll 4
+        for (int q = slice; q < nb; q += slices) {
+            int v[V];
+            const int32_t* p = a.blk + size_t(q) * a.E + c * V;
+            if constexpr (V == 4) {
+                const int4 x = *reinterpret_cast<const int4*>(p);
+                v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+            } else {
+                v[0] = p[0];
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                all[e] += v[e];
+                before[e] += q < b ? v[e] : 0;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            atomicAdd(&total[c * V + e], all[e]);
+            atomicAdd(&base[c * V + e], before[e]);
+        }
+    }
+}
+
 // `scanned`: after k_route_scan.
 __global__ void __launch_bounds__(1024) k_route_scatter(LogitArgs a, int nb, int scanned) {
     extern __shared__ __align__(16) uint32_t sm[];
@@ -578,27 +631,15 @@ __global__ void __launch_bounds__(1024) k_route_scatter(LogitArgs a, int nb, int
     for (int e = threadIdx.x; e < a.E; e += blockDim.x) total[e] = base[e] = 0;
     griddep_wait();  // the ids and counts of every block
     __syncthreads();
-    // threads cover (slice of blocks, expert), so that the loads of a column
-    // are spread over the block; integer sums, any order
-    const int cols = min(a.E, int(blockDim.x)), slices = int(blockDim.x) / cols;
-    const int slice = int(threadIdx.x) / cols;
     if (scanned) {
         for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
             total[e] = a.blk[size_t(nb) * a.E + e];
             base[e] = a.blk[size_t(b) * a.E + e];
         }
-    } else if (slice < slices) {
-        for (int e = int(threadIdx.x) % cols; e < a.E; e += cols) {
-            int all = 0, before = 0;
-#pragma unroll 8
-            for (int q = slice; q < nb; q += slices) {
-                const int c = a.blk[size_t(q) * a.E + e];
-                all += c;
-                before += q < b ? c : 0;
-            }
-            atomicAdd(&total[e], all);
-            atomicAdd(&base[e], before);
-        }
+    } else if (a.E % 4 == 0) {
+        add_counts<4>(a, nb, b, total, base);
+    } else {
+        add_counts<1>(a, nb, b, total, base);
     }
     set_masks(a, masks, t0, nt, words);
     __syncthreads();
@@ -613,14 +654,12 @@ __global__ void k_route_empty(LogitArgs a) {
     }
 }
 
-// Tokens per block: all of up to 16 tokens in one; else the smallest power of two
-// from 8 on that leaves at most one block per SM, 512 at most (the second launch
-// adds up the counts of all blocks).
+// Tokens per block: all of up to 16 tokens in one; else as many as leave one block
+// per SM, in steps of 8, 512 at most (the second launch adds up the counts of all
+// blocks).
 int tokens_per_block(int T) {
     if (T <= kOneBlockT) return kOneBlockT;
-    int tb = 8;
-    while (tb < 512 && (T + tb - 1) / tb > 148) tb *= 2;
-    return tb;
+    return std::min(512, ((T + 147) / 148 + 7) / 8 * 8);
 }
 
 int blocks_of(int T) {
@@ -640,8 +679,10 @@ hf_status launch(const LogitArgs& a, cudaStream_t st) {
     const int nb = blocks_of(a.T);
     const int smem = a.E * ((a.tb + 31) / 32 + 2) * 4;
     const auto kern = k_route_logits<NPL, kThreads>;
-    // a warp per token, eight at least (they also count and permute)
-    const int threads = std::min(kThreads, std::max(8, std::min(a.T, a.tb)) * 32);
+    // a warp per token, or per equal number of tokens; eight warps at least (they
+    // also count and permute)
+    const int most = kThreads / 32, tokens = std::min(a.T, a.tb), turns = (tokens + most - 1) / most;
+    const int threads = std::max(8, (tokens + turns - 1) / turns) * 32;
     const int own = smem + (nb == 1 ? a.T * a.k * 4 : 0) +
                     (a.topk_group < a.n_group ? threads / 32 * a.E * 8 : 0);
     if (own > 48 * 1024) HF_CUDA(ensure_smem(reinterpret_cast<const void*>(kern), own));

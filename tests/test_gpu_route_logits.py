@@ -72,7 +72,7 @@ def test_matches_plain_form(T, E, k, score, bias, ng, tg, gt, norm, dtype):
 
 @pytest.mark.parametrize("T,E", [(1190, 40), (9473, 8), (70000, 8), (270000, 3)])
 def test_long_batches(T, E):
-    """Blocks of 16, 64 and 512 tokens, and so many that their counts are scanned."""
+    """Blocks of 16, 72, 480 and 512 tokens, the last so many that their counts are scanned."""
     need_gpu()
     g = torch.Generator().manual_seed(T)
     check(torch.randn((T, E), generator=g).cuda(), None, 2, "softmax")
