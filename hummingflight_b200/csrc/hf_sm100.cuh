@@ -223,39 +223,14 @@ __device__ __forceinline__ void tmem_ld_wait_regs(uint32_t (&a)[16], uint32_t (&
                  :
                  : "memory");
 }
-// 64 columns, waited for, as 32 pairs of floats (columns 2i and 2i + 1). Load,
-// wait and pairing are one statement: with the wait apart, its operands (which
-// keep the compiler from moving uses across it) cost a move for each register.
-__device__ __forceinline__ void tmem_read64(uint32_t taddr, unsigned long long (&v)[32]) {
-    asm volatile(
-        "{\n\t"
-        ".reg .b32 r0, r1, r2, r3, r4, r5, r6, r7, r8, r9, r10, r11, r12, r13, r14, r15;\n\t"
-        ".reg .b32 r16, r17, r18, r19, r20, r21, r22, r23, r24, r25, r26, r27, r28, r29, r30, r31;\n\t"
-        ".reg .b32 r32, r33, r34, r35, r36, r37, r38, r39, r40, r41, r42, r43, r44, r45, r46, r47;\n\t"
-        ".reg .b32 r48, r49, r50, r51, r52, r53, r54, r55, r56, r57, r58, r59, r60, r61, r62, r63;\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
-        "r0, r1, r2, r3, r4, r5, r6, r7, r8, r9, r10, r11, r12, r13, r14, r15, "
-        "r16, r17, r18, r19, r20, r21, r22, r23, r24, r25, r26, r27, r28, r29, r30, r31, "
-        "r32, r33, r34, r35, r36, r37, r38, r39, r40, r41, r42, r43, r44, r45, r46, r47, "
-        "r48, r49, r50, r51, r52, r53, r54, r55, r56, r57, r58, r59, r60, r61, r62, r63}, [%32];\n\t"
-        "tcgen05.wait::ld.sync.aligned;\n\t"
-        "mov.b64 %0, {r0, r1}; mov.b64 %1, {r2, r3}; mov.b64 %2, {r4, r5}; mov.b64 %3, {r6, r7};"
-        "mov.b64 %4, {r8, r9}; mov.b64 %5, {r10, r11}; mov.b64 %6, {r12, r13}; mov.b64 %7, {r14, r15};"
-        "mov.b64 %8, {r16, r17}; mov.b64 %9, {r18, r19}; mov.b64 %10, {r20, r21}; mov.b64 %11, {r22, r23};"
-        "mov.b64 %12, {r24, r25}; mov.b64 %13, {r26, r27}; mov.b64 %14, {r28, r29}; mov.b64 %15, {r30, r31};"
-        "mov.b64 %16, {r32, r33}; mov.b64 %17, {r34, r35}; mov.b64 %18, {r36, r37}; mov.b64 %19, {r38, r39};"
-        "mov.b64 %20, {r40, r41}; mov.b64 %21, {r42, r43}; mov.b64 %22, {r44, r45}; mov.b64 %23, {r46, r47};"
-        "mov.b64 %24, {r48, r49}; mov.b64 %25, {r50, r51}; mov.b64 %26, {r52, r53}; mov.b64 %27, {r54, r55};"
-        "mov.b64 %28, {r56, r57}; mov.b64 %29, {r58, r59}; mov.b64 %30, {r60, r61}; mov.b64 %31, {r62, r63};"
-        "}"
-        : "=l"(v[0]), "=l"(v[1]), "=l"(v[2]), "=l"(v[3]), "=l"(v[4]), "=l"(v[5]),
-          "=l"(v[6]), "=l"(v[7]), "=l"(v[8]), "=l"(v[9]), "=l"(v[10]), "=l"(v[11]),
-          "=l"(v[12]), "=l"(v[13]), "=l"(v[14]), "=l"(v[15]), "=l"(v[16]), "=l"(v[17]),
-          "=l"(v[18]), "=l"(v[19]), "=l"(v[20]), "=l"(v[21]), "=l"(v[22]), "=l"(v[23]),
-          "=l"(v[24]), "=l"(v[25]), "=l"(v[26]), "=l"(v[27]), "=l"(v[28]), "=l"(v[29]),
-          "=l"(v[30]), "=l"(v[31])
-        : "r"(taddr)
-        : "memory");
+// tmem_ld_wait_regs for one load.
+__device__ __forceinline__ void tmem_ld_wait_reg16(uint32_t (&a)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]),
+                   "+r"(a[6]), "+r"(a[7]), "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]),
+                   "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15])
+                 :
+                 : "memory");
 }
 
 // Shared-memory matrix descriptor of a K-major tile stored as 128-byte rows
