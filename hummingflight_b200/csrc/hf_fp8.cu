@@ -119,8 +119,8 @@ __global__ void __launch_bounds__(256) k_quantize_flat(const void* x, long long 
 // Any pitch, ragged last blocks, gathered rows.
 template <bool XF32>
 __global__ void __launch_bounds__(256) k_quantize(QuantArgs a) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();  // behind the wait: see Fp8Args::early
     if (a.err && blockIdx.x == 0 && threadIdx.x == 0) *a.err = 0;
     const int sub = threadIdx.x & 15;
     const unsigned half = 0xffffu << (threadIdx.x & 16);
@@ -559,6 +559,7 @@ hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E,
     a.nsplit = L.up.n;  // 1 unless few
     a.kbper = L.up.per;
     a.err = qa.err;
+    a.early = 1;
     uint8_t* mq = ws + L.mq;
     float* ms = reinterpret_cast<float*>(ws + L.ms);
     if (L.few) {

@@ -75,6 +75,10 @@ struct Fp8Args {
     float* mid_s;
     int* err;               // error word: set when a bounded wait gives up
     int clear_err;          // the first kernel of a call clears it
+    // 1: the launch before this one is of the same call and lets this one start only
+    // after its own griddep_wait, so everything ahead of the call is done: offsets and
+    // weights can be read before this kernel's griddep_wait
+    int early;
 };
 hf_status launch_fp8_product(const Fp8Args& a, bool glu, cudaStream_t st);
 struct Fp8Split {

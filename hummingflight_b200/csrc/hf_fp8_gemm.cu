@@ -34,7 +34,6 @@
 namespace hf {
 namespace {
 
-
 using namespace sm100;
 
 constexpr int kThreads = 384;
@@ -215,7 +214,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_alloc(tmem_slot, C::kTmemCols);
         tmem_relinquish();
     }
-    griddep_wait();  // the rows, the offsets, the workspace's earlier users
+    // the rows, the offsets, the workspace's earlier users; early: the producer's first
+    // weights are on their way meanwhile, and each warp that needs the rest waits below
+    if (!a.early) griddep_wait();
     if (a.clear_err && blockIdx.x == 0 && threadIdx.x == 0) *a.err = 0;
     load_plan<BN>(a, MB, off, pref);
     tc_fence_before();
@@ -223,7 +224,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int total = pref[a.G] * (GLU ? 1 : a.nsplit);
-    griddep_launch_dependents();
     const auto wait = [&](uint64_t* bar, uint32_t parity) {
         return mbar_wait_for(smem_u32(bar), parity, abort_flag, kWaitNs);
     };
@@ -233,7 +233,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ------------------------------------------------------ TMA producer
             tma_prefetch_desc(&tmA);
             tma_prefetch_desc(&tmB);
-            uint32_t it = 0;
+            const auto bytes = [](const Tile& t) {
+                return 2 * kABytes + (t.n + C::kBoxB - 1) / C::kBoxB * C::kBoxB * 128;
+            };
+            const auto load_weights = [&](const Tile& t, uint32_t s, int kb) {
+                uint8_t* st = smem + s * C::kStageBytes;
+                mbar_arrive_expect_tx(&full[s], bytes(t));
+                tma_load_2d(st, &tmA, &full[s], kb * 128, t.a0);
+                tma_load_2d(st + kABytes, &tmA, &full[s], kb * 128, t.a1);
+            };
+            uint32_t it = 0, pre = 0;  // pre: stages whose weights are already requested
+            if (a.early && int(blockIdx.x) < total) {
+                Tile t;
+                decode<GLU, BN>(a, off, pref, KB, int(blockIdx.x), t);
+                pre = uint32_t(min(S, t.kb1 - t.kb0));
+                if (elect_one())
+                    for (uint32_t s = 0; s < pre; ++s) load_weights(t, s, t.kb0 + int(s));
+                __syncwarp();
+            }
+            griddep_wait();
+            griddep_launch_dependents();
             bool ok = true;
             for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
                 Tile t;
@@ -246,23 +265,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                         break;
                     }
                     if (elect_one()) {
-                        uint8_t* st = smem + s * C::kStageBytes;
-                        mbar_arrive_expect_tx(&full[s], 2 * kABytes + nb * C::kBoxB * 128);
-                        tma_load_2d(st, &tmA, &full[s], kb * 128, t.a0);
-                        tma_load_2d(st + kABytes, &tmA, &full[s], kb * 128, t.a1);
+                        if (it >= pre) load_weights(t, s, kb);
+                        uint8_t* st = smem + s * C::kStageBytes + 2 * kABytes;
                         for (int j = 0; j < nb; ++j)
-                            tma_load_2d(st + 2 * kABytes + j * C::kBoxB * 128, &tmB, &full[s],
-                                        kb * 128, t.row0 + j * C::kBoxB);
+                            tma_load_2d(st + j * C::kBoxB * 128, &tmB, &full[s], kb * 128,
+                                        t.row0 + j * C::kBoxB);
                     }
                     __syncwarp();
                 }
             }
             if (!ok) {  // every issued load lands before the CTA leaves
                 const uint32_t first = it > uint32_t(S) ? it - S : 0;
+                it = max(it, pre);
                 for (uint32_t i = first; i < it; ++i) drain_wait(&full[i % S], (i / S) & 1);
             }
         } else if (warp == 1) {
             // ------------------------------------------------------ MMA issuer
+            griddep_wait();  // so that its waits are timed from there
             uint32_t it = 0;
             bool ok = true;
             for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
@@ -296,6 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else if (warp == 2) {
             // ------------------------------------------------------ scales
             constexpr int PL = BN / 32;
+            griddep_wait();
             uint32_t it = 0;
             bool ok = true;
             for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
@@ -343,6 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int q = warp & 3, h = (warp - 4) >> 2;
         const int r = q * 32 + lane;
         const uint32_t lanes = tmem_base + (uint32_t(q * 32) << 16);
+        griddep_wait();
         uint32_t it = 0;
         bool ok = true;
         for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
@@ -450,22 +471,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int i = 0; i < CH; ++i)
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                            const int c = (2 * i + h) * 16 + j;
-                            if (i < nc && c < t.n) {
-                                const float y0 = g[i][j], y1 = v[i][j];
-                                const size_t o = size_t(t.out0 + c) * a.N + t.m0 + r;
-                                const bool r0 = t.m0 + r < a.N, r1 = t.m0 + 128 + r < a.N;
-                                if (a.out_f32) {
-                                    float* y = static_cast<float*>(a.out) + o;
-                                    if (r0) y[0] = y0;
-                                    if (r1) y[128] = y1;
-                                } else {
-                                    __nv_bfloat16* y = static_cast<__nv_bfloat16*>(a.out) + o;
-                                    if (r0) y[0] = __float2bfloat16_rn(y0);
-                                    if (r1) y[128] = __float2bfloat16_rn(y1);
-                                }
+                        const int c = (2 * i + h) * 16 + j;
+                        if (i < nc && c < t.n) {
+                            const float y0 = g[i][j], y1 = v[i][j];
+                            const size_t o = size_t(t.out0 + c) * a.N + t.m0 + r;
+                            const bool r0 = t.m0 + r < a.N, r1 = t.m0 + 128 + r < a.N;
+                            if (a.out_f32) {
+                                float* y = static_cast<float*>(a.out) + o;
+                                if (r0) y[0] = y0;
+                                if (r1) y[128] = y1;
+                            } else {
+                                __nv_bfloat16* y = static_cast<__nv_bfloat16*>(a.out) + o;
+                                if (r0) y[0] = __float2bfloat16_rn(y0);
+                                if (r1) y[128] = __float2bfloat16_rn(y1);
                             }
                         }
+                    }
             }
         }
     }
