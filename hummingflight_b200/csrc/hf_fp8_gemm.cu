@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         griddep_wait();
         uint32_t it = 0;
         bool ok = true;
-        for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
+        for (int u = blockIdx.x; u < total; u += gridDim.x) {
             Tile t;
             decode<GLU, BN>(a, off, pref, KB, u, t);
             // chunks of 16 columns at (2 i + h) * 16
@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < CH; ++i)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) g[i][j] = v[i][j] = 0.0f;
-            for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+            for (int kb = t.kb0; kb < t.kb1 && ok; ++kb, ++it) {
                 const uint32_t b = it % NB, sl = it % kScaleSlots;
                 if (!wait(&done[it % S], (it / S) & 1) ||
                     !wait(&sfull[sl], (it / kScaleSlots) & 1)) {
@@ -418,7 +418,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mbar_arrive(&sempty[sl]);
                 }
             }
-            if (!ok) break;
+            if (!ok) {
+                if (!GLU) break;
+                // the warps that gave up still meet the others at the barriers below,
+                // tile by tile, so that those get to their own bounded waits
+                named_bar_sync(1 + h, 128);
+                named_bar_sync(1 + h, 128);
+                continue;
+            }
             if constexpr (GLU) {
                 // silu(g) * u, and its maximum over the 128 rows per position
                 const bool rv = t.m0 + r < a.N;
@@ -826,7 +833,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         // ring positions: stage and its phase, buffer, scale slot and its phase
         uint32_t s = 0, ph = 0, b = 0, sl = 0, sph = 0;
         bool ok = true;
-        for (int u = first; u < total && ok; u += step) {
+        for (int u = first; u < total; u += step) {
             Tile t;
             decode<GLU, 256>(a, off, pref, KB, u, t);
             const int n = t.n - rank * 128;  // this CTA's positions
@@ -891,7 +898,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 sph ^= sl;
                 sl ^= 1;
             }
-            if (!ok) break;
+            if (!ok) {
+                if (!GLU) break;
+                named_bar_sync(1 + q, 64);  // the other half's warp may be there
+                named_bar_sync(1 + q, 64);
+                continue;
+            }
             const size_t row = size_t(t.row0 + rank * 128 + r);
             if constexpr (GLU) {
                 // silu(g) * u of this thread's 64 columns; the other 64 of the block are

@@ -88,6 +88,8 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
 
 // The same on a barrier's shared-memory address, with a limit of its own for
 // each wait: `limit` ns from the first slow poll, whatever the kernel's run time.
+// A whole warp calls it, and all lanes get the same answer: what follows is done
+// by the warp together, also when the wait gives up. (The vote costs no time.)
 __device__ __forceinline__ bool mbar_wait_for(uint32_t bar, uint32_t parity,
                                               volatile int* abort_flag, uint64_t limit) {
     uint32_t spins = 0;
@@ -101,12 +103,11 @@ __device__ __forceinline__ bool mbar_wait_for(uint32_t bar, uint32_t parity,
             : "=r"(ok)
             : "r"(bar), "r"(parity)
             : "memory");
-        if (ok) return true;
+        if (__all_sync(~0u, ok)) return true;
         if ((++spins & 255u) == 0) {
-            if (*abort_flag) return false;
             const uint64_t now = globaltimer();
             if (deadline == 0) deadline = now + limit;
-            else if (now > deadline) {
+            if (__any_sync(~0u, *abort_flag || now > deadline)) {
                 *abort_flag = 1;
                 return false;
             }
