@@ -418,8 +418,9 @@ extern "C" {
 
 hf_status hf_fp8_quantize(const void* x, hf_dtype x_dtype, long long ldx, int T, int K, uint8_t* q,
                           float* scales, hf_stream stream) {
-    if (T < 0 || K <= 0 || K % 16)
-        return fail(HF_ERR_ARG, "hf_fp8_quantize: T >= 0 and K a positive multiple of 16");
+    if (T < 0 || K <= 0 || K % 16 || std::max(T, K) > kMaxExtent)
+        return fail(HF_ERR_ARG, "hf_fp8_quantize: T >= 0 and K a positive multiple of 16, both at "
+                                "most 2^31 - 4096");
     if (bad_type(x_dtype)) return fail(HF_ERR_ARG, "hf_fp8_quantize: rows must be bf16 or f32");
     if (T == 0) return HF_OK;
     if (!x || !q || !scales) return fail(HF_ERR_ARG, "hf_fp8_quantize: null pointer");
@@ -441,7 +442,7 @@ hf_status hf_fp8_quantize(const void* x, hf_dtype x_dtype, long long ldx, int T,
 }
 
 size_t hf_fp8_gemm_workspace_size(int T, int N, int K) {
-    if (T <= 0 || N <= 0 || K <= 0) return 0;
+    if (T <= 0 || N <= 0 || K <= 0 || std::max({T, N, K}) > kMaxExtent) return 0;
     const Fp8Split sp = fp8_gemm_split(T, N, K);
     return kAlign + (sp.n > 1 ? up(size_t(sp.n) * T * N * sizeof(float)) : 0);
 }
@@ -449,8 +450,9 @@ size_t hf_fp8_gemm_workspace_size(int T, int N, int K) {
 hf_status hf_fp8_gemm(const uint8_t* xq, const float* sx, const uint8_t* wq, const float* sw, int T,
                       int N, int K, void* out, hf_dtype out_dtype, void* workspace,
                       size_t workspace_bytes, hf_stream stream) {
-    if (T < 0 || N <= 0 || K <= 0 || K % 16)
-        return fail(HF_ERR_ARG, "hf_fp8_gemm: T >= 0, N > 0 and K a positive multiple of 16");
+    if (T < 0 || N <= 0 || K <= 0 || K % 16 || std::max({T, N, K}) > kMaxExtent)
+        return fail(HF_ERR_ARG, "hf_fp8_gemm: T >= 0, N > 0 and K a positive multiple of 16, all "
+                                "at most 2^31 - 4096");
     if (bad_type(out_dtype)) return fail(HF_ERR_ARG, "hf_fp8_gemm: out must be bf16 or f32");
     if (T == 0) return HF_OK;
     if (!xq || !sx || !wq || !sw || !out || !workspace)
@@ -481,7 +483,9 @@ hf_status hf_fp8_gemm(const uint8_t* xq, const float* sx, const uint8_t* wq, con
 
 size_t hf_fp8_moe_experts_workspace_size(int T, int top_k, int E, int H, int I,
                                          hf_dtype out_dtype) {
-    if (T <= 0 || top_k <= 0 || E <= 0 || H <= 0 || I <= 0) return 0;
+    if (T <= 0 || top_k <= 0 || top_k > kMaxK || E <= 0 || E > kMaxExperts || H <= 0 || I <= 0 ||
+        (long long)T * top_k > kMaxExtent || 3ll * E * std::max(H, I) > kMaxExtent)
+        return 0;
     return experts_ws(T, top_k, E, H, I, out_dtype == HF_F32).total;
 }
 
@@ -494,11 +498,11 @@ hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E,
     if (E < 1 || E > kMaxExperts) return fail(HF_ERR_ARG, f + ": E must be in 1..1024");
     if (H <= 0 || I <= 0 || H % 16 || I % 16)
         return fail(HF_ERR_ARG, f + ": H and I must be positive multiples of 16");
-    if (3ll * E * std::max(H, I) > 0x7fffffffll)
-        return fail(HF_ERR_ARG, f + ": 3 * E * max(H, I) must be below 2^31");
+    if (3ll * E * std::max(H, I) > kMaxExtent)
+        return fail(HF_ERR_ARG, f + ": 3 * E * max(H, I) must be at most 2^31 - 4096");
     if (top_k < 1 || top_k > kMaxK) return fail(HF_ERR_ARG, f + ": top_k must be in 1..32");
-    if (T < 0 || (long long)T * top_k > 0x7fffffffll)
-        return fail(HF_ERR_ARG, f + ": T >= 0 and T * top_k below 2^31");
+    if (T < 0 || (long long)T * top_k > kMaxExtent)
+        return fail(HF_ERR_ARG, f + ": T >= 0 and T * top_k at most 2^31 - 4096");
     if (bad_type(x_dtype) || bad_type(out_dtype))
         return fail(HF_ERR_ARG, f + ": x and out must be bf16 or f32");
     if (T == 0) return HF_OK;

@@ -32,6 +32,7 @@ inline cudaStream_t as_cuda(hf_stream s) { return reinterpret_cast<cudaStream_t>
 
 // ------------------------------------------------------------------ limits
 constexpr int kMaxTopK = 8;        // TopKResult holds 8 (compute/moe_router.h:12-16)
+constexpr int kMaxExtent = 0x7fffffff - 4095;  // rows or columns that can be rounded up to tiles in 32 bits
 constexpr int kMaxExperts = 1024;  // top-k kernel keeps E/32 scores per lane
 constexpr int kSmallRouteT = 128;  // single-CTA routing up to this many tokens
 constexpr int kGemvTE = 4;         // tokens per grouped-GEMV chunk

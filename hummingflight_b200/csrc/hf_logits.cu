@@ -730,7 +730,7 @@ using namespace hf;
 extern "C" {
 
 size_t hf_route_workspace_size(int T, const hf_route_spec* spec) {
-    if (T <= 0 || check_spec(spec, "hf_route_workspace_size") != HF_OK) return 0;
+    if (T <= 0 || T > kMaxExtent || check_spec(spec, "hf_route_workspace_size") != HF_OK) return 0;
     return ws_bytes(T, spec->num_experts);
 }
 
@@ -740,8 +740,8 @@ hf_status hf_route_logits(const void* logits, hf_dtype dtype, const float* bias,
     HF_TRY(check_spec(spec, "hf_route_logits"));
     if (dtype != HF_BF16 && dtype != HF_F32)
         return fail(HF_ERR_ARG, "hf_route_logits: logits must be bf16 or f32");
-    if (T < 0 || (long long)T * spec->top_k > 0x7fffffffll)
-        return fail(HF_ERR_ARG, "hf_route_logits: T >= 0 and T * top_k below 2^31");
+    if (T < 0 || (long long)T * spec->top_k > kMaxExtent)
+        return fail(HF_ERR_ARG, "hf_route_logits: T >= 0 and T * top_k at most 2^31 - 4096");
     if (!r || !r->counts || !r->offsets || (T && (!logits || !r->topk_ids || !r->topk_weights || !r->perm)))
         return fail(HF_ERR_ARG, "hf_route_logits: null pointer");
     if (r->margins || r->slot_out)

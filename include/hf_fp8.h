@@ -32,7 +32,7 @@ extern "C" {
  * (scale and values): it is never saturated.
  * x: device [T x K] BF16 or fp32, rows ldx elements apart, 16-byte aligned
  * (pointer and pitch); q: device [T x K]; scales: device fp32 [T x ceil(K/128)].
- * K a multiple of 16. */
+ * K a multiple of 16; T, K (and N below) at most 2^31 - 4096. */
 HF_API hf_status hf_fp8_quantize(const void* x, hf_dtype x_dtype, long long ldx, int T, int K,
                                  uint8_t* q, float* scales, hf_stream stream);
 
@@ -66,10 +66,11 @@ HF_API hf_status hf_fp8_gemm(const uint8_t* xq, const float* sx, const uint8_t* 
  * the routed ones is left out; topk_ids is not read); offsets, perm entries out
  * of range are skipped. resid: device [T x H] of out_dtype or NULL, may be out
  * itself. out: device [T x H] of out_dtype; the expert outputs y_i are kept in
- * the same type until the combine (bf16 outputs: y_i rounded once more). The shared expert, or a dense MLP, is the call
- * with E = 1, k = 1 and the routed output as resid. H and I multiples of 16,
- * k in 1..32, E in 1..1024, T * k and 3 * E * max(H, I) below 2^31; pointers 16-byte aligned, the
- * workspace 256-byte. A workspace serves any number of layers in stream order. */
+ * the same type until the combine (bf16 outputs: y_i rounded once more). The
+ * shared expert, or a dense MLP, is the call with E = 1, k = 1 and the routed
+ * output as resid. H and I multiples of 16, k in 1..32, E in 1..1024, T * k and
+ * 3 * E * max(H, I) at most 2^31 - 4096; pointers 16-byte aligned, the workspace
+ * 256-byte. A workspace serves any number of layers in stream order. */
 HF_API size_t hf_fp8_moe_experts_workspace_size(int T, int top_k, int E, int H, int I,
                                                 hf_dtype out_dtype);
 HF_API hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E, int H,

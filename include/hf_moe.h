@@ -337,7 +337,7 @@ HF_API size_t hf_route_workspace_size(int T, const hf_route_spec* spec);
 /* logits: device [T x E] fp32 or BF16; bias: device fp32 [E] or NULL. Writes
  * routing->topk_ids [T x k], topk_weights [T x k], counts [E+1], offsets [E+2]
  * and perm [T*k] (the shared group E is empty); all five are required, margins
- * and slot_out must be NULL. T = 0 writes zero counts and offsets. workspace:
+ * and slot_out must be NULL. T * k at most 2^31 - 4096; T = 0 writes zero counts and offsets. workspace:
  * device scratch of hf_route_workspace_size bytes (0 and NULL up to 16 tokens),
  * 256-byte aligned, used in stream order only. Asynchronous on `stream`. */
 HF_API hf_status hf_route_logits(const void* logits, hf_dtype dtype, const float* bias, int T,

@@ -183,3 +183,23 @@ def test_calls_run_on_the_device_of_their_tensors(monkeypatch):
     with moe.on_device(torch.device("cuda", 0)) as s:
         assert s == 100
     assert log == [1, 0, 2, 0]
+
+
+def test_sizes_next_to_2_31_are_refused():
+    """Rounded up to tiles, these would pass 32 bits."""
+    L = _lib.lib()
+    big, ws = 0x7fffffff - 15, 1 << 62
+    r = _lib.HfMoeRouting(P, P, None, P, P, P, None)
+    assert L.hf_route_logits(P, 1, None, big, spec(num_experts=1, top_k=1), r, WS, ws,
+                             None) == _lib.HF_ERR_ARG
+    assert L.hf_route_workspace_size(big, spec(num_experts=1, top_k=1)) == 0
+    assert L.hf_fp8_quantize(P, 0, big, 1, big, P, P, None) == _lib.HF_ERR_ARG
+    assert L.hf_fp8_quantize(P, 0, 16, big, 16, P, P, None) == _lib.HF_ERR_ARG
+    for T, N, K in ((big, 16, 16), (16, big, 16), (16, 16, big)):
+        assert L.hf_fp8_gemm_workspace_size(T, N, K) == 0
+        assert L.hf_fp8_gemm(P, P, P, P, T, N, K, P, 0, WS, ws, None) == _lib.HF_ERR_ARG
+    for T, k, E, H, I in ((big, 1, 1, 16, 16), (big // 4, 4, 1, 16, 16), (1, 1, 1, 715827872, 16),
+                          (1, 1, 1, 16, 715827872)):
+        assert L.hf_fp8_moe_experts_workspace_size(T, k, E, H, I, 0) == 0
+        assert L.hf_fp8_moe_experts(P, P, E, H, I, P, 0, H, T, k, r, None, P, 0, WS, ws,
+                                    None) == _lib.HF_ERR_ARG
