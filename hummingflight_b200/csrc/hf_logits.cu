@@ -374,7 +374,8 @@ __device__ __forceinline__ int route_token(const LogitArgs& a, const float (&bia
             for (int j = 0; j < NPL; ++j)
                 s[j] = __fdividef(1.0f, 1.0f + __expf(-l[j])) + bias[j];
             tol = __fdividef(1.0f, 1.0f + __expf(-top)) *
-                  (0x1p-20f + fmaxf(-top, 0.0f) * 0x1p-21f);
+                      (0x1p-20f + fmaxf(-top, 0.0f) * 0x1p-21f) +
+                  0x1p-120f;  // quotients below 2^-126 come out as 0
         }
         uint32_t key[NPL];
 #pragma unroll

@@ -136,6 +136,19 @@ def test_masked_and_non_finite_logits(score, biased, groups):
         check(l.cuda(), b.cuda(), 8, score, *groups, 1.0, True)
 
 
+def test_scores_near_the_smallest_numbers_rank_as_in_64_bits():
+    """Biases of the size of the scores, 1e-39 and below: a quotient flushed to 0
+    must not count as exact."""
+    need_gpu()
+    l = torch.full((20, 8), -100.0)
+    l[:, 3], l[:, 6] = -88.0, -95.0
+    b = torch.zeros(8)
+    b[3], b[6] = 1e-39, 3e-39
+    check(l.cuda(), b.cuda(), 1, "sigmoid", 1, 1, 2, 1.0, False)
+    check(l.cuda(), b.cuda(), 4, "sigmoid", 1, 1, 2, 1.0, False)
+    check(l.cuda(), b.cuda(), 2, "sigmoid", 4, 2, 2, 1.0, False)
+
+
 def test_nan_logits():
     """A NaN key ranks below every number; a softmax row with one has NaN weights."""
     need_gpu()
