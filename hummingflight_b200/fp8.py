@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from ._lib import HF_BF16, HF_F32, HfError, HfMoeRouting, call
-from .moe import _ACT, _ptr, _stream, check_tensor, on_device, scratch
+from .moe import _ACT, check_tensor, new_tensor, on_device, scratch
 
 BLOCK = 128
 _Q = (torch.float8_e4m3fn, torch.uint8)
@@ -40,11 +40,11 @@ def quantize(x, q=None, scales=None, stream=None):
     check_tensor("x", x, _X, (T, K), rows=True)
     dev = x.device
     if q is None:
-        q = torch.empty((T, K), dtype=torch.float8_e4m3fn, device=dev)
+        q = new_tensor((T, K), torch.float8_e4m3fn, dev, stream)
     else:
         check_tensor("q", q, _Q, (T, K), dev)
     if scales is None:
-        scales = torch.empty((T, blocks(K)), dtype=torch.float32, device=dev)
+        scales = new_tensor((T, blocks(K)), torch.float32, dev, stream)
     else:
         check_tensor("scales", scales, _F32, (T, blocks(K)), dev)
     with on_device(dev, stream) as s:
@@ -77,15 +77,16 @@ def gemm(xq, sx, wq, sw, out=None, out_dtype: str = "bf16", workspace=None, stre
     check_tensor("wq", wq, _Q, (N, K), dev)
     check_tensor("sw", sw, _F32, (blocks(N), blocks(K)), dev)
     if out is None:
-        out = torch.empty((T, N), dtype=torch.float32 if out_dtype == "f32" else torch.bfloat16,
-                          device=dev)
+        out = new_tensor((T, N), torch.float32 if out_dtype == "f32" else torch.bfloat16, dev,
+                         stream)
     else:
         check_tensor("out", out, _X, (T, N), dev)
     with on_device(dev, stream) as s:
         need = gemm_workspace_size(T, N, K)
-        workspace = scratch(workspace, need, dev)
+        workspace = scratch(workspace, need, dev, stream)
         call("hf_fp8_gemm", xq.data_ptr(), sx.data_ptr(), wq.data_ptr(), sw.data_ptr(), T, N, K,
-             out.data_ptr(), _code(out.dtype), None if workspace is None else workspace.data_ptr(), need, s)
+             out.data_ptr(), _code(out.dtype),
+             None if workspace is None else workspace.data_ptr(), need, s)
     return out
 
 
@@ -123,8 +124,8 @@ def moe_experts(x, experts, scales, routing: dict, resid=None, out=None, out_dty
         raise ValueError(f"offsets, perm: {offsets.numel()} and {perm.numel()} entries, {E + 1} "
                          f"and {T * k} are needed")
     if out is None:
-        out = torch.empty((T, H), dtype=torch.float32 if out_dtype == "f32" else torch.bfloat16,
-                          device=dev)
+        out = new_tensor((T, H), torch.float32 if out_dtype == "f32" else torch.bfloat16, dev,
+                         stream)
     else:
         check_tensor("out", out, _X, (T, H), dev)
     if resid is not None:
@@ -133,7 +134,7 @@ def moe_experts(x, experts, scales, routing: dict, resid=None, out=None, out_dty
     code = _code(out.dtype)
     with on_device(dev, stream) as s:
         need = moe_experts_workspace_size(T, k, E, H, I, "f32" if code == HF_F32 else "bf16")
-        workspace = scratch(workspace, need, dev)
+        workspace = scratch(workspace, need, dev, stream)
         call("hf_fp8_moe_experts", experts.data_ptr(), scales.data_ptr(), E, H, I, x.data_ptr(),
              _code(x.dtype), _pitch(x), T, k, r,
              None if resid is None else resid.data_ptr(), out.data_ptr(), code,
@@ -143,8 +144,10 @@ def moe_experts(x, experts, scales, routing: dict, resid=None, out=None, out_dty
 
 def status(workspace, stream=None):
     """Waits for the stream; raises HfError (HF_ERR_TIMEOUT) if the last product
-    on this workspace hit a bounded-wait timeout."""
-    call("hf_fp8_status", _ptr(workspace), _stream(stream))
+    on this workspace hit a bounded-wait timeout. The stream: that of the product,
+    by default the current one of the workspace's device."""
+    with on_device(workspace.device, stream) as s:
+        call("hf_fp8_status", workspace.data_ptr(), s)
 
 
 __all__ = ["BLOCK", "blocks", "quantize", "gemm", "gemm_workspace_size", "moe_experts",

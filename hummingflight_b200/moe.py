@@ -127,11 +127,21 @@ class on_device:
             _set_device(self._back)
 
 
-def scratch(workspace, need: int, device):
+def new_tensor(shape, dtype, device, stream=None):
+    """Uninitialised memory for a call on `stream` (the current one unless given). It
+    belongs to that stream: freed, it goes to later work of that stream only."""
+    torch = _torch()
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def scratch(workspace, need: int, device, stream=None):
     """`workspace` if it has `need` bytes on the device, a new one if none is given."""
     torch = _torch()
     if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        return new_tensor(need, torch.uint8, device, stream) if need else None
     check_tensor("workspace", workspace, (torch.uint8,), workspace.shape, device)
     if workspace.numel() < need:
         raise ValueError(f"workspace: {workspace.numel()} bytes, {need} are needed")
@@ -430,11 +440,11 @@ def route_logits(logits, bias=None, top_k: int = 8, score: str = "sigmoid", n_gr
     spec = _route_spec(E, top_k, score, n_group, topk_group, group_top, routed_scaling_factor,
                        bool(norm_topk_prob))
     if out is None:
-        out = dict(topk_ids=torch.empty((T, top_k), dtype=torch.int32, device=dev),
-                   topk_weights=torch.empty((T, top_k), dtype=torch.float32, device=dev),
-                   counts=torch.empty(E + 1, dtype=torch.int32, device=dev),
-                   offsets=torch.empty(E + 2, dtype=torch.int32, device=dev),
-                   perm=torch.empty(T * top_k, dtype=torch.int32, device=dev))
+        out = dict(topk_ids=new_tensor((T, top_k), torch.int32, dev, stream),
+                   topk_weights=new_tensor((T, top_k), torch.float32, dev, stream),
+                   counts=new_tensor(E + 1, torch.int32, dev, stream),
+                   offsets=new_tensor(E + 2, torch.int32, dev, stream),
+                   perm=new_tensor(T * top_k, torch.int32, dev, stream))
     ids, w, counts, offsets, perm = (out["topk_ids"], out["topk_weights"], out["counts"],
                                      out["offsets"], out["perm"])
     check_tensor("topk_ids", ids, i32, (T, top_k), dev)
@@ -446,7 +456,7 @@ def route_logits(logits, bias=None, top_k: int = 8, score: str = "sigmoid", n_gr
                      perm.data_ptr(), None)
     with on_device(dev, stream) as s:
         need = route_workspace_size(T, E, top_k)
-        workspace = scratch(workspace, need, dev) if need else None
+        workspace = scratch(workspace, need, dev, stream) if need else None
         call("hf_route_logits", logits.data_ptr(),
              HF_F32 if logits.dtype == torch.float32 else HF_BF16,
              None if bias is None else bias.data_ptr(), T, spec, r,

@@ -203,3 +203,21 @@ def test_sizes_next_to_2_31_are_refused():
         assert L.hf_fp8_moe_experts_workspace_size(T, k, E, H, I, 0) == 0
         assert L.hf_fp8_moe_experts(P, P, E, H, I, P, 0, H, T, k, r, None, P, 0, WS, ws,
                                     None) == _lib.HF_ERR_ARG
+
+
+def test_status_asks_the_device_of_the_workspace(monkeypatch):
+    from hummingflight_b200 import fp8, moe
+    cur, seen = [0], []
+
+    class Workspace:
+        device = torch.device("cuda", 1)
+
+        def data_ptr(self):
+            return P
+
+    monkeypatch.setattr(moe, "_get_device", lambda: cur[0])
+    monkeypatch.setattr(moe, "_set_device", lambda d: cur.__setitem__(0, d))
+    monkeypatch.setattr(moe, "_raw_stream", lambda i: 100 + i)
+    monkeypatch.setattr(fp8, "call", lambda *a: seen.append((cur[0], *a)))
+    fp8.status(Workspace())
+    assert seen == [(1, "hf_fp8_status", P, 101)] and cur[0] == 0

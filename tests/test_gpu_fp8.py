@@ -361,6 +361,34 @@ def test_experts_bad_permutation_stays_in_bounds():
         fp8.status(ws)
 
 
+def test_memory_of_a_call_on_another_stream(monkeypatch):
+    """What a call allocates belongs to the stream that it runs on: the next tensor
+    of the current stream is not given the workspace of a call still running there."""
+    need_gpu()
+    from hummingflight_b200 import fp8, moe
+    T, N, K = 8, 512, 4096
+    need = fp8.gemm_workspace_size(T, N, K)
+    assert need > 1 << 16  # runs of K
+    xq, sx = fp8.quantize(torch.randn((T, K), device="cuda"))
+    wq = torch.randn((N, K), device="cuda").to(torch.float8_e4m3fn)
+    sw = torch.ones((fp8.blocks(N), fp8.blocks(K)), device="cuda")
+    made = []
+
+    def scratch(*args):
+        ws = moe.scratch(*args)
+        made.append(ws.data_ptr())
+        return ws
+
+    monkeypatch.setattr(fp8, "scratch", scratch)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    y = fp8.gemm(xq, sx, wq, sw, stream=side)
+    here = [torch.empty(need, dtype=torch.uint8, device="cuda") for _ in range(4)]
+    assert made and not set(made) & {t.data_ptr() for t in here}
+    side.synchronize()
+    assert torch.equal(y, fp8.gemm(xq, sx, wq, sw))
+
+
 def test_two_streams_at_once():
     """Independent calls that overlap on two streams, each with its own workspace."""
     need_gpu()
