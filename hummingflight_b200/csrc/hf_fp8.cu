@@ -281,6 +281,7 @@ __global__ void __launch_bounds__(256) k_fp8_combine(const void* y, int n, const
     constexpr int V = Y32 ? 4 : 8, kBatch = 8;
     const int t = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * V;
     griddep_wait();
+    griddep_launch_dependents();
     if (c >= H) return;
     const unsigned rows = unsigned(T) * unsigned(k);
     float acc[V] = {};

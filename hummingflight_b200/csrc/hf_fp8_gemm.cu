@@ -1045,6 +1045,7 @@ Fp8Split fp8_gemm_split(int T, int N, int K) {
 __global__ void __launch_bounds__(256) k_sum_planes(const float* planes, int n, long long count,
                                                     void* out, int out_f32) {
     griddep_wait();
+    griddep_launch_dependents();  // the next launch sets itself up meanwhile
     const long long quads = count / 4, rest = count - quads * 4;
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i < quads) {
