@@ -214,6 +214,7 @@ hf_status launch_quantize(const QuantArgs& a, bool f32, int dev, cudaStream_t st
     }
     const long long blocks = (long long)a.rows * a.nb;
     const long long most = num_sms(dev) * 8ll;
+    // one array of blocks, or rows: 16384 x 6144 bf16 56 and 71 us, 1024 x 6144 4.4 and 5.6
     if (!a.perm && a.ldx == a.K && a.K % kFp8Block == 0) {
         const int grid = int(std::min((blocks + 15) / 16, most));
         if (f32) k_quantize_flat<true><<<grid, 256, 0, st>>>(a.x, blocks, a.q, a.s);
@@ -363,8 +364,9 @@ hf_status launch_fp8_combine(const void* y, int n, const int32_t* pos, const flo
 
 // ------------------------------------------------------------------ workspaces
 // Runs of K of the experts' products: few positions make few tiles (at most one
-// per position and row block of the weights); beyond this number the tiles fill
-// the GPU.
+// per position and row block of the weights). H = 6144, I = 2048, us without runs and
+// with: 128 positions of 2 experts 68 and 42, 512 of 2: 73 and 72, 512 of 256: 1206
+// and 1200; beyond, the tiles fill the GPU and the planes only cost memory.
 constexpr int kFewPositions = 512;
 
 struct ExpertsWs {
@@ -380,9 +382,9 @@ ExpertsWs experts_ws(int T, int k, int E, int H, int I, bool f32) {
     w.down = Fp8Split{1, blocks128(I)};
     if (n <= kFewPositions) {
         const long long active = std::min<long long>(n, E);
-        w.down = fp8_split(active * ((H + 255) / 256), false, I, 4.0 * n * H);
+        w.down = fp8_split(active * ((H + 255) / 256), 32, I, 4.0 * n * H);
         if (I % kFp8Block == 0) {  // gate and up rows then have one run of scale blocks
-            w.up = fp8_split(active * (I / 128), false, H, 8.0 * n * I);
+            w.up = fp8_split(active * (I / 128), 32, H, 8.0 * n * I);
             w.few = w.up.n > 1;
         }
     }

@@ -84,7 +84,8 @@ hf_status launch_fp8_product(const Fp8Args& a, bool glu, cudaStream_t st);
 struct Fp8Split {
     int n, per;  // runs, blocks of K in each
 };
-Fp8Split fp8_split(long long tiles, bool pair, int K, double plane_bytes);
+// tiles: of bn positions (32, 64, or 256 for CTA pairs); plane_bytes: of one run
+Fp8Split fp8_split(long long tiles, int bn, int K, double plane_bytes);
 // One group, with its runs of K chosen by size; planes: fp32 [n x T x N] when n > 1.
 Fp8Split fp8_gemm_split(int T, int N, int K);
 hf_status launch_fp8_gemm(const Fp8Args& a, float* planes, cudaStream_t st);

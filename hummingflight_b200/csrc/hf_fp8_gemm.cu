@@ -159,8 +159,8 @@ __device__ __forceinline__ bool drain_wait(uint64_t* bar, uint32_t parity) {
 }
 
 // Four accumulators += sums times scales. (Packed pairs, fma.rn.f32x2, run at the
-// same rate and cost moves to pair the registers: 324 us against 297 on 4096 x
-// 12288 x 6144.)
+// same rate and cost moves to pair the registers: in the pair kernel 324 us against
+// 297 on 4096 x 12288 x 6144.)
 __device__ __forceinline__ void add4(float* acc, const uint32_t* d, float4 s) {
     acc[0] = fmaf(__uint_as_float(d[0]), s.x, acc[0]);
     acc[1] = fmaf(__uint_as_float(d[1]), s.y, acc[1]);
@@ -593,16 +593,23 @@ __device__ __forceinline__ void store32(const Fp8Args& a, long long row, int n, 
 // its position's times that of either weight block. Warp 2 writes these products
 // to a ring in shared memory, eight blocks of K at a time.
 //
+// 4096 x 12288 x 6144: 290 us in a burst (2.1 PFLOP/s; the same product with whole-
+// tensor scales, from the library, runs at 2.6 to 3.0), 338 in a long stream, under
+// the power cap. In a burst a block of K takes about twice the 515 clocks of its
+// MMAs (the chain below); on short K the output rows count (K = 2048: 119 us, 96
+// without them).
+//
 // The MMA's N is cut in two halves of 128 (64 rows of either weight block: that
 // is what N = 128 takes from each CTA's shared memory). Each half has two
 // buffers, an issuing warp and four accumulation warps (64 columns of both weight
 // blocks a thread) of its own. The chain MMA -> commit -> read-back -> release ->
 // MMA of one buffer costs about 1000 clocks, half of them barrier latencies (a
-// commit 200, a cluster arrive 120, a wait 50 each), against 515 for a block's
-// MMAs; two independent halves overlap their chains.
+// commit 200, a cluster arrive 120, a wait 50 each); two independent halves overlap
+// their chains.
 //
 // Warps: 0 TMA producer, 1 and 3 MMA issuers of the halves (leader CTA; 1 owns
-// TMEM), 2 scales, 4-11 accumulation with the registers that the first four give up: 4 * 32 * 56 + 8 * 32 * 224 of the launch's 384 * 168
+// TMEM), 2 scales, 4-11 accumulation, with the registers that the first four give
+// up: 4 * 32 * 56 + 8 * 32 * 224 of the launch's 384 * 168.
 constexpr int kPairThreads = 384;
 constexpr int kPairWarps = 8;
 constexpr int kPairStages = 6;
@@ -765,7 +772,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             }
         } else if (warp == 2) {
             // ------------------------------------------------------ scales
-            const bool vec = KB % 4 == 0 && (GLU || a.kbper % 4 == 0) && (reinterpret_cast<uintptr_t>(a.sx) & 15) == 0;
+            const bool vec = KB % 4 == 0 && (GLU || a.kbper % 4 == 0) &&
+                             (reinterpret_cast<uintptr_t>(a.sx) & 15) == 0;
             uint32_t is = 0;
             bool ok = true;
             for (int u = first; u < total && ok; u += step) {
@@ -1013,21 +1021,28 @@ hf_status launch_one(const Fp8Args& a, cudaStream_t st) {
 
 // The runs of K of a product: with few tiles for the GPU's places (148 CTAs, or
 // 74 pairs), each tile's blocks of K are dealt to several CTAs that write fp32
-// planes, which the next launch adds in order. The number that minimises
-// rounds x (blocks + 0.5 for the tile's end) + the planes' traffic; a block takes
-// about 0.7 us where the weights stream from memory.
-Fp8Split fp8_split(long long tiles, bool pair, int K, double plane_bytes) {
+// planes, which the next launch adds in order. The number with the least modelled
+// time, in us: rounds x (blocks x their time + 0.35 for a tile's end), and for the
+// planes 3 (a launch) + 0.1 each + their bytes, written and read once. A block takes
+// 0.7 where the weights stream from memory to every place; where some are idle less,
+// down to what one CTA can load (tiles of 32 positions 0.45, of 64 0.55; a pair's
+// MMAs take 0.7). Measured, cold, one run / the chosen number: 64 x 6144 x 12288
+// 65.6 / 31, 1 x 2048 x 6144 26.7 / 14.4, 64 x 24576 x 1536 20.5 (two runs: 28.7),
+// 128 x 6144 x 12288 (pairs) 55 / 35, 512 x 6144 x 6144 34.8 (two runs: 45).
+Fp8Split fp8_split(long long tiles, int bn, int K, double plane_bytes) {
     const int KB = (K + kFp8Block - 1) / kFp8Block;
+    const bool pair = bn == 256;
     const int slots = pair ? 74 : 148, mult = pair ? 4 : 1;
+    const double least_block = pair ? 0.7 : bn == 64 ? 0.55 : 0.45;
+    const double plane_us = plane_bytes * 2.0 / (pair ? 5e6 : 2.5e6);  // TB/s: 5, by columns 2.5
     Fp8Split best{1, KB};
     double least = 1e30;
     for (int n = 1; n <= 16 && n <= KB; ++n) {
         const int per = ((KB + n - 1) / n + mult - 1) / mult * mult;
         if ((KB + per - 1) / per != n) continue;  // no empty run
-        const double rounds = double((tiles * n + slots - 1) / slots);
-        // written and read once at about 5 TB/s, and a launch
-        const double sum = n == 1 ? 0.0 : (2.0 + n * plane_bytes * 2.0 / 5e6) / 0.7;
-        const double cost = rounds * (per + 0.5) + sum;
+        const long long rounds = tiles * n / slots, rest = tiles * n % slots;
+        double cost = rounds * (per * 0.7 + 0.35) + (n == 1 ? 0.0 : 3.0 + n * (0.1 + plane_us));
+        if (rest) cost += per * std::max(least_block, 0.7 * rest / slots) + 0.35;
         if (cost < least) {
             least = cost;
             best = Fp8Split{n, per};
@@ -1036,10 +1051,12 @@ Fp8Split fp8_split(long long tiles, bool pair, int K, double plane_bytes) {
     return best;
 }
 
+// Positions of a tile, by the mean per segment (256: the pair kernel's).
+static int tile_rows(int mean) { return mean > kNarrowRows ? 256 : mean > kNarrow32 ? 64 : 32; }
+
 Fp8Split fp8_gemm_split(int T, int N, int K) {
-    const bool pair = T > kNarrowRows;
-    const int bn = pair ? 256 : T > kNarrow32 ? 64 : 32;
-    return fp8_split((long long)((N + 255) / 256) * ((T + bn - 1) / bn), pair, K, 4.0 * T * N);
+    const int bn = tile_rows(T);
+    return fp8_split((long long)((N + 255) / 256) * ((T + bn - 1) / bn), bn, K, 4.0 * T * N);
 }
 
 __global__ void __launch_bounds__(256) k_sum_planes(const float* planes, int n, long long count,
@@ -1108,9 +1125,9 @@ hf_status launch_fp8_gemm(const Fp8Args& args, float* planes, cudaStream_t st) {
 }
 
 hf_status launch_fp8_product(const Fp8Args& a, bool glu, cudaStream_t st) {
-    const int avg = (a.rows + a.G - 1) / a.G;
-    if (avg > kNarrowRows) return glu ? launch_pair<true>(a, st) : launch_pair<false>(a, st);
-    if (avg > kNarrow32) return glu ? launch_one<true, 64>(a, st) : launch_one<false, 64>(a, st);
+    const int bn = tile_rows((a.rows + a.G - 1) / a.G);
+    if (bn == 256) return glu ? launch_pair<true>(a, st) : launch_pair<false>(a, st);
+    if (bn == 64) return glu ? launch_one<true, 64>(a, st) : launch_one<false, 64>(a, st);
     return glu ? launch_one<true, 32>(a, st) : launch_one<false, 32>(a, st);
 }
 
