@@ -381,10 +381,11 @@ ExpertsWs experts_ws(int T, int k, int E, int H, int I, bool f32) {
     w.up = Fp8Split{1, blocks128(H)};
     w.down = Fp8Split{1, blocks128(I)};
     if (n <= kFewPositions) {
-        const long long active = std::min<long long>(n, E);
-        w.down = fp8_split(active * ((H + 255) / 256), 32, I, 4.0 * n * H);
+        const int mean = int((n + E - 1) / E), bn = fp8_tile_rows(mean);
+        const long long active = std::min<long long>(n, E) * ((mean + bn - 1) / bn);
+        w.down = fp8_split(active * ((H + 255) / 256), bn, I, 4.0 * n * H);
         if (I % kFp8Block == 0) {  // gate and up rows then have one run of scale blocks
-            w.up = fp8_split(active * (I / 128), 32, H, 8.0 * n * I);
+            w.up = fp8_split(active * (I / 128), bn, H, 8.0 * n * I);
             w.few = w.up.n > 1;
         }
     }

@@ -81,6 +81,8 @@ struct Fp8Args {
     int early;
 };
 hf_status launch_fp8_product(const Fp8Args& a, bool glu, cudaStream_t st);
+// Positions of a tile, by the mean per segment (256: the pair kernel's).
+int fp8_tile_rows(int mean);
 struct Fp8Split {
     int n, per;  // runs, blocks of K in each
 };

@@ -1051,11 +1051,10 @@ Fp8Split fp8_split(long long tiles, int bn, int K, double plane_bytes) {
     return best;
 }
 
-// Positions of a tile, by the mean per segment (256: the pair kernel's).
-static int tile_rows(int mean) { return mean > kNarrowRows ? 256 : mean > kNarrow32 ? 64 : 32; }
+int fp8_tile_rows(int mean) { return mean > kNarrowRows ? 256 : mean > kNarrow32 ? 64 : 32; }
 
 Fp8Split fp8_gemm_split(int T, int N, int K) {
-    const int bn = tile_rows(T);
+    const int bn = fp8_tile_rows(T);
     return fp8_split((long long)((N + 255) / 256) * ((T + bn - 1) / bn), bn, K, 4.0 * T * N);
 }
 
@@ -1125,7 +1124,7 @@ hf_status launch_fp8_gemm(const Fp8Args& args, float* planes, cudaStream_t st) {
 }
 
 hf_status launch_fp8_product(const Fp8Args& a, bool glu, cudaStream_t st) {
-    const int bn = tile_rows((a.rows + a.G - 1) / a.G);
+    const int bn = fp8_tile_rows((a.rows + a.G - 1) / a.G);
     if (bn == 256) return glu ? launch_pair<true>(a, st) : launch_pair<false>(a, st);
     if (bn == 64) return glu ? launch_one<true, 64>(a, st) : launch_one<false, 64>(a, st);
     return glu ? launch_one<true, 32>(a, st) : launch_one<false, 32>(a, st);
