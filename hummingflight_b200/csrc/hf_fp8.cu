@@ -365,8 +365,8 @@ hf_status launch_fp8_combine(const void* y, int n, const int32_t* pos, const flo
 // ------------------------------------------------------------------ workspaces
 // Runs of K of the experts' products: few positions make few tiles (at most one
 // per position and row block of the weights). H = 6144, I = 2048, us without runs and
-// with: 128 positions of 2 experts 68 and 42, 512 of 2: 73 and 72, 512 of 256: 1206
-// and 1200; beyond, the tiles fill the GPU and the planes only cost memory.
+// with: 128 positions of 2 experts 68 and 39, 500 of 1: 57 and 50, 1000 of 1: 75 and
+// 82; the planes' bytes grow with the positions and the tiles fill the GPU by then.
 constexpr int kFewPositions = 512;
 
 struct ExpertsWs {
