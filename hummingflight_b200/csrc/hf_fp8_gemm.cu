@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < CH; ++i)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) g[i][j] = v[i][j] = 0.0f;
-            for (int kb = t.kb0; kb < t.kb1 && ok; ++kb, ++it) {
+            for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
                 const uint32_t b = it % NB, sl = it % kScaleSlots;
                 if (!wait(&done[it % S], (it / S) & 1) ||
                     !wait(&sfull[sl], (it / kScaleSlots) & 1)) {
@@ -419,12 +419,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             if (!ok) {
-                if (!GLU) break;
-                // the warps that gave up still meet the others at the barriers below,
-                // tile by tile, so that those get to their own bounded waits
-                named_bar_sync(1 + h, 128);
-                named_bar_sync(1 + h, 128);
-                continue;
+                // the half's other warps may wait at the barriers below: meet them there
+                // for this tile and the rest, so that they get to their own bounded waits
+                if (GLU)
+                    for (; u < total; u += gridDim.x) {
+                        named_bar_sync(1 + h, 128);
+                        named_bar_sync(1 + h, 128);
+                    }
+                break;
             }
             if constexpr (GLU) {
                 // silu(g) * u, and its maximum over the 128 rows per position
@@ -907,10 +909,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 sl ^= 1;
             }
             if (!ok) {
-                if (!GLU) break;
-                named_bar_sync(1 + q, 64);  // the other half's warp may be there
-                named_bar_sync(1 + q, 64);
-                continue;
+                // the other half's warp may wait at the barriers below: meet it there
+                // for this tile and the rest, so that it gets to its own bounded waits
+                if (GLU)
+                    for (; u < total; u += step) {
+                        named_bar_sync(1 + q, 64);
+                        named_bar_sync(1 + q, 64);
+                    }
+                break;
             }
             const size_t row = size_t(t.row0 + rank * 128 + r);
             if constexpr (GLU) {
@@ -930,21 +936,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 named_bar_sync(1 + q, 64);  // both have read before the next tile writes
                 float inv;
                 const float s = block_scale(__uint_as_float(both), inv);
-                if (rv) {
-                    if (h == 0) a.mid_s[row * ((a.N + 127) / 128) + t.m0 / 128] = s;
-                    uint8_t* o = a.mid_q + row * a.N + t.m0 + h * 64;
+                if (rv && h == 0) a.mid_s[row * ((a.N + 127) / 128) + t.m0 / 128] = s;
+                uint4 o[4];
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        uint32_t w[4];
+                for (int v = 0; v < 4; ++v) {
+                    uint32_t w[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float* m = &acc[0][v * 16 + e * 4];
-                            w[e] = pack4_e4m3(m[0] * inv, m[1] * inv, m[2] * inv, m[3] * inv);
-                        }
-                        if (v * 16 < left)
-                            *reinterpret_cast<uint4*>(o + v * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                    for (int e = 0; e < 4; ++e) {
+                        const float* m = &acc[0][v * 16 + e * 4];
+                        w[e] = pack4_e4m3(m[0] * inv, m[1] * inv, m[2] * inv, m[3] * inv);
                     }
+                    o[v] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
+                transpose4(o);  // 64-byte runs of four lanes, as in store32
+                const int col = (lane & 3) * 16, r0 = r & ~3;
+                uint8_t* y = a.mid_q + (row - r + r0) * a.N + t.m0 + h * 64 + col;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (r0 + j < n && col < left) *reinterpret_cast<uint4*>(y + size_t(j) * a.N) = o[j];
             } else if (work) {
                 const long long p = t.out0 + rank * 128 + q * 32;
 #pragma unroll
