@@ -288,6 +288,53 @@ def test_layer_of_operators():
         assert (np.abs(out.double().cpu().numpy() - b) <= ea + eb).all()
 
 
+@pytest.mark.parametrize("T,H,I", [(1, 2048, 384), (24, 512, 256), (600, 512, 256)])
+def test_inputs_written_just_before_the_call(T, H, I):
+    """Weights, scales, tokens and routing that the launches right ahead of the call
+    wrote are the ones it reads (the products ask for weights early): eager and
+    replayed, equal to the same call with the stream idle in between."""
+    need_gpu()
+    from hummingflight_b200 import fp8, moe
+    E, k = 8, 2
+    rng = np.random.default_rng(T)
+    sets = []
+    for _ in range(2):
+        q, s, _ = make_experts(rng, E, H, I)
+        sets.append((q, s, rows(rng, T, H, "bf16")[0].cuda(), torch.randn((T, E), device="cuda")))
+    q, s, x, l = (v.clone() for v in sets[0])
+    out = torch.empty((T, H), dtype=torch.bfloat16, device="cuda")
+
+    def write(v):
+        l.copy_(v[3])
+        x.copy_(v[2])
+        s.copy_(v[1])
+        q.copy_(v[0])
+
+    def call():
+        return fp8.moe_experts(x, q, s, moe.route_logits(l, None, k), out=out)
+
+    want = []
+    for v in sets:
+        write(v)
+        torch.cuda.synchronize()
+        call()
+        torch.cuda.synchronize()
+        want.append(out.clone())
+    assert not torch.equal(*want)
+    for i in [0, 1] * 4:  # back to back: the writes overwrite what the call before read
+        write(sets[i])
+        assert torch.equal(call(), want[i])
+    graphs = []
+    for v in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            write(v)
+            call()
+    for i in [0, 1] * 4:
+        graphs[i].replay()
+        assert torch.equal(out, want[i])
+
+
 def test_routing_of_the_bf16_layer_is_taken():
     """The dict of MoELayer.route (its permutation has the shared expert's slots
     behind the routed ones)."""
