@@ -270,13 +270,23 @@ __device__ __forceinline__ void unpack(const uint4 v, float (&f)[4]) {
     f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y);
     f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
 }
-__device__ __forceinline__ void unpack(const uint4 v, float (&f)[8]) { unpack8(v, f); }
+__device__ __forceinline__ void unpack(const uint4 v, float (&f)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        f[2 * i] = h.x;
+        f[2 * i + 1] = h.y;
+    }
+}
 
 // A thread takes 16 bytes of a token's columns, all of its picks' loads in flight
 // before the first is used. T = 16384, k = 8, H = 6144, bf16: 299 us, 6.0 TB/s.
-// Y32: the expert outputs are fp32, in n planes (runs of K) that are added in order.
+// Y32: the expert outputs are fp32, in n planes (runs of K) that are added in order;
+// else FP16 with the factors of y_exp (kYBlock).
 template <bool Y32, bool F32>
-__global__ void __launch_bounds__(256) k_fp8_combine(const void* y, int n, const int32_t* pos,
+__global__ void __launch_bounds__(256) k_fp8_combine(const void* y, const uint8_t* y_exp, int n,
+                                                     const int32_t* pos,
                                                      const float* w, int T, int k, int H,
                                                      const void* resid, void* out) {
     constexpr int V = Y32 ? 4 : 8, kBatch = 8;
@@ -289,6 +299,7 @@ __global__ void __launch_bounds__(256) k_fp8_combine(const void* y, int n, const
     for (int j0 = 0; j0 < k; j0 += kBatch) {
         uint4 v[kBatch];
         float wj[kBatch];
+        uint32_t ye[kBatch];
         unsigned at[kBatch];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
@@ -299,13 +310,19 @@ __global__ void __launch_bounds__(256) k_fp8_combine(const void* y, int n, const
             v[j] = in ? ld_nc_u4(static_cast<const char*>(y) +
                                  (size_t(at[j]) * H + c) * (Y32 ? 4 : 2))
                       : make_uint4(0, 0, 0, 0);
+            if constexpr (!Y32)
+                ye[j] = in ? y_exp[size_t(at[j]) * ((H + kYBlock - 1) / kYBlock) + c / kYBlock] : 127u;
         }
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
             if (j0 + j >= k) break;
             float f[V];
             unpack(v[j], f);
-            if constexpr (Y32) {
+            if constexpr (!Y32) {
+                const float s = y_factor(ye[j]);
+#pragma unroll
+                for (int e = 0; e < V; ++e) f[e] *= s;
+            } else {
                 for (int r = 1; r < n && at[j] < rows; ++r) {
                     float g[V];
                     unpack(ld_nc_u4(static_cast<const float*>(y) +
@@ -351,14 +368,15 @@ __global__ void __launch_bounds__(256) k_fp8_combine(const void* y, int n, const
     }
 }
 
-hf_status launch_fp8_combine(const void* y, int n, const int32_t* pos, const float* w, int T, int k,
-                             int H, const void* resid, void* out, bool f32, cudaStream_t st) {
+hf_status launch_fp8_combine(const void* y, const uint8_t* y_exp, int n, const int32_t* pos,
+                             const float* w, int T, int k, int H, const void* resid, void* out,
+                             bool f32, cudaStream_t st) {
     const bool y32 = f32 || n > 1;
     const int v = y32 ? 4 : 8;
     const dim3 grid(unsigned(T), unsigned((H / v + 255) / 256));
     HF_CUDA(launch_pdl(f32 ? k_fp8_combine<true, true>
                            : y32 ? k_fp8_combine<true, false> : k_fp8_combine<false, false>,
-                       grid, dim3(256), 0, st, y, n, pos, w, T, k, H, resid, out));
+                       grid, dim3(256), 0, st, y, y_exp, n, pos, w, T, k, H, resid, out));
     return HF_OK;
 }
 
@@ -372,7 +390,7 @@ constexpr int kFewPositions = 512;
 struct ExpertsWs {
     Fp8Split up, down;  // runs of the gate/up and down products
     bool few;           // the gate/up product writes planes, one for each run
-    size_t pos, xq, sx, gu, mq, ms, y, total;
+    size_t pos, xq, sx, gu, mq, ms, y, ye, total;
 };
 
 ExpertsWs experts_ws(int T, int k, int E, int H, int I, bool f32) {
@@ -401,7 +419,9 @@ ExpertsWs experts_ws(int T, int k, int E, int H, int I, bool f32) {
     w.gu = take(w.few ? size_t(w.up.n) * n * 2 * I * 4 : 0);
     w.mq = take(n * I);
     w.ms = take(n * blocks128(I) * 4);
-    w.y = take(size_t(w.down.n) * n * H * (f32 || w.down.n > 1 ? 4 : 2));
+    const bool y32 = f32 || w.down.n > 1;
+    w.y = take(size_t(w.down.n) * n * H * (y32 ? 4 : 2));
+    w.ye = take(y32 ? 0 : n * ((H + kYBlock - 1) / kYBlock));
     w.total = o;
     return w;
 }
@@ -597,8 +617,9 @@ hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E,
     a.kbper = L.down.per;
     a.out = ws + L.y;
     a.out_f32 = f32 || L.down.n > 1;
+    a.y_exp = a.out_f32 ? nullptr : ws + L.ye;
     HF_TRY(launch_fp8_product(a, false, st));
-    return launch_fp8_combine(ws + L.y, L.down.n, qa.pos, r->topk_weights, T, top_k, H, resid, out,
+    return launch_fp8_combine(ws + L.y, ws + L.ye, L.down.n, qa.pos, r->topk_weights, T, top_k, H, resid, out,
                               f32, st);
 }
 

@@ -65,8 +65,9 @@ HF_API hf_status hf_fp8_gemm(const uint8_t* xq, const float* sx, const uint8_t* 
  * hf_route_logits or hf_moe_route for the same T and k (a shared segment behind
  * the routed ones is left out; topk_ids is not read); offsets, perm entries out
  * of range are skipped. resid: device [T x H] of out_dtype or NULL, may be out
- * itself. out: device [T x H] of out_dtype; the expert outputs y_i are kept in
- * the same type until the combine (bf16 outputs: y_i rounded once more). The
+ * itself. out: device [T x H] of out_dtype; until the combine the expert outputs
+ * y_i are kept in fp32 for fp32 outputs, and for bf16 ones in FP16 times a power of
+ * two per 32 columns (11 significant bits down to 2^-28 of a block's largest). The
  * shared expert, or a dense MLP, is the call with E = 1, k = 1 and the routed
  * output as resid. H and I multiples of 16, k in 1..32, E in 1..1024, T * k and
  * 3 * E * max(H, I) at most 2^31 - 4096; pointers 16-byte aligned, the workspace
