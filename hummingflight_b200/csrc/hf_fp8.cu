@@ -152,8 +152,8 @@ __global__ void __launch_bounds__(256) k_quantize(QuantArgs a) {
     }
 }
 
-// pos[perm[p]] = p. What perm does not name keeps what the workspace holds; its
-// readers check the range.
+// pos[perm[p]] = p. A slot that perm does not name keeps what the workspace holds (a
+// position of an earlier call, say), so pos is read through position_of only.
 __global__ void __launch_bounds__(256) k_positions(const int32_t* perm, int n, int32_t* pos,
                                                    int* err) {
     const int p = blockIdx.x * 256 + threadIdx.x;
@@ -161,6 +161,13 @@ __global__ void __launch_bounds__(256) k_positions(const int32_t* perm, int n, i
     if (p >= n) return;
     const int slot = perm[p];
     if (slot >= 0 && slot < n) pos[slot] = p;
+}
+
+// The position that perm gives a slot, or ~0. n: positions.
+__device__ __forceinline__ unsigned position_of(const int32_t* pos, const int32_t* perm, unsigned n,
+                                                unsigned slot) {
+    const unsigned p = unsigned(pos[slot]);
+    return p < n && unsigned(perm[p]) == slot ? p : ~0u;
 }
 
 // Token-major gather of large batches: a block of a token's row is read and
@@ -172,7 +179,8 @@ __global__ void __launch_bounds__(256) k_quantize_tokens(QuantArgs a) {
     const unsigned half = 0xffffu << (threadIdx.x & 16);
     const int t = blockIdx.x, n = a.n_tok * a.k;
     __shared__ int32_t at[kMaxK];
-    if (int(threadIdx.x) < a.k) at[threadIdx.x] = a.pos[t * a.k + threadIdx.x];
+    if (int(threadIdx.x) < a.k)
+        at[threadIdx.x] = int(position_of(a.pos, a.perm, unsigned(n), t * a.k + threadIdx.x));
     __syncthreads();
     for (int b0 = threadIdx.x >> 4; b0 < a.nb; b0 += 16 * kQuantBatch) {
         Raw8<XF32> r[kQuantBatch];
@@ -283,39 +291,46 @@ __device__ __forceinline__ void unpack(const uint4 v, float (&f)[8]) {
 // A thread takes 16 bytes of a token's columns, all of its picks' loads in flight
 // before the first is used. T = 16384, k = 8, H = 6144, bf16: 299 us, 6.0 TB/s.
 // Y32: the expert outputs are fp32, in n planes (runs of K) that are added in order;
-// else FP16 with the factors of y_exp (kYBlock).
-template <bool Y32, bool F32>
+// else FP16 with the factors of y_exp (kYBlock). A slot without a position in the
+// segments [offsets[0], offsets[E]) counts as 0: its y was not written.
+template <bool Y32, bool F32, int kBatch>
 __global__ void __launch_bounds__(256) k_fp8_combine(const void* y, const uint8_t* y_exp, int n,
-                                                     const int32_t* pos,
-                                                     const float* w, int T, int k, int H,
-                                                     const void* resid, void* out) {
-    constexpr int V = Y32 ? 4 : 8, kBatch = 8;
+                                                     const int32_t* pos, const int32_t* perm,
+                                                     const int32_t* offsets, int E, const float* w,
+                                                     int T, int k, int H, const void* resid,
+                                                     void* out) {
+    constexpr int V = Y32 ? 4 : 8;
     const int t = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * V;
     griddep_wait();
     griddep_launch_dependents();
-    if (c >= H) return;
+    // lane i: the position and weight of pick i (a slot that perm names is one it has
+    // at that position; k_positions); y is asked for before perm has answered
     const unsigned rows = unsigned(T) * unsigned(k);
+    const int lane = threadIdx.x & 31, slot = t * k + lane;
+    const unsigned p = lane < k ? unsigned(pos[slot]) : ~0u;
+    const float wl = lane < k ? w[slot] : 0.0f;
+    const int has = p < rows ? perm[p] : -1, first = offsets[0], end = offsets[E];
+    unsigned named = 0;
     float acc[V] = {};
     for (int j0 = 0; j0 < k; j0 += kBatch) {
         uint4 v[kBatch];
-        float wj[kBatch];
         uint32_t ye[kBatch];
-        unsigned at[kBatch];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            at[j] = j0 + j < k ? unsigned(pos[size_t(t) * k + j0 + j]) : ~0u;
-            // a position out of range (perm does not name the slot) counts as 0
-            const bool in = at[j] < rows;
-            wj[j] = in ? w[size_t(t) * k + j0 + j] : 0.0f;
-            v[j] = in ? ld_nc_u4(static_cast<const char*>(y) +
-                                 (size_t(at[j]) * H + c) * (Y32 ? 4 : 2))
+            const unsigned at = __shfl_sync(~0u, p, (j0 + j) & 31);
+            const bool in = j0 + j < k && at < rows && c < H;
+            v[j] = in ? ld_nc_u4(static_cast<const char*>(y) + (size_t(at) * H + c) * (Y32 ? 4 : 2))
                       : make_uint4(0, 0, 0, 0);
             if constexpr (!Y32)
-                ye[j] = in ? y_exp[size_t(at[j]) * ((H + kYBlock - 1) / kYBlock) + c / kYBlock] : 127u;
+                ye[j] = in ? y_exp[size_t(at) * ((H + kYBlock - 1) / kYBlock) + c / kYBlock] : 127u;
         }
+        if (j0 == 0) named = __ballot_sync(~0u, has == slot && int(p) >= first && int(p) < end);
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
             if (j0 + j >= k) break;
+            const float wj = __shfl_sync(~0u, wl, j0 + j);
+            const unsigned at = __shfl_sync(~0u, p, j0 + j);
+            if (!((named >> (j0 + j)) & 1u)) continue;
             float f[V];
             unpack(v[j], f);
             if constexpr (!Y32) {
@@ -323,18 +338,19 @@ __global__ void __launch_bounds__(256) k_fp8_combine(const void* y, const uint8_
 #pragma unroll
                 for (int e = 0; e < V; ++e) f[e] *= s;
             } else {
-                for (int r = 1; r < n && at[j] < rows; ++r) {
+                for (int r = 1; r < n && c < H; ++r) {
                     float g[V];
                     unpack(ld_nc_u4(static_cast<const float*>(y) +
-                                    (size_t(r) * rows + at[j]) * H + c), g);
+                                    (size_t(r) * rows + at) * H + c), g);
 #pragma unroll
                     for (int e = 0; e < V; ++e) f[e] += g[e];
                 }
             }
 #pragma unroll
-            for (int e = 0; e < V; ++e) acc[e] = __fadd_rn(acc[e], __fmul_rn(wj[j], f[e]));
+            for (int e = 0; e < V; ++e) acc[e] = __fadd_rn(acc[e], __fmul_rn(wj, f[e]));
         }
     }
+    if (c >= H) return;
     const size_t o = size_t(t) * H + c;
     if constexpr (F32) {
         static_assert(Y32, "fp32 outputs come from fp32 expert outputs");
@@ -369,14 +385,19 @@ __global__ void __launch_bounds__(256) k_fp8_combine(const void* y, const uint8_
 }
 
 hf_status launch_fp8_combine(const void* y, const uint8_t* y_exp, int n, const int32_t* pos,
-                             const float* w, int T, int k, int H, const void* resid, void* out,
-                             bool f32, cudaStream_t st) {
+                             const int32_t* perm, const int32_t* offsets, int E, const float* w,
+                             int T, int k, int H, const void* resid, void* out, bool f32,
+                             cudaStream_t st) {
     const bool y32 = f32 || n > 1;
     const int v = y32 ? 4 : 8;
+    // one or two picks: two loads in flight a thread, 32 registers and not 60. The whole
+    // call with one expert of 16384 rows, fp32 onto fp32, us: 1235, with eight 1467
+    const bool one = k <= 2;
     const dim3 grid(unsigned(T), unsigned((H / v + 255) / 256));
-    HF_CUDA(launch_pdl(f32 ? k_fp8_combine<true, true>
-                           : y32 ? k_fp8_combine<true, false> : k_fp8_combine<false, false>,
-                       grid, dim3(256), 0, st, y, y_exp, n, pos, w, T, k, H, resid, out));
+    HF_CUDA(launch_pdl(f32 ? (one ? k_fp8_combine<true, true, 2> : k_fp8_combine<true, true, 8>)
+                           : y32 ? (one ? k_fp8_combine<true, false, 2> : k_fp8_combine<true, false, 8>)
+                                 : (one ? k_fp8_combine<false, false, 2> : k_fp8_combine<false, false, 8>),
+                       grid, dim3(256), 0, st, y, y_exp, n, pos, perm, offsets, E, w, T, k, H, resid, out));
     return HF_OK;
 }
 
@@ -619,8 +640,8 @@ hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E,
     a.out_f32 = f32 || L.down.n > 1;
     a.y_exp = a.out_f32 ? nullptr : ws + L.ye;
     HF_TRY(launch_fp8_product(a, false, st));
-    return launch_fp8_combine(ws + L.y, ws + L.ye, L.down.n, qa.pos, r->topk_weights, T, top_k, H, resid, out,
-                              f32, st);
+    return launch_fp8_combine(ws + L.y, ws + L.ye, L.down.n, qa.pos, r->perm, r->offsets, E,
+                              r->topk_weights, T, top_k, H, resid, out, f32, st);
 }
 
 hf_status hf_fp8_status(const void* workspace, hf_stream stream) {

@@ -63,8 +63,10 @@ HF_API hf_status hf_fp8_gemm(const uint8_t* xq, const float* sx, const uint8_t* 
  * ceil(I/128)]. x: device [T x H] BF16 or fp32, rows ldx elements apart.
  * routing: topk_weights [T x k], counts, offsets and perm as written by
  * hf_route_logits or hf_moe_route for the same T and k (a shared segment behind
- * the routed ones is left out; topk_ids is not read); offsets, perm entries out
- * of range are skipped. resid: device [T x H] of out_dtype or NULL, may be out
+ * the routed ones is left out; topk_ids is not read). offsets do not decrease and
+ * perm names a slot once at most; entries out of range are clipped (offsets) or
+ * skipped (perm), and a slot that perm does not name, or at a position outside
+ * [offsets[0], offsets[E]), adds nothing to its token. resid: device [T x H] of out_dtype or NULL, may be out
  * itself. out: device [T x H] of out_dtype; until the combine the expert outputs
  * y_i are kept in fp32 for fp32 outputs, and for bf16 ones in FP16 times a power of
  * two per 32 columns (11 significant bits down to 2^-28 of a block's largest). The
