@@ -47,6 +47,8 @@ constexpr int kOneBlockT = 16;
 // 586 (300000 x 256) 277 and 296, 1954 (1000000 x 64) 654 and 705.
 constexpr int kScanBlocks = 512;
 constexpr size_t kWsAlign = 256;
+// Dynamic shared memory that needs no opt-in: 48 KB with the kernels' static 144 bytes.
+constexpr int kPlainSmem = 47 * 1024;
 
 struct LogitArgs {
     const void* logits;  // [T x E]
@@ -707,11 +709,11 @@ hf_status launch(const LogitArgs& a, cudaStream_t st) {
     const int threads = std::max(8, (tokens + turns - 1) / turns) * 32;
     const int own = smem + (nb == 1 ? a.T * a.k * 4 : 0) +
                     (a.topk_group < a.n_group ? threads / 32 * a.E * 8 : 0);
-    if (own > 48 * 1024) HF_CUDA(ensure_smem(reinterpret_cast<const void*>(kern), own));
+    if (own > kPlainSmem) HF_CUDA(ensure_smem(reinterpret_cast<const void*>(kern), own));
     kern<<<nb, threads, own, st>>>(a);
     HF_CUDA(cudaGetLastError());
     if (nb > 1) {
-        if (smem > 48 * 1024)
+        if (smem > kPlainSmem)
             HF_CUDA(ensure_smem(reinterpret_cast<const void*>(k_route_scatter), smem));
         const int scan = nb > kScanBlocks;
         if (scan) {
