@@ -106,37 +106,32 @@ struct Place {
     static constexpr uint32_t kMask = (1u << kBits) - 1u;
 };
 
-template <int NPL, typename C>
-__device__ __forceinline__ C packed(C code, int j) {
-    return (code & ~C(Place<NPL>::kMask)) | C(NPL - 1 - j);
+template <int NPL>
+__device__ __forceinline__ uint32_t packed(uint32_t code, int j) {
+    return (code & ~Place<NPL>::kMask) | uint32_t(NPL - 1 - j);
 }
-template <int NPL, typename C>
-__device__ __forceinline__ auto value_at(C packed_code) {
-    return value_of(packed_code & ~C(Place<NPL>::kMask));
+template <int NPL>
+__device__ __forceinline__ float value_at(uint32_t packed_code) {
+    return value_of(packed_code & ~Place<NPL>::kMask);
 }
 
 // How far the key of code a is above that of code b, beyond what the fp32 sums
 // (2^-23 of each) and the replaced bits (2^(kBits - 23)) may hide: not positive
-// when either could be the larger. On 64-bit keys the replaced bits are far below
-// any difference of interest.
+// when either could be the larger.
 template <int NPL>
 __device__ __forceinline__ float beyond(float diff, float size) {
     constexpr float kRel = float(2 + (1 << Place<NPL>::kBits)) * 0x1p-23f;
     return diff - kRel * size;
 }
 template <int NPL>
-__device__ __forceinline__ double beyond(double diff, double) {
-    return diff;
-}
-template <int NPL, typename C>
-__device__ __forceinline__ auto above(C a, C b) {
-    const auto x = value_at<NPL>(a), y = value_at<NPL>(b);
+__device__ __forceinline__ float above(uint32_t a, uint32_t b) {
+    const float x = value_at<NPL>(a), y = value_at<NPL>(b);
     return beyond<NPL>(x - y, fabs(x) + fabs(y));
 }
 
 // Descending sort of a lane's codes: Batcher's merge exchange.
-template <int NPL, typename C>
-__device__ __forceinline__ void sort_lane(C (&c)[NPL]) {
+template <int NPL>
+__device__ __forceinline__ void sort_lane(uint32_t (&c)[NPL]) {
 #pragma unroll
     for (int p = 1; p < NPL; p <<= 1)
 #pragma unroll
@@ -146,10 +141,38 @@ __device__ __forceinline__ void sort_lane(C (&c)[NPL]) {
 #pragma unroll
                 for (int i = 0; i < k; ++i)
                     if (i + j + k < NPL && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
-                        const C hi = max(c[i + j], c[i + j + k]), lo = min(c[i + j], c[i + j + k]);
+                        const uint32_t hi = max(c[i + j], c[i + j + k]);
+                        const uint32_t lo = min(c[i + j], c[i + j + k]);
                         c[i + j] = hi;
                         c[i + j + k] = lo;
                     }
+}
+
+// The best two of a group's n codes, read from place i on. (Equal keys count twice.)
+template <typename C>
+__device__ __forceinline__ void best_two(const C* g, int n, int i, C* b1, C* b2) {
+    C m1 = 0, m2 = 0;
+#pragma unroll 4
+    for (int q = 0; q < n; ++q) {
+        const C v = g[i];
+        m2 = max(m2, min(m1, v));
+        m1 = max(m1, v);
+        if (++i == n) i = 0;
+    }
+    *b1 = m1;
+    *b2 = m2;
+}
+
+// Rank of the lane's group by its score's code and its number.
+template <typename C>
+__device__ __forceinline__ int group_rank(C code, int n_group, int lane) {
+    int rank = 0;
+#pragma unroll 4
+    for (int g = 0; g < n_group; ++g) {
+        const C o = __shfl_sync(~0u, code, g);
+        rank += (o > code) || (o == code && g < lane);
+    }
+    return rank;
 }
 
 // Drops the experts of the groups that are not kept (their codes become 0).
@@ -157,47 +180,32 @@ __device__ __forceinline__ void sort_lane(C (&c)[NPL]) {
 // scans group g's codes in the warp's scratch `scr` [E], from a place of its own
 // so that groups of 32 do not meet in one bank. *gap: how far the last kept group
 // is above the best dropped one.
-template <int NPL, typename C, typename F>
-__device__ __forceinline__ void keep_groups(C (&c)[NPL], const C (&gc)[NPL], const LogitArgs& a,
-                                            int lane, C* scr, F* gap) {
+template <int NPL>
+__device__ __forceinline__ void keep_groups(uint32_t (&c)[NPL], const uint32_t (&gc)[NPL],
+                                            const LogitArgs& a, int lane, uint32_t* scr,
+                                            float* gap) {
     const int gs = a.E / a.n_group;
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < NPL; ++j)
         if (j * 32 + lane < a.E) scr[j * 32 + lane] = gc[j];
     __syncwarp();
-    C b1 = 0, b2 = 0, code = 0;  // the best two keys of group `lane`, its score's code
-    F size = 0;                  // and the magnitudes that were added
+    uint32_t code = 0;  // of the score of group `lane`
+    float size = 0.0f;  // and the magnitudes that were added
     if (lane < a.n_group) {
-        const C* g = scr + lane * gs;
-        int i = lane % gs;
-#pragma unroll 4
-        for (int q = 0; q < gs; ++q) {
-            // places differ inside a lane's codes only: equal keys of two lanes may
-            // be equal codes, and count twice all the same
-            const C v = g[i];
-            b2 = max(b2, min(b1, v));
-            b1 = max(b1, v);
-            if (++i == gs) i = 0;
-        }
-        F s = value_at<NPL>(b1);
-        size = fabs(s);
+        uint32_t b1, b2;
+        best_two(scr + lane * gs, gs, lane % gs, &b1, &b2);
+        float s = value_at<NPL>(b1);
+        size = fabsf(s);
         if (a.group_top == 2 && gs > 1) {
-            const F s2 = value_at<NPL>(b2);
+            const float s2 = value_at<NPL>(b2);
             s = s + s2;
-            size = size + fabs(s2);
+            size = size + fabsf(s2);
         }
         code = code_of(s);
     }
-    // rank of lane's group: the groups before it
-    int rank = 0;
-#pragma unroll 4
-    for (int g = 0; g < a.n_group; ++g) {
-        const C o = __shfl_sync(~0u, code, g);
-        rank += (o > code) || (o == code && g < lane);
-    }
-    const bool in = lane < a.n_group && rank < a.topk_group;
-    const unsigned kept = __ballot_sync(~0u, in);
+    const int rank = group_rank(code, a.n_group, lane);
+    const unsigned kept = __ballot_sync(~0u, lane < a.n_group && rank < a.topk_group);
     const unsigned last = __ballot_sync(~0u, lane < a.n_group && rank == a.topk_group - 1);
     const unsigned next = __ballot_sync(~0u, lane < a.n_group && rank == a.topk_group);
     const int ll = __ffs(last) - 1, ln = __ffs(next) - 1;
@@ -212,12 +220,12 @@ __device__ __forceinline__ void keep_groups(C (&c)[NPL], const C (&gc)[NPL], con
 
 // Takes the best code of the warp out of the lanes' sorted lists: its packed code
 // (0 when none is left), and the id in *id.
-template <int NPL, typename C>
-__device__ __forceinline__ C take_best(C (&c)[NPL], int lane, int* id) {
-    const C m = warp_max(c[0]);
+template <int NPL>
+__device__ __forceinline__ uint32_t take_best(uint32_t (&c)[NPL], int lane, int* id) {
+    const uint32_t m = warp_max(c[0]);
     // equal codes have equal places, so the lowest lane has the lowest id
     const int w = __ffs(__ballot_sync(~0u, c[0] == m)) - 1;
-    *id = (NPL - 1 - int(uint32_t(m) & Place<NPL>::kMask)) * 32 + w;
+    *id = (NPL - 1 - int(m & Place<NPL>::kMask)) * 32 + w;
     const bool mine = lane == w;
 #pragma unroll
     for (int j = 0; j + 1 < NPL; ++j) c[j] = mine ? c[j + 1] : c[j];
@@ -228,9 +236,9 @@ __device__ __forceinline__ C take_best(C (&c)[NPL], int lane, int* id) {
 // Whether code b (<= a) is not clearly below a: the codes are equal but for the
 // place (`exact`), or not more than tol apart; a NaN difference (inf - inf)
 // counts as close.
-template <int NPL, typename C, typename F>
-__device__ __forceinline__ bool is_close(C a, C b, bool exact, F tol) {
-    const C place = C(Place<NPL>::kMask);
+template <int NPL>
+__device__ __forceinline__ bool is_close(uint32_t a, uint32_t b, bool exact, float tol) {
+    constexpr uint32_t place = Place<NPL>::kMask;
     return exact ? (a | place) == (b | place) : !(above<NPL>(a, b) > tol);
 }
 
@@ -301,34 +309,60 @@ __device__ __noinline__ int refine(const LogitArgs& a, int t, int lane, int id, 
 }
 
 // The whole choice in 64 bits (groups too close to tell apart, more candidates
-// than lanes).
+// than lanes): whole codes, so that equal keys and scores are the only ties, and the
+// lowest id or group takes those. scr: the warp's row of E codes.
 template <int NPL>
 __device__ __noinline__ int pick_exact(const LogitArgs& a, int t, int lane,
                                        unsigned long long* scr) {
-    unsigned long long c[NPL];
+    unsigned long long c[NPL];  // 0: not in the choice
     double mx = 0.0, sum = 1.0;
     if (a.score == HF_SCORE_SOFTMAX) sum = softmax_sum(a, t, lane, &mx);
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
         const int e = j * 32 + lane;
-        c[j] = e < a.E ? packed<NPL>(code_of(key64(a, t, e, mx, sum)), j) : 0ull;
+        c[j] = e < a.E ? code_of(key64(a, t, e, mx, sum)) : 0ull;
     }
-    double gap;
-    if (a.topk_group < a.n_group) keep_groups(c, c, a, lane, scr, &gap);
-    if (a.bias == nullptr) {  // by logit, whose codes lose nothing in 64 bits
+    unsigned kept = ~0u;
+    const int gs = a.E / a.n_group;
+    if (a.topk_group < a.n_group) {
+        __syncwarp();
 #pragma unroll
         for (int j = 0; j < NPL; ++j)
-            if (c[j])
-                c[j] = ((unsigned long long)code_of(load_logit(a, size_t(t) * a.E + j * 32 + lane))
-                        << 32) | (unsigned long long)(NPL - 1 - j);
+            if (j * 32 + lane < a.E) scr[j * 32 + lane] = c[j];
+        __syncwarp();
+        unsigned long long code = 0;
+        if (lane < a.n_group) {
+            unsigned long long b1, b2;
+            best_two(scr + lane * gs, gs, lane % gs, &b1, &b2);
+            code = a.group_top == 2 && gs > 1 ? code_of(value_of(b1) + value_of(b2)) : b1;
+        }
+        const int rank = group_rank(code, a.n_group, lane);
+        kept = __ballot_sync(~0u, lane < a.n_group && rank < a.topk_group);
     }
-    sort_lane(c);
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) {
+        const int e = j * 32 + lane;
+        if (e >= a.E || !((kept >> (e / gs)) & 1u)) c[j] = 0;
+        else if (a.bias == nullptr)  // by logit
+            c[j] = (unsigned long long)code_of(load_logit(a, size_t(t) * a.E + e)) << 32;
+    }
     int mine = 0;
 #pragma unroll 1
     for (int r = 0; r < a.k; ++r) {
-        int id;
-        take_best(c, lane, &id);
-        if (lane == r) mine = id;
+        unsigned long long m = 0;
+        int at = 0;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j)
+            if (c[j] > m) {
+                m = c[j];
+                at = j;
+            }
+        const unsigned long long best = warp_max(m);
+        const unsigned id = __reduce_min_sync(~0u, m == best ? unsigned(at * 32 + lane) : ~0u);
+        if (lane == r) mine = int(id);
+#pragma unroll
+        for (int j = 0; j < NPL; ++j)
+            if (id == unsigned(j * 32 + lane)) c[j] = 0;
     }
     return mine;
 }
