@@ -197,7 +197,7 @@ __device__ __forceinline__ void keep_groups(uint32_t (&c)[NPL], const uint32_t (
         best_two(scr + lane * gs, gs, lane % gs, &b1, &b2);
         float s = value_at<NPL>(b1);
         size = fabsf(s);
-        if (a.group_top == 2 && gs > 1) {
+        if (a.group_top == 2) {
             const float s2 = value_at<NPL>(b2);
             s = s + s2;
             size = size + fabsf(s2);
@@ -315,12 +315,18 @@ template <int NPL>
 __device__ __noinline__ int pick_exact(const LogitArgs& a, int t, int lane,
                                        unsigned long long* scr) {
     unsigned long long c[NPL];  // 0: not in the choice
+    // without a bias logits rank, but for the sums of two scores
+    const bool by_logit = a.bias == nullptr, by_score = !by_logit || a.group_top == 2;
+    const auto logit_code = [&](int e) {
+        return (unsigned long long)code_of(load_logit(a, size_t(t) * a.E + e)) << 32;
+    };
     double mx = 0.0, sum = 1.0;
-    if (a.score == HF_SCORE_SOFTMAX) sum = softmax_sum(a, t, lane, &mx);
+    if (by_score && a.score == HF_SCORE_SOFTMAX) sum = softmax_sum(a, t, lane, &mx);
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
         const int e = j * 32 + lane;
-        c[j] = e < a.E ? code_of(key64(a, t, e, mx, sum)) : 0ull;
+        if (e >= a.E) c[j] = 0;
+        else c[j] = by_score ? code_of(key64(a, t, e, mx, sum)) : logit_code(e);
     }
     unsigned kept = ~0u;
     const int gs = a.E / a.n_group;
@@ -334,7 +340,7 @@ __device__ __noinline__ int pick_exact(const LogitArgs& a, int t, int lane,
         if (lane < a.n_group) {
             unsigned long long b1, b2;
             best_two(scr + lane * gs, gs, lane % gs, &b1, &b2);
-            code = a.group_top == 2 && gs > 1 ? code_of(value_of(b1) + value_of(b2)) : b1;
+            code = a.group_top == 2 ? code_of(value_of(b1) + value_of(b2)) : b1;
         }
         const int rank = group_rank(code, a.n_group, lane);
         kept = __ballot_sync(~0u, lane < a.n_group && rank < a.topk_group);
@@ -343,8 +349,7 @@ __device__ __noinline__ int pick_exact(const LogitArgs& a, int t, int lane,
     for (int j = 0; j < NPL; ++j) {
         const int e = j * 32 + lane;
         if (e >= a.E || !((kept >> (e / gs)) & 1u)) c[j] = 0;
-        else if (a.bias == nullptr)  // by logit
-            c[j] = (unsigned long long)code_of(load_logit(a, size_t(t) * a.E + e)) << 32;
+        else if (by_logit && by_score) c[j] = logit_code(e);
     }
     int mine = 0;
 #pragma unroll 1
@@ -821,7 +826,7 @@ hf_status hf_route_logits(const void* logits, hf_dtype dtype, const float* bias,
     a.score = spec->score;
     a.n_group = spec->n_group;
     a.topk_group = spec->topk_group;
-    a.group_top = spec->group_top;
+    a.group_top = a.E == a.n_group ? 1 : spec->group_top;  // a group of one has no second key
     a.norm = spec->norm;
     a.scale = spec->scale;
     a.ids = r->topk_ids;

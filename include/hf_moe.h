@@ -319,7 +319,8 @@ HF_API hf_status hf_topk_scores(const float* scores, int T, int E, const float* 
  * divided by their sum (rank order) when norm is set and that sum is positive,
  * times scale. Ties (of keys and of groups) go to the lower id. Which expert
  * ranks before which is decided as if in 64-bit arithmetic; without a bias the
- * keys rank as the logits do. A NaN key ranks below every number. A softmax
+ * keys, and the scores of groups of which one key counts, rank as the logits do
+ * (so that sigmoids of 40 and 50 are no tie). A NaN key ranks below every number. A softmax
  * row of which every logit is -inf has p = 0; one with a NaN or +inf logit has
  * NaN weights. */
 typedef enum hf_score { HF_SCORE_SIGMOID = 0, HF_SCORE_SOFTMAX = 1 } hf_score;

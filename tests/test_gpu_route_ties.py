@@ -52,3 +52,33 @@ def test_keys_a_few_units_apart(E, groups):
     check(l, b, min(8, E // 8), *groups)
     check(l, b, min(8, E // 8), *groups, 1)
     check(l, np.zeros(E), min(8, E // 8), *groups)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("E,n_group,group_top", [(64, 8, 1), (300, 10, 1), (512, 32, 1), (32, 32, 2),
+                                                 (8, 8, 2)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_groups_without_a_bias_rank_by_logit(score, E, n_group, group_top, dtype):
+    """One key a group: their order is that of the largest logits, also where every
+    score is the same number (1, or a softmax of 0), far apart and one step apart."""
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from hummingflight_b200 import moe
+    rng = np.random.default_rng(E)
+    keep, k = n_group // 2, min(8, E // n_group * (n_group // 2))
+    t = torch.float32 if dtype == "f32" else torch.bfloat16
+    for base, step in ((100.0, 2.0 ** -17), (40.0, 0.5), (100.0, 1.0), (-1000.0, 2.0 ** -14),
+                       (-1000.0, 8.0)):
+        l = base + step * rng.integers(0, E, (29, E))
+        if score == "softmax" and base < 0:
+            l[:, 0] = 0.0
+        l = torch.from_numpy(l).to(t)
+        d = l.double().numpy()
+        top = d.reshape(29, n_group, -1).max(2)
+        ids = np.empty((29, k), np.int64)
+        for i in range(29):
+            kept = sorted(range(n_group), key=lambda g: (-top[i, g], g))[:keep]
+            ids[i] = sorted((e for e in range(E) if e // (E // n_group) in kept),
+                            key=lambda e: (-d[i, e], e))[:k]
+        got = moe.route_logits(l.cuda(), None, k, score, n_group, keep, group_top)
+        assert np.array_equal(got["topk_ids"].cpu().numpy(), ids)
