@@ -241,11 +241,11 @@ hf_status launch_quantize(const QuantArgs& a, bool f32, int dev, cudaStream_t st
 // quantised. 16 threads a block of 128 columns.
 __global__ void __launch_bounds__(256) k_swiglu_planes(const float* planes, int n, int rows, int I,
                                                        int nb, uint8_t* q, float* s) {
-    griddep_launch_dependents();
     const int sub = threadIdx.x & 15;
     const unsigned half = 0xffffu << (threadIdx.x & 16);
     const int i = blockIdx.x * 16 + (threadIdx.x >> 4);
     griddep_wait();
+    griddep_launch_dependents();  // behind the wait: see Fp8Args::early
     if (i >= rows * nb) return;  // the 16 threads of a block agree
     const int p = i / nb, b = i % nb, c = b * kFp8Block + sub * 8;
     float f[8] = {};
