@@ -35,6 +35,19 @@ struct QuantArgs {
 };
 constexpr int kQuantBatch = 4;
 
+// 16 bytes that are read once. These kernels may start while the launch that writes
+// what they read still runs, so the read-only path (.nc), which holds for memory that
+// nobody writes while the kernel lives, is not theirs; nor may a load move ahead of
+// griddep_wait.
+__device__ __forceinline__ uint4 ld_once_u4(const void* p) {
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                 : "l"(p)
+                 : "memory");
+    return r;
+}
+
 // 8 columns as they lie in memory.
 template <bool XF32>
 struct Raw8 {
@@ -42,10 +55,10 @@ struct Raw8 {
     __device__ __forceinline__ void load(const void* x, long long i) {
         if constexpr (XF32) {
             const float* p = static_cast<const float*>(x) + i;
-            v[0] = ld_stream_u4(p);
-            v[1] = ld_stream_u4(p + 4);
+            v[0] = ld_once_u4(p);
+            v[1] = ld_once_u4(p + 4);
         } else {
-            v[0] = ld_stream_u4(static_cast<const uint16_t*>(x) + i);
+            v[0] = ld_once_u4(static_cast<const uint16_t*>(x) + i);
         }
     }
     __device__ __forceinline__ void zero() {
@@ -319,7 +332,7 @@ __global__ void __launch_bounds__(256) k_fp8_combine(const void* y, const uint8_
         for (int j = 0; j < kBatch; ++j) {
             const unsigned at = __shfl_sync(~0u, p, (j0 + j) & 31);
             const bool in = j0 + j < k && at < rows && c < H;
-            v[j] = in ? ld_nc_u4(static_cast<const char*>(y) + (size_t(at) * H + c) * (Y32 ? 4 : 2))
+            v[j] = in ? ld_once_u4(static_cast<const char*>(y) + (size_t(at) * H + c) * (Y32 ? 4 : 2))
                       : make_uint4(0, 0, 0, 0);
             if constexpr (!Y32)
                 ye[j] = in ? y_exp[size_t(at) * ((H + kYBlock - 1) / kYBlock) + c / kYBlock] : 127u;
@@ -340,7 +353,7 @@ __global__ void __launch_bounds__(256) k_fp8_combine(const void* y, const uint8_
             } else {
                 for (int r = 1; r < n && c < H; ++r) {
                     float g[V];
-                    unpack(ld_nc_u4(static_cast<const float*>(y) +
+                    unpack(ld_once_u4(static_cast<const float*>(y) +
                                     (size_t(r) * rows + at) * H + c), g);
 #pragma unroll
                     for (int e = 0; e < V; ++e) f[e] += g[e];

@@ -30,3 +30,11 @@ def test_a_launch_lets_the_next_start_behind_its_own_wait():
                 seen += 1
                 assert 0 <= body.find("griddep_wait()") < trigger, kernel
     assert seen >= 5
+
+
+def test_kernels_that_start_early_do_not_read_through_the_read_only_path():
+    """ld.global.nc is for memory that nobody writes while the kernel lives; a kernel
+    that starts ahead of its predecessor's end lives while its inputs are written."""
+    for name in ("hf_fp8.cu", "hf_fp8_gemm.cu", "hf_logits.cu"):
+        src = re.sub(r"//[^\n]*", "", open(os.path.join(CSRC, name)).read())
+        assert not re.findall(r"\b(ld_nc_\w+|ld_stream_\w+|__ldg)\(|ld\.global\.nc", src), name
