@@ -314,30 +314,30 @@ __global__ void __launch_bounds__(256) k_fp8_combine(const void* y, const uint8_
                                                      void* out) {
     constexpr int V = Y32 ? 4 : 8;
     const int t = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * V;
-    griddep_wait();
-    griddep_launch_dependents();
     // lane i: the position and weight of pick i (a slot that perm names is one it has
-    // at that position; k_positions); y is asked for before perm has answered
+    // at that position; k_positions). They are older than the down product, which lets
+    // this launch start behind its own wait (Fp8Args::early), and are read ahead of its end.
     const unsigned rows = unsigned(T) * unsigned(k);
     const int lane = threadIdx.x & 31, slot = t * k + lane;
     const unsigned p = lane < k ? unsigned(pos[slot]) : ~0u;
     const float wl = lane < k ? w[slot] : 0.0f;
     const int has = p < rows ? perm[p] : -1, first = offsets[0], end = offsets[E];
-    unsigned named = 0;
+    const unsigned named = __ballot_sync(~0u, has == slot && int(p) >= first && int(p) < end);
+    griddep_wait();
+    griddep_launch_dependents();
     float acc[V] = {};
     for (int j0 = 0; j0 < k; j0 += kBatch) {
         uint4 v[kBatch];
         uint32_t ye[kBatch];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            const unsigned at = __shfl_sync(~0u, p, (j0 + j) & 31);
-            const bool in = j0 + j < k && at < rows && c < H;
+            const unsigned at = __shfl_sync(~0u, p, j0 + j);
+            const bool in = ((named >> (j0 + j)) & 1u) && c < H;
             v[j] = in ? ld_once_u4(static_cast<const char*>(y) + (size_t(at) * H + c) * (Y32 ? 4 : 2))
                       : make_uint4(0, 0, 0, 0);
             if constexpr (!Y32)
                 ye[j] = in ? y_exp[size_t(at) * ((H + kYBlock - 1) / kYBlock) + c / kYBlock] : 127u;
         }
-        if (j0 == 0) named = __ballot_sync(~0u, has == slot && int(p) >= first && int(p) < end);
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
             if (j0 + j >= k) break;
