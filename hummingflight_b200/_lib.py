@@ -136,6 +136,8 @@ SIGNATURES = {
                                    c_int, c_int, ctypes.POINTER(HfMoeRouting), c_vp, c_vp, c_int,
                                    c_vp, c_size, c_vp]),
     "hf_fp8_status": (c_int, [c_vp, c_vp]),
+    "hf_fp8_set_wait_timeout": (c_int, [c_u64]),
+    "hf_fp8_debug_stall": (c_int, [c_int]),
     "hf_ingest_release_staging": (c_int, []),
     "hf_st_layer_shards": (c_int, [ctypes.c_char_p, c_int, c_vp, c_size, ctypes.POINTER(c_int)]),
 }

@@ -657,6 +657,17 @@ hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E,
                               r->topk_weights, T, top_k, H, resid, out, f32, st);
 }
 
+hf_status hf_fp8_set_wait_timeout(uint64_t ns) {
+    set_fp8_wait(ns);
+    return HF_OK;
+}
+
+hf_status hf_fp8_debug_stall(int block) {
+    if (block < -kMaxExtent) return fail(HF_ERR_ARG, "hf_fp8_debug_stall: block out of range");
+    set_fp8_stall(block);
+    return HF_OK;
+}
+
 hf_status hf_fp8_status(const void* workspace, hf_stream stream) {
     if (!workspace) return fail(HF_ERR_ARG, "hf_fp8_status: null workspace");
     HF_CUDA(cudaStreamSynchronize(as_cuda(stream)));

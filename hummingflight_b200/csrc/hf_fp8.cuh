@@ -93,12 +93,19 @@ struct Fp8Args {
     float* mid_s;
     int* err;               // error word: set when a bounded wait gives up
     int clear_err;          // the first kernel of a call clears it
+    // limit of a wait, unsigned us (set by launch_fp8_product), and the test hook: the copies
+    // stop ahead of a CTA's stall-th block of K (0: never) and wait on a barrier that
+    // nothing signals; stall < 0: those of a pair's second CTA only
+    int wait_us;
+    int stall;
     // 1: the launch before this one is of the same call and lets this one start only
     // after its own griddep_wait, so everything ahead of the call is done: offsets and
     // weights can be read before this kernel's griddep_wait
     int early;
 };
-hf_status launch_fp8_product(const Fp8Args& a, bool glu, cudaStream_t st);
+hf_status launch_fp8_product(Fp8Args a, bool glu, cudaStream_t st);
+void set_fp8_wait(unsigned long long ns);  // 0: the default
+void set_fp8_stall(int block);
 // Positions of a tile, by the mean per segment (256: the pair kernel's).
 int fp8_tile_rows(int mean);
 struct Fp8Split {

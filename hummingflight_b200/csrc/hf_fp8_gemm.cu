@@ -25,6 +25,7 @@
 // 128 intermediate columns (one block) per position and writes e4m3 values and
 // the scale, so the intermediate never leaves the SM in more than 8 bits.
 #include <algorithm>
+#include <atomic>
 #include <map>
 #include <mutex>
 
@@ -48,7 +49,10 @@ constexpr int kNarrow32 = 48;
 constexpr int kScaleSlots = 4;
 constexpr uint32_t kABytes = 128 * 128;  // 128 weight rows x 128 bytes
 constexpr uint64_t kWaitNs = 2000ull * 1000 * 1000;
-constexpr uint64_t kDrainNs = 500ull * 1000 * 1000;
+// What a warp that gave up waits for its copies or MMAs in flight, all together: a
+// thousand times what they take. (Barriers that also wait for copies never asked for
+// do not complete.)
+constexpr uint64_t kDrainNs = 20ull * 1000 * 1000;
 
 template <int BN>
 struct Cfg {
@@ -64,7 +68,7 @@ struct Cfg {
     // the plan: offsets and tile prefix of up to 1024 segments
     static constexpr int kStages0 = (227 * 1024 - 1024 - kFixed - 2 * 1025 * 4) / kStageBytes;
     static constexpr int kStages = kStages0 > 8 ? 8 : kStages0;
-    static_assert((2 * kStages + kBufs + 2 * kScaleSlots + 1) * 8 + 8 <= kBarBytes, "barriers");
+    static_assert((2 * kStages + kBufs + 2 * kScaleSlots + 2) * 8 + 12 <= kBarBytes, "barriers");
     static_assert(kStageBytes % 1024 == 0 && kStages >= 3, "stages");
     static int smem(int G) { return 1024 + kStages * kStageBytes + kFixed + 2 * (G + 1) * 4; }
 };
@@ -151,11 +155,9 @@ __device__ __forceinline__ void decode(const Fp8Args& a, const int* off, const i
     else t.s1 = t.m0 + 128 < a.N ? t.s0 + KB : t.s0;
 }
 
-__device__ __forceinline__ bool drain_wait(uint64_t* bar, uint32_t parity) {
-    const uint64_t dl = globaltimer() + kDrainNs;
+__device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity, uint64_t deadline) {
     while (!mbar_try_wait(bar, parity))
-        if (globaltimer() > dl) return false;
-    return true;
+        if (globaltimer() > deadline) return;
 }
 
 // Four accumulators += sums times scales. (Packed pairs, fma.rn.f32x2, run at the
@@ -195,8 +197,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* sfull = tempty + NB;
     uint64_t* sempty = sfull + kScaleSlots;
     uint64_t* final_bar = sempty + kScaleSlots;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 1);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    uint64_t* stall_bar = final_bar + 1;  // never signalled (test hook)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stall_bar + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);  // and the limit
     int* off = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(full) + C::kBarBytes);  // [G+1]
     int* pref = off + a.G + 1;                                                           // [G+1]
 
@@ -215,7 +218,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&sempty[b], kAccWarps);
         }
         mbar_init(final_bar, 1);
-        *abort_flag = 0;
+        mbar_init(stall_bar, 1);
+        abort_flag[0] = 0;
+        abort_flag[1] = a.wait_us;
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -233,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem_base = *tmem_slot;
     const int total = pref[a.G] * (GLU ? 1 : a.nsplit);
     const auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return mbar_wait_for(smem_u32(bar), parity, abort_flag, kWaitNs);
+        return mbar_wait_for(smem_u32(bar), parity, abort_flag);
     };
 
     if (warp < 4) {
@@ -261,6 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             griddep_wait();
             griddep_launch_dependents();
+            const uint32_t stall = a.stall > 0 ? uint32_t(a.stall) - 1 : ~0u;
             bool ok = true;
             for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
                 Tile t;
@@ -268,24 +274,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int nb = (t.n + C::kBoxB - 1) / C::kBoxB;
                 for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
                     const uint32_t s = it % S;
-                    if (!wait(&done[s], ((it / S) & 1) ^ 1)) {
+                    const bool st = it == stall;
+                    if (!wait(st ? stall_bar : &done[s], st ? 0 : ((it / S) & 1) ^ 1)) {
                         ok = false;
                         break;
                     }
                     if (elect_one()) {
                         if (it >= pre) load_weights(t, s, kb);
-                        uint8_t* st = smem + s * C::kStageBytes + 2 * kABytes;
+                        uint8_t* at = smem + s * C::kStageBytes + 2 * kABytes;
                         for (int j = 0; j < nb; ++j)
-                            tma_load_2d(st + j * C::kBoxB * 128, &tmB, &full[s], kb * 128,
+                            tma_load_2d(at + j * C::kBoxB * 128, &tmB, &full[s], kb * 128,
                                         t.row0 + j * C::kBoxB);
                     }
                     __syncwarp();
                 }
             }
             if (!ok) {  // every issued load lands before the CTA leaves
+                const uint64_t dl = globaltimer() + kDrainNs;
                 const uint32_t first = it > uint32_t(S) ? it - S : 0;
                 it = max(it, pre);
-                for (uint32_t i = first; i < it; ++i) drain_wait(&full[i % S], (i / S) & 1);
+                for (uint32_t i = first; i < it; ++i) drain_wait(&full[i % S], (i / S) & 1, dl);
             }
         } else if (warp == 1) {
             // ------------------------------------------------------ MMA issuer
@@ -319,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (elect_one()) mma_commit(final_bar);  // once every MMA issued above is done
             __syncwarp();
-            drain_wait(final_bar, 0);
+            drain_wait(final_bar, 0, globaltimer() + kDrainNs);
         } else if (warp == 2) {
             // ------------------------------------------------------ scales
             constexpr int PL = BN / 32;
@@ -707,9 +715,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     uint64_t* sfull = tempty + 4;
     uint64_t* sempty = sfull + kPairSlots;
     uint64_t* final_bar = sempty + kPairSlots;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 1);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    static_assert((3 * S + 4 + 2 * kPairSlots + 1) * 8 + 8 <= kPairBar, "barriers");
+    uint64_t* stall_bar = final_bar + 1;  // never signalled (test hook)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stall_bar + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);  // and the limit
+    static_assert((3 * S + 4 + 2 * kPairSlots + 2) * 8 + 12 <= kPairBar, "barriers");
     float* sc = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(full) + kPairBar);
     uint32_t* red = reinterpret_cast<uint32_t*>(sc + kPairSlots * kPairScale / 4);
     int* off = reinterpret_cast<int*>(red + 2 * 128);
@@ -733,7 +742,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             mbar_init(&sempty[b], kPairWarps);
         }
         mbar_init(final_bar, 2);
-        *abort_flag = 0;
+        mbar_init(stall_bar, 1);
+        abort_flag[0] = 0;
+        abort_flag[1] = a.wait_us;
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -754,7 +765,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     // and the MMAs write and read shared memory, tcgen05 fences order the tensor
     // memory), so every wait orders this CTA's accesses only.
     const auto wait = [&](uint32_t bar, uint32_t parity) {
-        return mbar_wait_for(bar, parity, abort_flag, kWaitNs);
+        return mbar_wait_for(bar, parity, abort_flag);
     };
     const uint32_t full_at = smem_u32(full), done_at = smem_u32(done);
 
@@ -765,6 +776,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             tma_prefetch_desc(&tmA);
             tma_prefetch_desc(&tmB);
             uint32_t s = 0, ph = 1, issued = 0;
+            // (folded into a wait that is there: a wait of its own cost 5 % of the kernel)
+            const uint32_t stall = a.stall > 0 || (a.stall < 0 && rank) ? uint32_t(abs(a.stall)) - 1 : ~0u;
             bool ok = true;
             for (int u = first; u < total && ok; u += step) {
                 Tile t;
@@ -775,18 +788,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 const int wrow = rank ? t.a1 : t.a0;
                 const uint32_t bytes = 2 * kABytes + (nb0 + nb1) * kPairBox * 128;
                 for (int kb = t.kb0; kb < t.kb1; ++kb, ++issued) {
-                    if (!wait(done_at + s * 8, ph) || !wait(done_at + (S + s) * 8, ph)) {
+                    const bool st = issued == stall;
+                    if (!wait(st ? smem_u32(stall_bar) : done_at + s * 8, st ? 0 : ph) ||
+                        !wait(done_at + (S + s) * 8, ph)) {
                         ok = false;
                         break;
                     }
                     if (elect_one()) {
-                        uint8_t* st = smem + s * kPairStage;
+                        uint8_t* at = smem + s * kPairStage;
                         const uint32_t fb = cluster_addr(&full[s], 0);
                         if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
                         for (int j = 0; j < nb; ++j)
-                            tma_load_2d_pair(st + j * kPairBox * 128, &tmB, fb, kb * 128,
+                            tma_load_2d_pair(at + j * kPairBox * 128, &tmB, fb, kb * 128,
                                              row + j * kPairBox);
-                        tma_load_2d_pair(st + kABytes, &tmA, fb, kb * 128, wrow);
+                        tma_load_2d_pair(at + kABytes, &tmA, fb, kb * 128, wrow);
                     }
                     __syncwarp();
                     if (++s == S) {
@@ -795,9 +810,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     }
                 }
             }
-            if (!ok && rank == 0) {  // every issued load lands before the pair leaves
+            if (!ok) {  // every issued load lands before the pair leaves
+                // (both CTAs' loads count on the leader's barriers: the other waits its time)
+                const uint64_t dl = globaltimer() + kDrainNs;
                 const uint32_t from = issued > uint32_t(S) ? issued - S : 0;
-                for (uint32_t i = from; i < issued; ++i) drain_wait(&full[i % S], (i / S) & 1);
+                if (rank == 0)
+                    for (uint32_t i = from; i < issued; ++i) drain_wait(&full[i % S], (i / S) & 1, dl);
+                else
+                    while (globaltimer() < dl) {}
             }
         } else if (warp != 2) {
             // ------------------------------------------------------ MMA issuers
@@ -837,7 +857,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 }
                 if (elect_one()) mma_commit_pair(smem_u32(final_bar));  // every MMA above is done
                 __syncwarp();
-                drain_wait(final_bar, 0);
+                drain_wait(final_bar, 0, globaltimer() + kDrainNs);
             }
         } else if (warp == 2) {
             // ------------------------------------------------------ scales
@@ -1220,7 +1240,16 @@ hf_status launch_tiles(const Fp8Args& a, cudaStream_t st) {
     return launch_one<GLU, 32, Y16>(a, st);
 }
 
-hf_status launch_fp8_product(const Fp8Args& a, bool glu, cudaStream_t st) {
+namespace {
+std::atomic<unsigned long long> g_wait_ns{kWaitNs};
+std::atomic<int> g_stall{0};
+}  // namespace
+void set_fp8_wait(unsigned long long ns) { g_wait_ns = ns ? ns : kWaitNs; }
+void set_fp8_stall(int block) { g_stall = block; }
+
+hf_status launch_fp8_product(Fp8Args a, bool glu, cudaStream_t st) {
+    a.wait_us = int(std::min<unsigned long long>((g_wait_ns + 999) / 1000, 0xffffffffu));
+    a.stall = g_stall;
     if (glu) return launch_tiles<true, false>(a, st);
     return a.y_exp ? launch_tiles<false, true>(a, st) : launch_tiles<false, false>(a, st);
 }

@@ -150,5 +150,16 @@ def status(workspace, stream=None):
         call("hf_fp8_status", workspace.data_ptr(), s)
 
 
+def set_wait_timeout(ns: int):
+    """Limit of every bounded device wait of the products from now on (0: the default, 2 s)."""
+    call("hf_fp8_set_wait_timeout", ns)
+
+
+def debug_stall(block: int):
+    """Test hook: the products' copies stop ahead of a CTA's block-th 128 columns of K
+    (hf_fp8_debug_stall in include/hf_fp8.h); 0 turns it off."""
+    call("hf_fp8_debug_stall", block)
+
+
 __all__ = ["BLOCK", "blocks", "quantize", "gemm", "gemm_workspace_size", "moe_experts",
-           "moe_experts_workspace_size", "status", "HfError"]
+           "moe_experts_workspace_size", "status", "set_wait_timeout", "debug_stall", "HfError"]

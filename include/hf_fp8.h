@@ -87,6 +87,16 @@ HF_API hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales,
  * that call's outputs are invalid). */
 HF_API hf_status hf_fp8_status(const void* workspace, hf_stream stream);
 
+/* Limit of every bounded device wait of the products launched or captured from now
+ * on, in this process, in nanoseconds (default 2 s, 0 restores it), and a test hook
+ * (failure detection without a GPU fault): with block b > 0 the products' copies stop
+ * ahead of each CTA's b-th block of 128 columns and wait on a barrier that nothing
+ * signals (b < 0: those of every CTA pair's second CTA only, ahead of the |b|-th), so
+ * that the waits run out and hf_fp8_status reports HF_ERR_TIMEOUT. 0 turns it off.
+ * As hf_moe_set_wait_timeout and hf_moe_debug_stall, for calls without a context. */
+HF_API hf_status hf_fp8_set_wait_timeout(uint64_t ns);
+HF_API hf_status hf_fp8_debug_stall(int block);
+
 #ifdef __cplusplus
 }
 #endif
