@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < CH; ++i)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) g[i][j] = v[i][j] = 0.0f;
-            for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+            for (int kb = t.kb0; kb < t.kb1 && ok; ++kb, ++it) {
                 const uint32_t b = it % NB, sl = it % kScaleSlots;
                 if (!wait(&done[it % S], (it / S) & 1) ||
                     !wait(&sfull[sl], (it / kScaleSlots) & 1)) {
@@ -434,15 +434,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mbar_arrive(&sempty[sl]);
                 }
             }
-            if (!ok) {
-                // the half's other warps may wait at the barriers below: meet them there
-                // for this tile and the rest, so that they get to their own bounded waits
-                if (GLU)
-                    for (; u < total; u += gridDim.x) {
-                        named_bar_sync(1 + h, 128);
-                        named_bar_sync(1 + h, 128);
-                    }
-                break;
+            if (!ok) {  // gave up: NaN for this tile and the rest (and the barriers below,
+                        // where the half's other warps may wait, are met)
+#pragma unroll
+                for (int i = 0; i < CH; ++i)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) g[i][j] = v[i][j] = __uint_as_float(0x7fffffffu);
             }
             if constexpr (GLU) {
                 // silu(g) * u, and its maximum over the 128 rows per position
@@ -995,15 +992,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 sph ^= sl;
                 sl ^= 1;
             }
-            if (!ok) {
-                // the other half's warp may wait at the barriers below: meet it there
-                // for this tile and the rest, so that it gets to its own bounded waits
-                if (GLU)
-                    for (; u < total; u += step) {
-                        named_bar_sync(1 + q, 64);
-                        named_bar_sync(1 + q, 64);
-                    }
-                break;
+            if (!ok) {  // gave up: NaN for this tile and the rest (and the barriers below,
+                        // where the other half's warp may wait, are met)
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) acc[c][j] = __uint_as_float(0x7fffffffu);
             }
             const size_t row = size_t(t.row0 + rank * 128 + r);
             if constexpr (GLU) {

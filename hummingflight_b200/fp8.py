@@ -68,7 +68,7 @@ def gemm(xq, sx, wq, sw, out=None, out_dtype: str = "bf16", workspace=None, stre
     (from :func:`quantize`), wq e4m3 [N x K] with scales sw [ceil(N/128) x
     ceil(K/128)] -> [T x N] bf16 or fp32 (the type of `out` when given).
     `workspace`: uint8 scratch of gemm_workspace_size bytes, kept by callers that
-    check :func:`status`."""
+    check :func:`status`; without one a bounded wait that gave up shows as NaN only."""
     T, K = xq.shape
     N = wq.shape[0]
     dev = xq.device
@@ -106,7 +106,9 @@ def moe_experts(x, experts, scales, routing: dict, resid=None, out=None, out_dty
     experts: e4m3 [E x 3*I*H], each row one expert's [gate | up | down] block;
     scales: fp32 [E x 3*ceil(I/128)*ceil(H/128)] in the same order; routing: the
     dict of route_logits or MoELayer.route (topk_weights, offsets and perm are
-    read); resid: [T x H] of out's type, may be `out`."""
+    read); resid: [T x H] of out's type, may be `out`. `workspace`: uint8 scratch of
+    moe_experts_workspace_size bytes, kept by callers that check :func:`status`; without
+    one a bounded wait that gave up shows as NaN only."""
     T, H = x.shape
     dev = x.device
     E = experts.shape[0]
@@ -144,7 +146,7 @@ def moe_experts(x, experts, scales, routing: dict, resid=None, out=None, out_dty
 
 def status(workspace, stream=None):
     """Waits for the stream; raises HfError (HF_ERR_TIMEOUT) if the last product
-    on this workspace hit a bounded-wait timeout. The stream: that of the product,
+    on this workspace hit a bounded-wait timeout (its outputs are right or NaN). The stream: that of the product,
     by default the current one of the workspace's device."""
     with on_device(workspace.device, stream) as s:
         call("hf_fp8_status", workspace.data_ptr(), s)

@@ -83,8 +83,9 @@ HF_API hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales,
                                     size_t workspace_bytes, hf_stream stream);
 
 /* Waits for `stream` and reports whether a bounded device wait of the last
- * hf_fp8_gemm or hf_fp8_moe_experts on this workspace gave up (HF_ERR_TIMEOUT:
- * that call's outputs are invalid). */
+ * hf_fp8_gemm or hf_fp8_moe_experts on this workspace gave up (HF_ERR_TIMEOUT).
+ * Every output of such a call is right or NaN, so that it does not pass unnoticed
+ * where nobody asks. */
 HF_API hf_status hf_fp8_status(const void* workspace, hf_stream stream);
 
 /* Limit of every bounded device wait of the products launched or captured from now

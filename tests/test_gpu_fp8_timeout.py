@@ -1,6 +1,7 @@
 """The FP8 products' bounded waits run out (no GPU fault is involved: the copies stop
 and wait on a barrier that nothing signals, under a limit of 1 ms). The call returns,
-hf_fp8_status reports HF_ERR_TIMEOUT, and the next call on the workspace is right."""
+hf_fp8_status reports HF_ERR_TIMEOUT, outputs without their sum are NaN, and the next
+call on the workspace is right."""
 import contextlib
 
 import numpy as np
@@ -42,10 +43,12 @@ def run(call, ws, blocks):
     fp8.status(ws)
     for block in blocks:
         with stalled(block):
-            call()
+            bad = call()
             with pytest.raises(fp8.HfError) as e:
                 fp8.status(ws)
             assert e.value.status == 4  # HF_ERR_TIMEOUT
+            assert bad.isnan().all() if abs(block) == 1 else bad.isnan().any()
+            assert ((bad == good) | bad.isnan()).all()
         again = call()
         fp8.status(ws)
         assert torch.equal(again, good)
