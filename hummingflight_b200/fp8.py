@@ -70,7 +70,7 @@ def gemm(xq, sx, wq, sw, out=None, out_dtype: str = "bf16", workspace=None, stre
     `workspace`: uint8 scratch of gemm_workspace_size bytes, kept by callers that
     check :func:`status`; without one a bounded wait that gave up shows as NaN only."""
     T, K = xq.shape
-    N = wq.shape[0]
+    N, _ = wq.shape
     dev = xq.device
     check_tensor("xq", xq, _Q, (T, K))
     check_tensor("sx", sx, _F32, (T, blocks(K)), dev)
@@ -111,10 +111,12 @@ def moe_experts(x, experts, scales, routing: dict, resid=None, out=None, out_dty
     one a bounded wait that gave up shows as NaN only."""
     T, H = x.shape
     dev = x.device
-    E = experts.shape[0]
+    E, block = experts.shape
     w = routing["topk_weights"]
-    k = w.shape[1]
-    I = experts.shape[1] // (3 * H)
+    _, k = w.shape
+    if H == 0:
+        raise ValueError("x: rows of no columns")
+    I = block // (3 * H)
     check_tensor("x", x, _X, (T, H), rows=True)
     check_tensor("experts", experts, _Q, (E, 3 * I * H), dev)
     check_tensor("scales", scales, _F32, (E, 3 * blocks(I) * blocks(H)), dev)
