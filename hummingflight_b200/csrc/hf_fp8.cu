@@ -552,37 +552,38 @@ hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E,
                              const hf_moe_routing* r, const void* resid, void* out,
                              hf_dtype out_dtype, void* workspace, size_t workspace_bytes,
                              hf_stream stream) {
-    const std::string f("hf_fp8_moe_experts");
-    if (E < 1 || E > kMaxExperts) return fail(HF_ERR_ARG, f + ": E must be in 1..1024");
+    const auto refuse = [](const char* why) {
+        return fail(HF_ERR_ARG, std::string("hf_fp8_moe_experts: ") + why);
+    };
+    if (E < 1 || E > kMaxExperts) return refuse("E must be in 1..1024");
     if (H <= 0 || I <= 0 || H % 16 || I % 16)
-        return fail(HF_ERR_ARG, f + ": H and I must be positive multiples of 16");
+        return refuse("H and I must be positive multiples of 16");
     if (3ll * E * std::max(H, I) > kMaxExtent)
-        return fail(HF_ERR_ARG, f + ": 3 * E * max(H, I) must be at most 2^31 - 4096");
-    if (top_k < 1 || top_k > kMaxK) return fail(HF_ERR_ARG, f + ": top_k must be in 1..32");
+        return refuse("3 * E * max(H, I) must be at most 2^31 - 4096");
+    if (top_k < 1 || top_k > kMaxK) return refuse("top_k must be in 1..32");
     if (T < 0 || (long long)T * top_k > kMaxExtent)
-        return fail(HF_ERR_ARG, f + ": T >= 0 and T * top_k at most 2^31 - 4096");
+        return refuse("T >= 0 and T * top_k at most 2^31 - 4096");
     if (bad_type(x_dtype) || bad_type(out_dtype))
-        return fail(HF_ERR_ARG, f + ": x and out must be bf16 or f32");
+        return refuse("x and out must be bf16 or f32");
     if (T == 0) return HF_OK;
     if (!experts || !scales || !x || !out || !workspace || !r || !r->topk_weights || !r->offsets ||
         !r->perm)
-        return fail(HF_ERR_ARG, f + ": null pointer");
+        return refuse("null pointer");
     if (bad_rows(x, x_dtype, ldx, H))
-        return fail(HF_ERR_ARG, f + ": x and its pitch must be 16-byte aligned, the pitch at "
-                                    "least H");
+        return refuse("x and its pitch must be 16-byte aligned, the pitch at least H");
     if (!aligned16(experts) || !aligned16(out) || (resid && !aligned16(resid)))
-        return fail(HF_ERR_ARG, f + ": pointers must be 16-byte aligned");
+        return refuse("pointers must be 16-byte aligned");
     if (reinterpret_cast<uintptr_t>(workspace) % kAlign)
-        return fail(HF_ERR_ARG, f + ": workspace must be 256-byte aligned");
+        return refuse("workspace must be 256-byte aligned");
     const bool f32 = out_dtype == HF_F32;
     const ExpertsWs L = experts_ws(T, top_k, E, H, I, f32);
     if (workspace_bytes < L.total)
-        return fail(HF_ERR_ARG, f + ": workspace smaller than hf_fp8_moe_experts_workspace_size");
+        return refuse("workspace smaller than hf_fp8_moe_experts_workspace_size");
     if (resid && resid != out) {
         const uintptr_t p = reinterpret_cast<uintptr_t>(resid), q = reinterpret_cast<uintptr_t>(out);
         const uintptr_t bytes = size_t(T) * H * (f32 ? 4 : 2);
         if (p < q + bytes && q < p + bytes)
-            return fail(HF_ERR_ARG, f + ": resid and out overlap without being the same buffer");
+            return refuse("resid and out overlap without being the same buffer");
     }
     int dev = 0;
     HF_CUDA(cudaGetDevice(&dev));

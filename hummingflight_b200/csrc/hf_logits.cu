@@ -766,22 +766,23 @@ hf_status launch(const LogitArgs& a, cudaStream_t st) {
 }
 
 hf_status check_spec(const hf_route_spec* s, const char* fn) {
-    const std::string f(fn);
-    if (!s) return fail(HF_ERR_ARG, f + ": null spec");
+    const auto refuse = [&](const char* why) {
+        return fail(HF_ERR_ARG, std::string(fn) + ": " + why);
+    };
+    if (!s) return refuse("null spec");
     if (s->num_experts < 1 || s->num_experts > kMaxExperts)
-        return fail(HF_ERR_ARG, f + ": num_experts must be in 1..1024");
+        return refuse("num_experts must be in 1..1024");
     if (s->score != HF_SCORE_SIGMOID && s->score != HF_SCORE_SOFTMAX)
-        return fail(HF_ERR_ARG, f + ": score must be HF_SCORE_SIGMOID or HF_SCORE_SOFTMAX");
+        return refuse("score must be HF_SCORE_SIGMOID or HF_SCORE_SOFTMAX");
     if (s->n_group < 1 || s->n_group > kMaxRouteGroups || s->num_experts % s->n_group)
-        return fail(HF_ERR_ARG, f + ": n_group must be in 1..32 and divide num_experts");
+        return refuse("n_group must be in 1..32 and divide num_experts");
     if (s->topk_group < 1 || s->topk_group > s->n_group)
-        return fail(HF_ERR_ARG, f + ": topk_group must be in 1..n_group");
+        return refuse("topk_group must be in 1..n_group");
     if (s->group_top != 1 && s->group_top != 2)
-        return fail(HF_ERR_ARG, f + ": group_top must be 1 or 2");
+        return refuse("group_top must be 1 or 2");
     if (s->top_k < 1 || s->top_k > kMaxRouteK ||
         s->top_k > s->topk_group * (s->num_experts / s->n_group))
-        return fail(HF_ERR_ARG, f + ": top_k must be in 1..32 and at most the experts of the "
-                                    "kept groups");
+        return refuse("top_k must be in 1..32 and at most the experts of the kept groups");
     return HF_OK;
 }
 

@@ -38,7 +38,8 @@ HF_API hf_status hf_fp8_quantize(const void* x, hf_dtype x_dtype, long long ldx,
 
 /* out = (xq * sx) (wq * sw)^T over T rows:
  *   out[t, n] = sum_b sx[t, b] sw[n / 128, b] sum_{j in block b} xq[t, j] wq[n, j]
- * with products and sums in fp32. xq: device e4m3 [T x K]; sx: fp32
+ * with products and sums in fp32 (the two scales are multiplied first: their product
+ * neither overflows nor is subnormal). xq: device e4m3 [T x K]; sx: fp32
  * [T x ceil(K/128)] (any values, not only powers of two); wq: e4m3 [N x K];
  * sw: fp32 [ceil(N/128) x ceil(K/128)]; out: [T x N] of out_dtype. K a multiple
  * of 16, any T and N; xq, wq and the workspace 16-byte (workspace: 256-byte)
