@@ -1040,14 +1040,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 if constexpr (Y16) {
                     const int yb = (a.N + kYBlock - 1) / kYBlock;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        float* y = &acc[c >> 1][(c & 1) * 32];
-                        const int col = t.m0 + (c >> 1) * 128 + h * 64 + (c & 1) * 32;
-                        const uint32_t e = y_exponent(row_top(y, a.N - col));
-                        const float inv = y_inverse(e);
+                    for (int c = 0; c < 2; ++c) {
+                        const int col = t.m0 + c * 128 + h * 64;
+                        uint32_t e[2];
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) y[j] *= inv;
-                        if (rv && col < a.N) a.y_exp[size_t(p + lane) * yb + col / kYBlock] = uint8_t(e);
+                        for (int k = 0; k < 2; ++k) {
+                            float* y = &acc[c][k * 32];
+                            e[k] = y_exponent(row_top(y, a.N - col - k * 32));
+                            const float inv = y_inverse(e[k]);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) y[j] *= inv;
+                        }
+                        uint8_t* ye = a.y_exp + size_t(p + lane) * yb + col / kYBlock;
+                        if (rv && yb % 2 == 0 && col < a.N) {  // col / kYBlock is even
+                            *reinterpret_cast<uint16_t*>(ye) = uint16_t(e[0] | e[1] << 8);
+                        } else if (rv) {
+                            if (col < a.N) ye[0] = uint8_t(e[0]);
+                            if (col + 32 < a.N) ye[1] = uint8_t(e[1]);
+                        }
                     }
                 }
 #pragma unroll
