@@ -1252,7 +1252,8 @@ void set_fp8_wait(unsigned long long ns) { g_wait_ns = ns ? ns : kWaitNs; }
 void set_fp8_stall(int block) { g_stall = block; }
 
 hf_status launch_fp8_product(Fp8Args a, bool glu, cudaStream_t st) {
-    a.wait_us = int(std::min<unsigned long long>((g_wait_ns + 999) / 1000, 0xffffffffu));
+    const unsigned long long ns = g_wait_ns, us = ns / 1000 + (ns % 1000 != 0);
+    a.wait_us = int(std::min(us, 0xffffffffull));
     a.stall = g_stall;
     if (glu) return launch_tiles<true, false>(a, st);
     return a.y_exp ? launch_tiles<false, true>(a, st) : launch_tiles<false, false>(a, st);

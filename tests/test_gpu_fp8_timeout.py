@@ -113,3 +113,22 @@ def test_captured_limit_stays():
         graphs[0].replay()
         fp8.status(ws)
         assert np.array_equal(y.float().cpu().numpy(), good.float().cpu().numpy())
+
+
+@gpu
+def test_longest_limit():
+    """The largest number of nanoseconds is a long limit, not none."""
+    need_gpu()
+    from hummingflight_b200 import fp8
+    fp8.set_wait_timeout(2 ** 64 - 1)
+    try:
+        for T in (8, 300):
+            xq, sx = fp8.quantize(torch.ones((T, 6144), device="cuda"))
+            wq = torch.ones((2048, 6144), device="cuda").to(torch.float8_e4m3fn)
+            sw = torch.ones((16, 48), device="cuda")
+            ws = torch.empty(fp8.gemm_workspace_size(T, 2048, 6144), dtype=torch.uint8,
+                             device="cuda")
+            assert (fp8.gemm(xq, sx, wq, sw, out_dtype="f32", workspace=ws) == 6144).all()
+            fp8.status(ws)
+    finally:
+        fp8.set_wait_timeout(0)
