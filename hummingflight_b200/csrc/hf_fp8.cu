@@ -291,25 +291,15 @@ __device__ __forceinline__ void unpack(const uint4 v, float (&f)[4]) {
     f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y);
     f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
 }
-__device__ __forceinline__ void unpack(const uint4 v, float (&f)[8]) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        f[2 * i] = h.x;
-        f[2 * i + 1] = h.y;
-    }
-}
-
 // A thread takes 16 bytes of a token's columns, all of its picks' loads in flight
-// before the first is used. T = 4096, k = 8, H = 6144: 86 us for bf16 outputs (5.3 TB/s),
-// 149 for fp32 ones (6.1).
+// before the first is used. T = 4096, k = 8, H = 6144: 106 us for bf16 outputs (6.2 TB/s),
+// 150 for fp32 ones (6.1).
 // Y32: the expert outputs are fp32, in n planes (runs of K) that are added in order;
-// else FP16 with the factors of y_exp (kYBlock). A slot without a position in the
+// else 24 bits (Fp8Args::out_low). A slot without a position in the
 // segments [offsets[0], offsets[E]) counts as 0: its y was not written.
 template <bool Y32, bool F32, int kBatch>
 __global__ void __launch_bounds__(256, kBatch == 2 ? 8 : 4)
-    k_fp8_combine(const void* y, const uint8_t* y_exp, int n, const int32_t* pos,
+    k_fp8_combine(const void* y, const uint8_t* y_low, int n, const int32_t* pos,
                   const int32_t* perm, const int32_t* offsets, int E, const float* w, int T, int k,
                   int H, const void* resid, void* out) {
     constexpr int V = Y32 ? 4 : 8;
@@ -328,7 +318,7 @@ __global__ void __launch_bounds__(256, kBatch == 2 ? 8 : 4)
     float acc[V] = {};
     for (int j0 = 0; j0 < k; j0 += kBatch) {
         uint4 v[kBatch];
-        uint32_t ye[kBatch];
+        uint2 low[kBatch];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
             const unsigned at = __shfl_sync(~0u, p, j0 + j);
@@ -336,7 +326,7 @@ __global__ void __launch_bounds__(256, kBatch == 2 ? 8 : 4)
             v[j] = in ? ld_once_u4(static_cast<const char*>(y) + (size_t(at) * H + c) * (Y32 ? 4 : 2))
                       : make_uint4(0, 0, 0, 0);
             if constexpr (!Y32)
-                ye[j] = in ? y_exp[size_t(at) * ((H + kYBlock - 1) / kYBlock) + c / kYBlock] : 127u;
+                low[j] = in ? *reinterpret_cast<const uint2*>(y_low + size_t(at) * H + c) : make_uint2(0, 0);
         }
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
@@ -345,12 +335,10 @@ __global__ void __launch_bounds__(256, kBatch == 2 ? 8 : 4)
             const unsigned at = __shfl_sync(~0u, p, j0 + j);
             if (!((named >> (j0 + j)) & 1u)) continue;
             float f[V];
-            unpack(v[j], f);
             if constexpr (!Y32) {
-                const float s = y_factor(ye[j]);
-#pragma unroll
-                for (int e = 0; e < V; ++e) f[e] *= s;
+                unpack24(v[j], low[j], f);
             } else {
+                unpack(v[j], f);
                 for (int r = 1; r < n && c < H; ++r) {
                     float g[V];
                     unpack(ld_once_u4(static_cast<const float*>(y) +
@@ -397,7 +385,7 @@ __global__ void __launch_bounds__(256, kBatch == 2 ? 8 : 4)
     }
 }
 
-hf_status launch_fp8_combine(const void* y, const uint8_t* y_exp, int n, const int32_t* pos,
+hf_status launch_fp8_combine(const void* y, const uint8_t* y_low, int n, const int32_t* pos,
                              const int32_t* perm, const int32_t* offsets, int E, const float* w,
                              int T, int k, int H, const void* resid, void* out, bool f32,
                              cudaStream_t st) {
@@ -410,7 +398,7 @@ hf_status launch_fp8_combine(const void* y, const uint8_t* y_exp, int n, const i
     HF_CUDA(launch_pdl(f32 ? (one ? k_fp8_combine<true, true, 2> : k_fp8_combine<true, true, 8>)
                            : y32 ? (one ? k_fp8_combine<true, false, 2> : k_fp8_combine<true, false, 8>)
                                  : (one ? k_fp8_combine<false, false, 2> : k_fp8_combine<false, false, 8>),
-                       grid, dim3(256), 0, st, y, y_exp, n, pos, perm, offsets, E, w, T, k, H, resid, out));
+                       grid, dim3(256), 0, st, y, y_low, n, pos, perm, offsets, E, w, T, k, H, resid, out));
     return HF_OK;
 }
 
@@ -424,7 +412,7 @@ constexpr int kFewPositions = 512;
 struct ExpertsWs {
     Fp8Split up, down;  // runs of the gate/up and down products
     bool few;           // the gate/up product writes planes, one for each run
-    size_t pos, xq, sx, gu, mq, ms, y, ye, total;
+    size_t pos, xq, sx, gu, mq, ms, y, low, total;
 };
 
 ExpertsWs experts_ws(int T, int k, int E, int H, int I, bool f32) {
@@ -455,7 +443,7 @@ ExpertsWs experts_ws(int T, int k, int E, int H, int I, bool f32) {
     w.ms = take(n * blocks128(I) * 4);
     const bool y32 = f32 || w.down.n > 1;
     w.y = take(size_t(w.down.n) * n * H * (y32 ? 4 : 2));
-    w.ye = take(y32 ? 0 : n * ((H + kYBlock - 1) / kYBlock));
+    w.low = take(y32 ? 0 : n * H);
     w.total = o;
     return w;
 }
@@ -652,9 +640,9 @@ hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E,
     a.kbper = L.down.per;
     a.out = ws + L.y;
     a.out_f32 = f32 || L.down.n > 1;
-    a.y_exp = a.out_f32 ? nullptr : ws + L.ye;
+    a.out_low = a.out_f32 ? nullptr : ws + L.low;
     HF_TRY(launch_fp8_product(a, false, st));
-    return launch_fp8_combine(ws + L.y, ws + L.ye, L.down.n, qa.pos, r->perm, r->offsets, E,
+    return launch_fp8_combine(ws + L.y, ws + L.low, L.down.n, qa.pos, r->perm, r->offsets, E,
                               r->topk_weights, T, top_k, H, resid, out, f32, st);
 }
 
