@@ -101,10 +101,10 @@ struct Fp8Args {
     float* mid_s;
     int* err;               // error word: set when a bounded wait gives up
     int clear_err;          // the first kernel of a call clears it
-    // limit of a wait, unsigned us (set by launch_fp8_product), and the test hook: the copies
+    // limit of a wait, ns (set by launch_fp8_product), and the test hook: the copies
     // stop ahead of a CTA's stall-th block of K (0: never) and wait on a barrier that
     // nothing signals; stall < 0: those of a pair's second CTA only
-    int wait_us;
+    unsigned long long wait_ns;
     int stall;
     // 1: the launch before this one is of the same call and lets this one start only
     // after its own griddep_wait, so everything ahead of the call is done: offsets and

@@ -68,7 +68,7 @@ struct Cfg {
     // the plan: offsets and tile prefix of up to 1024 segments
     static constexpr int kStages0 = (227 * 1024 - 1024 - kFixed - 2 * 1025 * 4) / kStageBytes;
     static constexpr int kStages = kStages0 > 8 ? 8 : kStages0;
-    static_assert((2 * kStages + kBufs + 2 * kScaleSlots + 2) * 8 + 12 <= kBarBytes, "barriers");
+    static_assert((2 * kStages + kBufs + 2 * kScaleSlots + 2) * 8 + 8 <= kBarBytes, "barriers");
     static_assert(kStageBytes % 1024 == 0 && kStages >= 3, "stages");
     static int smem(int G) { return 1024 + kStages * kStageBytes + kFixed + 2 * (G + 1) * 4; }
 };
@@ -170,9 +170,20 @@ __device__ __forceinline__ void add4(float* acc, const uint32_t* d, float4 s) {
     acc[3] = fmaf(__uint_as_float(d[3]), s.w, acc[3]);
 }
 
+// What a warp that gave up leaves in place of an output.
+__device__ __forceinline__ void store_nan(const Fp8Args& a, long long row, int col) {
+    if (col >= a.N) return;
+    const size_t o = size_t(row) * a.N + col;
+    if (a.out_f32) static_cast<uint32_t*>(a.out)[o] = 0x7fffffffu;
+    else static_cast<uint16_t*>(a.out)[o] = 0x7fffu;  // bf16, or the upper half of 24 bits
+}
+
 // Y24: the outputs take Fp8Args::out_low's form. (A kernel of its own: as a branch its
 // unrolled code cost the plain form 4 us of 41 where each CTA has one tile.)
-template <bool GLU, int BN, bool Y24>
+// HOOK: Fp8Args::wait_ns and stall hold. (A kernel of its own as well: a limit that is
+// not a constant and the check of the block cost 64 x 6144 x 12288 0.8 us of 23.7, and
+// the pair kernel up to 5 %.)
+template <bool GLU, int BN, bool Y24, bool HOOK>
 __global__ void __launch_bounds__(kThreads, 1)
     k_fp8_mma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
               const Fp8Args a) {
@@ -193,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* final_bar = sempty + kScaleSlots;
     uint64_t* stall_bar = final_bar + 1;  // never signalled (test hook)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stall_bar + 1);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);  // and the limit
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* off = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(full) + C::kBarBytes);  // [G+1]
     int* pref = off + a.G + 1;                                                           // [G+1]
 
@@ -213,8 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mbar_init(final_bar, 1);
         mbar_init(stall_bar, 1);
-        abort_flag[0] = 0;
-        abort_flag[1] = a.wait_us;
+        *abort_flag = 0;
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -232,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem_base = *tmem_slot;
     const int total = pref[a.G] * (GLU ? 1 : a.nsplit);
     const auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return mbar_wait_for(smem_u32(bar), parity, abort_flag);
+        return mbar_wait_for(smem_u32(bar), parity, abort_flag, HOOK ? a.wait_ns : kWaitNs);
     };
 
     if (warp < 4) {
@@ -260,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             griddep_wait();
             griddep_launch_dependents();
-            const uint32_t stall = a.stall > 0 ? uint32_t(a.stall) - 1 : ~0u;
+            const uint32_t stall = HOOK && a.stall > 0 ? uint32_t(a.stall) - 1 : ~0u;
             bool ok = true;
             for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
                 Tile t;
@@ -268,8 +278,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int nb = (t.n + C::kBoxB - 1) / C::kBoxB;
                 for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
                     const uint32_t s = it % S;
-                    const bool st = it == stall;
-                    if (!wait(st ? stall_bar : &done[s], st ? 0 : ((it / S) & 1) ^ 1)) {
+                    if (!wait(&done[s], ((it / S) & 1) ^ 1) ||
+                        (HOOK && it == stall && !wait(stall_bar, 0))) {
                         ok = false;
                         break;
                     }
@@ -386,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < CH; ++i)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) g[i][j] = v[i][j] = 0.0f;
-            for (int kb = t.kb0; kb < t.kb1 && ok; ++kb, ++it) {
+            for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
                 const uint32_t b = it % NB, sl = it % kScaleSlots;
                 if (!wait(&done[it % S], (it / S) & 1) ||
                     !wait(&sfull[sl], (it / kScaleSlots) & 1)) {
@@ -428,12 +438,35 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mbar_arrive(&sempty[sl]);
                 }
             }
-            if (!ok) {  // gave up: NaN for this tile and the rest (and the barriers below,
-                        // where the half's other warps may wait, are met)
-#pragma unroll
-                for (int i = 0; i < CH; ++i)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) g[i][j] = v[i][j] = __uint_as_float(0x7fffffffu);
+            if (!ok) {
+                // NaN for this tile and the rest. GLU: through the maxima and scales, and
+                // the barriers below, where the half's other warps may wait, are met.
+                // (NaN in the sums and the ordinary epilogue: 64 x 6144 x 12288 24.8 us
+                // instead of 23.7, since the accumulators outlive the loop over blocks.)
+#pragma unroll 1
+                for (; u < total; u += gridDim.x) {
+                    decode<GLU, BN>(a, off, pref, KB, u, t);
+                    if constexpr (GLU) {
+                        for (int c = lane; c < BN; c += 32)
+                            if (((c >> 4) & 1) == h) red[q * BN + c] = 0x7fffffffu;
+                        named_bar_sync(1 + h, 128);
+                        for (int c = r; c < BN / 2; c += 128) {
+                            const int col = ((c >> 4) * 2 + h) * 16 + (c & 15);
+                            invs[col] = __uint_as_float(0x7fffffffu);
+                            if (col < t.n)
+                                a.mid_s[size_t(t.row0 + col) * ((a.N + 127) / 128) + t.m0 / 128] =
+                                    __uint_as_float(0x7fffffffu);
+                        }
+                        named_bar_sync(1 + h, 128);
+                    } else {
+#pragma unroll 1
+                        for (int c = h * 16; c < t.n; c += (c & 15) == 15 ? 17 : 1) {
+                            store_nan(a, t.out0 + c, t.m0 + r);
+                            store_nan(a, t.out0 + c, t.m0 + 128 + r);
+                        }
+                    }
+                }
+                break;
             }
             if constexpr (GLU) {
                 // silu(g) * u, and its maximum over the 128 rows per position
@@ -689,7 +722,7 @@ inline int pair_smem(int G) {
            2 * (G + 1) * 4;
 }
 
-template <bool GLU, bool Y24>
+template <bool GLU, bool Y24, bool HOOK>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     k_fp8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                const Fp8Args a) {
@@ -705,8 +738,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     uint64_t* final_bar = sempty + kPairSlots;
     uint64_t* stall_bar = final_bar + 1;  // never signalled (test hook)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stall_bar + 1);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);  // and the limit
-    static_assert((3 * S + 4 + 2 * kPairSlots + 2) * 8 + 12 <= kPairBar, "barriers");
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    static_assert((3 * S + 4 + 2 * kPairSlots + 2) * 8 + 8 <= kPairBar, "barriers");
     float* sc = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(full) + kPairBar);
     uint32_t* red = reinterpret_cast<uint32_t*>(sc + kPairSlots * kPairScale / 4);
     int* off = reinterpret_cast<int*>(red + 2 * 128);
@@ -731,8 +764,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         }
         mbar_init(final_bar, 2);
         mbar_init(stall_bar, 1);
-        abort_flag[0] = 0;
-        abort_flag[1] = a.wait_us;
+        *abort_flag = 0;
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -753,7 +785,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     // and the MMAs write and read shared memory, tcgen05 fences order the tensor
     // memory), so every wait orders this CTA's accesses only.
     const auto wait = [&](uint32_t bar, uint32_t parity) {
-        return mbar_wait_for(bar, parity, abort_flag);
+        return mbar_wait_for(bar, parity, abort_flag, HOOK ? a.wait_ns : kWaitNs);
     };
     const uint32_t full_at = smem_u32(full), done_at = smem_u32(done);
 
@@ -764,8 +796,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             tma_prefetch_desc(&tmA);
             tma_prefetch_desc(&tmB);
             uint32_t s = 0, ph = 1, issued = 0;
-            // (folded into a wait that is there: a wait of its own cost 5 % of the kernel)
-            const uint32_t stall = a.stall > 0 || (a.stall < 0 && rank) ? uint32_t(abs(a.stall)) - 1 : ~0u;
+            const uint32_t stall =
+                HOOK && (a.stall > 0 || (a.stall < 0 && rank)) ? uint32_t(abs(a.stall)) - 1 : ~0u;
             bool ok = true;
             for (int u = first; u < total && ok; u += step) {
                 Tile t;
@@ -776,9 +808,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 const int wrow = rank ? t.a1 : t.a0;
                 const uint32_t bytes = 2 * kABytes + (nb0 + nb1) * kPairBox * 128;
                 for (int kb = t.kb0; kb < t.kb1; ++kb, ++issued) {
-                    const bool st = issued == stall;
-                    if (!wait(st ? smem_u32(stall_bar) : done_at + s * 8, st ? 0 : ph) ||
-                        !wait(done_at + (S + s) * 8, ph)) {
+                    if (!wait(done_at + s * 8, ph) || !wait(done_at + (S + s) * 8, ph) ||
+                        (HOOK && issued == stall && !wait(smem_u32(stall_bar), 0))) {
                         ok = false;
                         break;
                     }
@@ -983,8 +1014,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 sph ^= sl;
                 sl ^= 1;
             }
-            if (!ok) {  // gave up: NaN for this tile and the rest (and the barriers below,
-                        // where the other half's warp may wait, are met)
+            if (!ok) {  // NaN for this tile and the rest (and the barriers below, where the
+                        // other half's warp may wait, are met)
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -1071,11 +1102,11 @@ int pair_grid(const void* kern, int smem, int dev) {
     return grid;
 }
 
-template <bool GLU, bool Y24>
+template <bool GLU, bool Y24, bool HOOK>
 hf_status launch_pair(const Fp8Args& a, cudaStream_t st) {
     int dev = 0;
     HF_CUDA(cudaGetDevice(&dev));
-    const auto kern = k_fp8_pair<GLU, Y24>;
+    const auto kern = k_fp8_pair<GLU, Y24, HOOK>;
     const void* kp = reinterpret_cast<const void*>(kern);
     const int smem = pair_smem(a.G);
     HF_CUDA(ensure_smem(kp, pair_smem(kMaxExperts)));
@@ -1087,12 +1118,12 @@ hf_status launch_pair(const Fp8Args& a, cudaStream_t st) {
     return HF_OK;
 }
 
-template <bool GLU, int BN, bool Y24>
+template <bool GLU, int BN, bool Y24, bool HOOK>
 hf_status launch_one(const Fp8Args& a, cudaStream_t st) {
     using C = Cfg<BN>;
     int dev = 0;
     HF_CUDA(cudaGetDevice(&dev));
-    const auto kern = k_fp8_mma<GLU, BN, Y24>;
+    const auto kern = k_fp8_mma<GLU, BN, Y24, HOOK>;
     const int smem = C::smem(a.G);
     HF_CUDA(ensure_smem(reinterpret_cast<const void*>(kern), smem));
     CUtensorMap A, B;
@@ -1208,27 +1239,32 @@ hf_status launch_fp8_gemm(const Fp8Args& args, float* planes, cudaStream_t st) {
     return HF_OK;
 }
 
-template <bool GLU, bool Y24>
+template <bool GLU, bool Y24, bool HOOK>
 hf_status launch_tiles(const Fp8Args& a, cudaStream_t st) {
     const int bn = fp8_tile_rows((a.rows + a.G - 1) / a.G);
-    if (bn == 256) return launch_pair<GLU, Y24>(a, st);
-    if (bn == 64) return launch_one<GLU, 64, Y24>(a, st);
-    return launch_one<GLU, 32, Y24>(a, st);
+    if (bn == 256) return launch_pair<GLU, Y24, HOOK>(a, st);
+    if (bn == 64) return launch_one<GLU, 64, Y24, HOOK>(a, st);
+    return launch_one<GLU, 32, Y24, HOOK>(a, st);
+}
+
+template <bool HOOK>
+hf_status launch_form(const Fp8Args& a, bool glu, cudaStream_t st) {
+    if (glu) return launch_tiles<true, false, HOOK>(a, st);
+    return a.out_low ? launch_tiles<false, true, HOOK>(a, st) : launch_tiles<false, false, HOOK>(a, st);
 }
 
 namespace {
 std::atomic<unsigned long long> g_wait_ns{kWaitNs};
 std::atomic<int> g_stall{0};
 }  // namespace
-void set_fp8_wait(unsigned long long ns) { g_wait_ns = ns ? ns : kWaitNs; }
+void set_fp8_wait(unsigned long long ns) { g_wait_ns = ns ? std::min(ns, 1ull << 62) : kWaitNs; }
 void set_fp8_stall(int block) { g_stall = block; }
 
 hf_status launch_fp8_product(Fp8Args a, bool glu, cudaStream_t st) {
-    const unsigned long long ns = g_wait_ns, us = ns / 1000 + (ns % 1000 != 0);
-    a.wait_us = int(std::min(us, 0xffffffffull));
+    a.wait_ns = g_wait_ns;
     a.stall = g_stall;
-    if (glu) return launch_tiles<true, false>(a, st);
-    return a.out_low ? launch_tiles<false, true>(a, st) : launch_tiles<false, false>(a, st);
+    return a.wait_ns != kWaitNs || a.stall ? launch_form<true>(a, glu, st)
+                                           : launch_form<false>(a, glu, st);
 }
 
 }  // namespace hf
