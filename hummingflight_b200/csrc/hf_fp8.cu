@@ -294,14 +294,16 @@ __device__ __forceinline__ void unpack(const uint4 v, float (&f)[4]) {
 // A thread takes 16 bytes of a token's columns, all of its picks' loads in flight
 // before the first is used. T = 4096, k = 8, H = 6144: 106 us for bf16 outputs (6.2 TB/s),
 // 150 for fp32 ones (6.1).
-// Y32: the expert outputs are fp32, in n planes (runs of K) that are added in order;
-// else 24 bits (Fp8Args::out_low). A slot without a position in the
+// Y: the expert outputs are fp32, in n planes (runs of K) that are added in order, or 24
+// bits or FP16 (Fp8Args::out_aux). A slot without a position in the
 // segments [offsets[0], offsets[E]) counts as 0: its y was not written.
-template <bool Y32, bool F32, int kBatch>
+enum class Y { f32, b24, f16 };
+template <Y Form, bool F32, int kBatch>
 __global__ void __launch_bounds__(256, kBatch == 2 ? 8 : 4)
-    k_fp8_combine(const void* y, const uint8_t* y_low, int n, const int32_t* pos,
+    k_fp8_combine(const void* y, const uint8_t* aux, int n, const int32_t* pos,
                   const int32_t* perm, const int32_t* offsets, int E, const float* w, int T, int k,
                   int H, const void* resid, void* out) {
+    constexpr bool Y32 = Form == Y::f32;
     constexpr int V = Y32 ? 4 : 8;
     const int t = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * V;
     // lane i: the position and weight of pick i (a slot that perm names is one it has
@@ -325,8 +327,11 @@ __global__ void __launch_bounds__(256, kBatch == 2 ? 8 : 4)
             const bool in = ((named >> (j0 + j)) & 1u) && c < H;
             v[j] = in ? ld_once_u4(static_cast<const char*>(y) + (size_t(at) * H + c) * (Y32 ? 4 : 2))
                       : make_uint4(0, 0, 0, 0);
-            if constexpr (!Y32)
-                low[j] = in ? *reinterpret_cast<const uint2*>(y_low + size_t(at) * H + c) : make_uint2(0, 0);
+            low[j] = make_uint2(0, 0);
+            if constexpr (Form == Y::b24)
+                if (in) low[j] = *reinterpret_cast<const uint2*>(aux + size_t(at) * H + c);
+            if constexpr (Form == Y::f16)
+                if (in) low[j].x = aux[size_t(at) * ((H + kYBlock - 1) / kYBlock) + c / kYBlock];
         }
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
@@ -335,8 +340,10 @@ __global__ void __launch_bounds__(256, kBatch == 2 ? 8 : 4)
             const unsigned at = __shfl_sync(~0u, p, j0 + j);
             if (!((named >> (j0 + j)) & 1u)) continue;
             float f[V];
-            if constexpr (!Y32) {
+            if constexpr (Form == Y::b24) {
                 unpack24(v[j], low[j], f);
+            } else if constexpr (Form == Y::f16) {
+                unpack16(v[j], low[j].x, f);
             } else {
                 unpack(v[j], f);
                 for (int r = 1; r < n && c < H; ++r) {
@@ -385,20 +392,16 @@ __global__ void __launch_bounds__(256, kBatch == 2 ? 8 : 4)
     }
 }
 
-hf_status launch_fp8_combine(const void* y, const uint8_t* y_low, int n, const int32_t* pos,
+template <Y Form, bool F32>
+hf_status launch_fp8_combine(const void* y, const uint8_t* aux, int n, const int32_t* pos,
                              const int32_t* perm, const int32_t* offsets, int E, const float* w,
-                             int T, int k, int H, const void* resid, void* out, bool f32,
-                             cudaStream_t st) {
-    const bool y32 = f32 || n > 1;
-    const int v = y32 ? 4 : 8;
+                             int T, int k, int H, const void* resid, void* out, cudaStream_t st) {
+    constexpr int v = Form == Y::f32 ? 4 : 8;
     // one or two picks: two loads in flight a thread, 32 registers and not 60. The whole
     // call with one expert of 16384 rows, fp32 onto fp32, us: 1170, with eight 1467
-    const bool one = k <= 2;
-    const dim3 grid(unsigned(T), unsigned((H / v + 255) / 256));
-    HF_CUDA(launch_pdl(f32 ? (one ? k_fp8_combine<true, true, 2> : k_fp8_combine<true, true, 8>)
-                           : y32 ? (one ? k_fp8_combine<true, false, 2> : k_fp8_combine<true, false, 8>)
-                                 : (one ? k_fp8_combine<false, false, 2> : k_fp8_combine<false, false, 8>),
-                       grid, dim3(256), 0, st, y, y_low, n, pos, perm, offsets, E, w, T, k, H, resid, out));
+    HF_CUDA(launch_pdl(k <= 2 ? k_fp8_combine<Form, F32, 2> : k_fp8_combine<Form, F32, 8>,
+                       dim3(unsigned(T), unsigned((H / v + 255) / 256)), dim3(256), 0, st, y, aux, n,
+                       pos, perm, offsets, E, w, T, k, H, resid, out));
     return HF_OK;
 }
 
@@ -412,7 +415,8 @@ constexpr int kFewPositions = 512;
 struct ExpertsWs {
     Fp8Split up, down;  // runs of the gate/up and down products
     bool few;           // the gate/up product writes planes, one for each run
-    size_t pos, xq, sx, gu, mq, ms, y, low, total;
+    Y form;             // of the down product's rows
+    size_t pos, xq, sx, gu, mq, ms, y, aux, total;
 };
 
 ExpertsWs experts_ws(int T, int k, int E, int H, int I, bool f32) {
@@ -441,9 +445,9 @@ ExpertsWs experts_ws(int T, int k, int E, int H, int I, bool f32) {
     w.gu = take(w.few ? size_t(w.up.n) * n * 2 * I * 4 : 0);
     w.mq = take(n * I);
     w.ms = take(n * blocks128(I) * 4);
-    const bool y32 = f32 || w.down.n > 1;
-    w.y = take(size_t(w.down.n) * n * H * (y32 ? 4 : 2));
-    w.low = take(y32 ? 0 : n * H);
+    w.form = f32 || w.down.n > 1 ? Y::f32 : fp8_pairs(int((n + E - 1) / E)) ? Y::f16 : Y::b24;
+    w.y = take(size_t(w.down.n) * n * H * (w.form == Y::f32 ? 4 : 2));
+    w.aux = take(w.form == Y::f32 ? 0 : w.form == Y::b24 ? n * H : n * ((H + kYBlock - 1) / kYBlock));
     w.total = o;
     return w;
 }
@@ -639,11 +643,15 @@ hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E,
     a.nsplit = L.down.n;
     a.kbper = L.down.per;
     a.out = ws + L.y;
-    a.out_f32 = f32 || L.down.n > 1;
-    a.out_low = a.out_f32 ? nullptr : ws + L.low;
+    a.out_f32 = L.form == Y::f32;
+    a.out_aux = a.out_f32 ? nullptr : ws + L.aux;
     HF_TRY(launch_fp8_product(a, false, st));
-    return launch_fp8_combine(ws + L.y, ws + L.low, L.down.n, qa.pos, r->perm, r->offsets, E,
-                              r->topk_weights, T, top_k, H, resid, out, f32, st);
+    const auto combine = f32                  ? launch_fp8_combine<Y::f32, true>
+                         : L.form == Y::f32   ? launch_fp8_combine<Y::f32, false>
+                         : L.form == Y::b24   ? launch_fp8_combine<Y::b24, false>
+                                              : launch_fp8_combine<Y::f16, false>;
+    return combine(ws + L.y, ws + L.aux, L.down.n, qa.pos, r->perm, r->offsets, E, r->topk_weights,
+                   T, top_k, H, resid, out, st);
 }
 
 hf_status hf_fp8_set_wait_timeout(uint64_t ns) {

@@ -175,15 +175,15 @@ __device__ __forceinline__ void store_nan(const Fp8Args& a, long long row, int c
     if (col >= a.N) return;
     const size_t o = size_t(row) * a.N + col;
     if (a.out_f32) static_cast<uint32_t*>(a.out)[o] = 0x7fffffffu;
-    else static_cast<uint16_t*>(a.out)[o] = 0x7fffu;  // bf16, or the upper half of 24 bits
+    else static_cast<uint16_t*>(a.out)[o] = 0x7fffu;  // bf16, FP16 or the upper half of 24 bits
 }
 
-// Y24: the outputs take Fp8Args::out_low's form. (A kernel of its own: as a branch its
+// AUX: the outputs take Fp8Args::out_aux's form. (A kernel of its own: as a branch its
 // unrolled code cost the plain form 4 us of 41 where each CTA has one tile.)
 // HOOK: Fp8Args::wait_ns and stall hold. (A kernel of its own as well: a limit that is
 // not a constant and the check of the block cost 64 x 6144 x 12288 0.8 us of 23.7, and
 // the pair kernel up to 5 %.)
-template <bool GLU, int BN, bool Y24, bool HOOK>
+template <bool GLU, int BN, bool AUX, bool HOOK>
 __global__ void __launch_bounds__(kThreads, 1)
     k_fp8_mma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
               const Fp8Args a) {
@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
-            } else if constexpr (Y24) {
+            } else if constexpr (AUX) {
 #pragma unroll
                 for (int i = 0; i < CH; ++i)
 #pragma unroll
@@ -527,11 +527,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                             uint16_t* y = static_cast<uint16_t*>(a.out) + o;
                             if (t.m0 + r < a.N) {
                                 y[0] = uint16_t(y0 >> 16);
-                                a.out_low[o] = uint8_t(y0 >> 8);
+                                a.out_aux[o] = uint8_t(y0 >> 8);
                             }
                             if (t.m0 + 128 + r < a.N) {
                                 y[128] = uint16_t(y1 >> 16);
-                                a.out_low[o + 128] = uint8_t(y1 >> 8);
+                                a.out_aux[o + 128] = uint8_t(y1 >> 8);
                             }
                         }
                     }
@@ -592,12 +592,29 @@ __device__ __forceinline__ void transpose4(uint4 (&c)[4]) {
     }
 }
 
+// Bits of the largest finite magnitude of the first n of 32 values.
+__device__ __forceinline__ uint32_t row_top(const float* v, int n) {
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) m = fmaxf(m, fabsf(v[j]));  // passes over NaN
+    uint32_t top = __float_as_uint(m);
+    if (top >= 0x7f800000u || n < 32) {  // Inf, or columns past the last
+        top = 0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            const uint32_t b = __float_as_uint(v[j]) & 0x7fffffffu;
+            if (j < n && b < 0x7f800000u) top = max(top, b);
+        }
+    }
+    return top;
+}
+
 // A warp's 32 x 32 block of outputs: lane l holds position row + l (of which n
 // exist), columns [col, col + 32). Rows that start on a 16-byte boundary leave
 // as 64-byte runs of four lanes, so that a store instruction touches 8 rows and
 // not 32 (which bounded the epilogue); others value by value (N = 12287 instead of
 // 12288: 777 us against 294 on 4096 x 6144, bf16).
-template <bool Y24>
+template <bool AUX>
 __device__ __forceinline__ void store32(const Fp8Args& a, long long row, int n, int col,
                                         const float* v) {
     const int lane = threadIdx.x & 31, size = a.out_f32 ? 4 : 2;
@@ -620,8 +637,9 @@ __device__ __forceinline__ void store32(const Fp8Args& a, long long row, int n, 
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const float lo = v[8 * j + 2 * k], hi = v[8 * j + 2 * k + 1];
-                        if constexpr (Y24) {
-                            w[k] = upper_halves(lo, hi);
+                        if constexpr (AUX) {
+                            const __half2 b = __floats2half2_rn(lo, hi);
+                            w[k] = *reinterpret_cast<const uint32_t*>(&b);
                         } else {
                             const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
                             w[k] = *reinterpret_cast<const uint32_t*>(&b);
@@ -645,38 +663,9 @@ __device__ __forceinline__ void store32(const Fp8Args& a, long long row, int n, 
         for (int j = 0; j < 32; ++j)
             if (col + j < a.N) {
                 if (a.out_f32) reinterpret_cast<float*>(base)[j] = v[j];
-                else if constexpr (Y24) reinterpret_cast<uint16_t*>(base)[j] = uint16_t(__float_as_uint(v[j]) >> 16);
+                else if constexpr (AUX) reinterpret_cast<__half*>(base)[j] = __float2half_rn(v[j]);
                 else reinterpret_cast<__nv_bfloat16*>(base)[j] = __float2bfloat16_rn(v[j]);
             }
-    }
-}
-
-// The third bytes of 64 columns (Fp8Args::out_low), in the same runs.
-__device__ __forceinline__ void store_low64(const Fp8Args& a, long long row, int n, int col,
-                                            const float* v) {
-    const int lane = threadIdx.x & 31;
-    uint8_t* base = a.out_low + row * a.N + col;
-    if (col + 64 <= a.N && a.N % 16 == 0) {
-        uint4 c[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float* f = v + 16 * j;
-            c[j] = make_uint4(third_bytes(f[0], f[1], f[2], f[3]), third_bytes(f[4], f[5], f[6], f[7]),
-                              third_bytes(f[8], f[9], f[10], f[11]),
-                              third_bytes(f[12], f[13], f[14], f[15]));
-        }
-        transpose4(c);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int r = (lane & ~3) + j;
-            if (r < n)
-                *reinterpret_cast<uint4*>(base + (long long)r * a.N + (lane & 3) * 16) = c[j];
-        }
-    } else if (lane < n) {
-        base += (long long)lane * a.N;
-#pragma unroll
-        for (int j = 0; j < 64; ++j)
-            if (col + j < a.N) base[j] = uint8_t(__float_as_uint(v[j]) >> 8);
     }
 }
 
@@ -722,7 +711,7 @@ inline int pair_smem(int G) {
            2 * (G + 1) * 4;
 }
 
-template <bool GLU, bool Y24, bool HOOK>
+template <bool GLU, bool AUX, bool HOOK>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     k_fp8_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                const Fp8Args a) {
@@ -1059,14 +1048,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     if (r0 + j < n && col < left) *reinterpret_cast<uint4*>(y + size_t(j) * a.N) = o[j];
             } else if (work) {
                 const long long p = t.out0 + rank * 128 + q * 32;
+                if constexpr (AUX) {
+                    const int yb = (a.N + kYBlock - 1) / kYBlock;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int col = t.m0 + c * 128 + h * 64;
+                        uint32_t e[2];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            float* y = &acc[c][k * 32];
+                            e[k] = y_exponent(row_top(y, a.N - col - k * 32));
+                            const float inv = y_inverse(e[k]);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) y[j] *= inv;
+                        }
+                        // two together (a byte each touched as many sectors again: 670 us
+                        // instead of 636)
+                        uint8_t* ye = a.out_aux + size_t(p + lane) * yb + col / kYBlock;
+                        if (rv && yb % 2 == 0 && col < a.N) {  // col / kYBlock is even
+                            *reinterpret_cast<uint16_t*>(ye) = uint16_t(e[0] | e[1] << 8);
+                        } else if (rv) {
+                            if (col < a.N) ye[0] = uint8_t(e[0]);
+                            if (col + 32 < a.N) ye[1] = uint8_t(e[1]);
+                        }
+                    }
+                }
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    store32<Y24>(a, p, n - q * 32, t.m0 + (c >> 1) * 128 + h * 64 + (c & 1) * 32,
+                    store32<AUX>(a, p, n - q * 32, t.m0 + (c >> 1) * 128 + h * 64 + (c & 1) * 32,
                                  &acc[c >> 1][(c & 1) * 32]);
-                if constexpr (Y24)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-                        store_low64(a, p, n - q * 32, t.m0 + c * 128 + h * 64, acc[c]);
             }
         }
     }
@@ -1102,11 +1112,11 @@ int pair_grid(const void* kern, int smem, int dev) {
     return grid;
 }
 
-template <bool GLU, bool Y24, bool HOOK>
+template <bool GLU, bool AUX, bool HOOK>
 hf_status launch_pair(const Fp8Args& a, cudaStream_t st) {
     int dev = 0;
     HF_CUDA(cudaGetDevice(&dev));
-    const auto kern = k_fp8_pair<GLU, Y24, HOOK>;
+    const auto kern = k_fp8_pair<GLU, AUX, HOOK>;
     const void* kp = reinterpret_cast<const void*>(kern);
     const int smem = pair_smem(a.G);
     HF_CUDA(ensure_smem(kp, pair_smem(kMaxExperts)));
@@ -1118,12 +1128,12 @@ hf_status launch_pair(const Fp8Args& a, cudaStream_t st) {
     return HF_OK;
 }
 
-template <bool GLU, int BN, bool Y24, bool HOOK>
+template <bool GLU, int BN, bool AUX, bool HOOK>
 hf_status launch_one(const Fp8Args& a, cudaStream_t st) {
     using C = Cfg<BN>;
     int dev = 0;
     HF_CUDA(cudaGetDevice(&dev));
-    const auto kern = k_fp8_mma<GLU, BN, Y24, HOOK>;
+    const auto kern = k_fp8_mma<GLU, BN, AUX, HOOK>;
     const int smem = C::smem(a.G);
     HF_CUDA(ensure_smem(reinterpret_cast<const void*>(kern), smem));
     CUtensorMap A, B;
@@ -1239,18 +1249,18 @@ hf_status launch_fp8_gemm(const Fp8Args& args, float* planes, cudaStream_t st) {
     return HF_OK;
 }
 
-template <bool GLU, bool Y24, bool HOOK>
+template <bool GLU, bool AUX, bool HOOK>
 hf_status launch_tiles(const Fp8Args& a, cudaStream_t st) {
     const int bn = fp8_tile_rows((a.rows + a.G - 1) / a.G);
-    if (bn == 256) return launch_pair<GLU, Y24, HOOK>(a, st);
-    if (bn == 64) return launch_one<GLU, 64, Y24, HOOK>(a, st);
-    return launch_one<GLU, 32, Y24, HOOK>(a, st);
+    if (bn == 256) return launch_pair<GLU, AUX, HOOK>(a, st);
+    if (bn == 64) return launch_one<GLU, 64, AUX, HOOK>(a, st);
+    return launch_one<GLU, 32, AUX, HOOK>(a, st);
 }
 
 template <bool HOOK>
 hf_status launch_form(const Fp8Args& a, bool glu, cudaStream_t st) {
     if (glu) return launch_tiles<true, false, HOOK>(a, st);
-    return a.out_low ? launch_tiles<false, true, HOOK>(a, st) : launch_tiles<false, false, HOOK>(a, st);
+    return a.out_aux ? launch_tiles<false, true, HOOK>(a, st) : launch_tiles<false, false, HOOK>(a, st);
 }
 
 namespace {

@@ -109,8 +109,9 @@ def test_fp32_outputs_are_exact(i):
 @pytest.mark.parametrize("i", range(len(SIZES)))
 def test_bf16_outputs_are_rounded_once(i, shift):
     """The residual takes nearly all of the sum away, so that what the expert outputs
-    lost before the sum shows: less than a step of 16 significant bits each, then half a
-    step of bf16 of what is left (2 (k + 2) half steps of fp32 for the sum)."""
+    lost before the sum shows: less than a step of 16 significant bits each, or half a
+    step of FP16 where there are many positions, then half a step of bf16 of what is left
+    (2 (k + 2) half steps of fp32 for the sum)."""
     need_gpu()
     from hummingflight_b200 import fp8
     T, E, k, H, I = SIZES[i]
@@ -121,7 +122,7 @@ def test_bf16_outputs_are_rounded_once(i, shift):
     xg, q, s, r = to_gpu(x, blocks, routing)
     out = fp8.moe_experts(xg, q, s, r, resid.cuda()).double().cpu().numpy()
     lost = np.abs(wy).sum(1)
-    tol = (2.0 ** -15 + 2 * (k + 2) * R.U) * lost
+    tol = (2.0 ** (-15 if T * k <= 96 * E else -11) + 2 * (k + 2) * R.U) * lost
     assert (np.abs(out - ref) <= tol + 2.0 ** -8 * (np.abs(ref) + tol)).all()
 
 
