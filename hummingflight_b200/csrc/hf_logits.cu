@@ -25,7 +25,7 @@
 // second launch adds the counts of the blocks before its own.
 //
 // 16384 tokens, E = 256, k = 8, bias: 30.6 us, of which routing 21 to 25, bound by
-// issue slots (822 instructions a token, 61 % of the slots used; the rounds of the
+// issue slots (825 instructions a token, 61 % of the slots used; the rounds of the
 // choice are the largest part). The logits' 16.8 MB would take 2.6.
 #include "hf_internal.cuh"
 
