@@ -292,11 +292,11 @@ __device__ __forceinline__ void unpack(const uint4 v, float (&f)[4]) {
     f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
 }
 // A thread takes 16 bytes of a token's columns, all of its picks' loads in flight
-// before the first is used. T = 4096, k = 8, H = 6144: 106 us for bf16 outputs (6.2 TB/s),
-// 150 for fp32 ones (6.1).
+// before the first is used. T = 16384, k = 8, H = 6144: 369 us for bf16 outputs (5.0 TB/s),
+// 602 for fp32 ones (6.0).
 // Y: the expert outputs are fp32, in n planes (runs of K) that are added in order, or 24
-// bits or FP16 (Fp8Args::out_aux). A slot without a position in the
-// segments [offsets[0], offsets[E]) counts as 0: its y was not written.
+// bits or FP16 (Fp8Args::out_aux). A slot without a position in the segments [offsets[0],
+// offsets[E]) counts as 0: its y was not written.
 enum class Y { f32, b24, f16 };
 template <Y Form, bool F32, int kBatch>
 __global__ void __launch_bounds__(256, kBatch == 2 ? 8 : 4)
