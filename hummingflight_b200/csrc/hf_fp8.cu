@@ -291,6 +291,7 @@ __device__ __forceinline__ void unpack(const uint4 v, float (&f)[4]) {
     f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y);
     f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
 }
+
 // A thread takes 16 bytes of a token's columns, all of its picks' loads in flight
 // before the first is used. T = 16384, k = 8, H = 6144: 369 us for bf16 outputs (5.0 TB/s),
 // 602 for fp32 ones (6.0).
@@ -646,10 +647,10 @@ hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E,
     a.out_f32 = L.form == Y::f32;
     a.out_aux = a.out_f32 ? nullptr : ws + L.aux;
     HF_TRY(launch_fp8_product(a, false, st));
-    const auto combine = f32                  ? launch_fp8_combine<Y::f32, true>
-                         : L.form == Y::f32   ? launch_fp8_combine<Y::f32, false>
-                         : L.form == Y::b24   ? launch_fp8_combine<Y::b24, false>
-                                              : launch_fp8_combine<Y::f16, false>;
+    const auto combine = f32                ? launch_fp8_combine<Y::f32, true>
+                         : L.form == Y::f32 ? launch_fp8_combine<Y::f32, false>
+                         : L.form == Y::b24 ? launch_fp8_combine<Y::b24, false>
+                                            : launch_fp8_combine<Y::f16, false>;
     return combine(ws + L.y, ws + L.aux, L.down.n, qa.pos, r->perm, r->offsets, E, r->topk_weights,
                    T, top_k, H, resid, out, st);
 }

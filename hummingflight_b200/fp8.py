@@ -148,8 +148,8 @@ def moe_experts(x, experts, scales, routing: dict, resid=None, out=None, out_dty
 
 def status(workspace, stream=None):
     """Waits for the stream; raises HfError (HF_ERR_TIMEOUT) if the last product
-    on this workspace hit a bounded-wait timeout (its outputs are right or NaN). The stream: that of the product,
-    by default the current one of the workspace's device."""
+    on this workspace hit a bounded-wait timeout (its outputs are right or NaN). The
+    stream: that of the product, by default the current one of the workspace's device."""
     with on_device(workspace.device, stream) as s:
         call("hf_fp8_status", workspace.data_ptr(), s)
 

@@ -67,16 +67,16 @@ HF_API hf_status hf_fp8_gemm(const uint8_t* xq, const float* sx, const uint8_t* 
  * the routed ones is left out; topk_ids is not read). offsets do not decrease and
  * perm names a slot once at most; entries out of range are clipped (offsets) or
  * skipped (perm), and a slot that perm does not name, or at a position outside
- * [offsets[0], offsets[E]), adds nothing to its token. resid: device [T x H] of out_dtype or NULL, may be out
- * itself. out: device [T x H] of out_dtype; until the combine the expert outputs
- * y_i are kept in fp32 for fp32 outputs, and for bf16 ones with 16 significant
- * bits (the rest of the fp32 number cut off) or, from a mean of 97 positions an expert
- * on, in FP16 times a power of two per 32 columns (11 significant bits down to 2^-28 of
- * a block's largest). The
- * shared expert, or a dense MLP, is the call with E = 1, k = 1 and the routed
- * output as resid. H and I multiples of 16, k in 1..32, E in 1..1024, T * k and
- * 3 * E * max(H, I) at most 2^31 - 4096; pointers 16-byte aligned, the workspace
- * 256-byte. A workspace serves any number of layers in stream order. */
+ * [offsets[0], offsets[E]), adds nothing to its token. resid: device [T x H] of
+ * out_dtype or NULL, may be out itself. out: device [T x H] of out_dtype; until the
+ * combine the expert outputs y_i are kept in fp32 for fp32 outputs, and for bf16
+ * ones with 16 significant bits (the rest of the fp32 number cut off) or, from a
+ * mean of 97 positions an expert on, in FP16 times a power of two per 32 columns
+ * (11 significant bits down to 2^-28 of a block's largest). The shared expert, or a
+ * dense MLP, is the call with E = 1, k = 1 and the routed output as resid. H and I
+ * multiples of 16, k in 1..32, E in 1..1024, T * k and 3 * E * max(H, I) at most
+ * 2^31 - 4096; pointers 16-byte aligned, the workspace 256-byte. A workspace serves
+ * any number of layers in stream order. */
 HF_API size_t hf_fp8_moe_experts_workspace_size(int T, int top_k, int E, int H, int I,
                                                 hf_dtype out_dtype);
 HF_API hf_status hf_fp8_moe_experts(const uint8_t* experts, const float* scales, int E, int H,
